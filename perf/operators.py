@@ -125,12 +125,15 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------ plain forms
+TAG = 0x44524F50  # the counter's second word: these numbers meet none that the sampler draws under the same seed
+
+
 def _keep(case, s):
     """Which elements stay: Philox-4x32-10 in whole numbers of 64 bits, one block of four words for eight neighbours of a row."""
     m, n, low = case["m"], case["n"], 0xFFFFFFFF
     block = torch.arange((n + 7) // 8, device="cuda").expand(m, -1)
     row = (torch.arange(m, device="cuda") + s["first_row"])[:, None].expand(-1, block.shape[1])
-    c0, c1, c2, c3 = block, torch.zeros_like(block), row & low, row >> 32
+    c0, c1, c2, c3 = block, torch.full_like(block, TAG), row & low, row >> 32
     k0, k1 = s["seed"] & low, s["seed"] >> 32
     for _ in range(10):
         p0, p1 = c0 * 0xD2511F53, c2 * 0xCD9E8D57
@@ -282,7 +285,7 @@ def _exact_factor(case, s):
     rows = np.arange(m, dtype=np.uint64) + np.uint64(s["first_row"])
     shape = (m, (n + 7) // 8)
     word = lambda a: np.ascontiguousarray(np.broadcast_to(a, shape)).astype(np.uint32)  # noqa: E731
-    ctr = [word(np.arange(shape[1])[None]), word(0), word((rows & np.uint64(0xFFFFFFFF))[:, None]), word((rows >> np.uint64(32))[:, None])]
+    ctr = [word(np.arange(shape[1])[None]), word(TAG), word((rows & np.uint64(0xFFFFFFFF))[:, None]), word((rows >> np.uint64(32))[:, None])]
     key = [s["seed"] % 2 ** 32, s["seed"] // 2 ** 32]
     for r in range(10):
         a, b = ctr[0].astype(np.uint64) * np.uint64(0xD2511F53), ctr[2].astype(np.uint64) * np.uint64(0xCD9E8D57)
