@@ -253,6 +253,81 @@ int veex_band_outside_counts(const float* z, int N, int L, int nb, const double*
                              veexStream_t s);
 
 /* ------------------------------------------------------------------------------------------
+ * Dense-trunk operators: a Dense layer with its epilogue, dropout, and the normalised residual step -- what a user
+ * composes a dense residual network from beside the convolution layers above.  Data of all tensors of a call has one
+ * type (VEEX_T_*); all sums and statistics are fp32.  Rows are row-major and unpadded except where a stride is given.
+ * No reference call site beyond keras.layers.Dense (models.py:238-241,264).
+ * ---------------------------------------------------------------------------------------- */
+#define VEEX_T_F32 0
+#define VEEX_T_BF16 1
+#define VEEX_T_F16 2
+
+/* Inverted dropout: y[r][c] = residual[r][c] + keep(r, c) x[r][c] 65536 / (65536 - cut), cut = rint(rate * 65536), keep =
+ * (16-bit number of (r, c) >= cut).  The number is half word c & 1 of word (c & 7) >> 1 of Philox-4x32-10 with key = seed and
+ * counter (c >> 3, 0x44524F50, row low, row high), row = first_row + counter[0] + r: it does not depend on how a batch is
+ * split over calls.  The mask is never stored: the backward pass is the same call on dy without residual.  residual and
+ * counter (a DEVICE word read when the kernel runs) may be NULL; y may be x. */
+int veex_dropout(const void* x, const void* residual, void* y, long long rows, int cols, int dtype, double rate,
+                 unsigned long long seed, unsigned long long first_row, const unsigned long long* counter, veexStream_t s);
+
+#define VEEX_ACT_NONE 0
+#define VEEX_ACT_RELU 1
+#define VEEX_ACT_GELU 2    /* z Phi(z), erf form */
+#define VEEX_ACT_SILU 3
+#define VEEX_ACT_SIGMOID 4
+
+/* y = residual + D(act(x w + bias)): x [rows][k] (row stride ldx elements), w [k][n] (Keras Dense layout), D = dropout as
+ * veex_dropout draws it over y's rows and columns (rate 0: none).  bias, residual, pre may be NULL.
+ * Forward writes y, and what the backward pass needs of z = x w + bias into pre when that is not NULL.
+ * Backward: dz = D'(dy) act'(z), dx = dz w^T, dw = x^T dz, db = column sums of dz; each of dx, dw, db may be NULL.  pre is what
+ * the forward wrote there; for VEEX_ACT_RELU without residual it may be the forward's y instead (y > 0 exactly where an element
+ * was kept and z > 0), for VEEX_ACT_NONE it is not read.  d(residual) is dy.
+ * Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned,
+ * of at least the bytes that the _workspace function of the direction returns for the same struct (host only; -1: bad). */
+typedef struct VeexDense {
+  const void* x; const void* w; const void* bias; const void* residual;
+  void* y; void* pre;
+  const void* dy; void* dx; void* dw; void* db;
+  void* workspace; long long workspace_bytes;
+  long long rows, ldx;
+  int32_t k, n, dtype, activation;
+  double rate;
+  unsigned long long seed, first_row;
+  const unsigned long long* counter;
+  int32_t struct_size, reserved;
+} VeexDense;
+long long veex_dense_fwd_workspace_bytes(const VeexDense* d);
+int veex_dense_fwd(const VeexDense* d, veexStream_t s);
+long long veex_dense_bwd_workspace_bytes(const VeexDense* d);
+int veex_dense_bwd(const VeexDense* d, veexStream_t s);
+
+#define VEEX_NORM_LAYER 0
+#define VEEX_NORM_RMS 1
+#define VEEX_NORM_MAX_COLS 16384
+
+/* x_out = x + scale gate Norm(h; post_w, post_b), u = Norm(x_out; pre_w, pre_b); with h NULL: u = Norm(x; pre_w, pre_b).
+ * Norm: (v - mean) / sqrt(var + eps) * w + b over the row (LAYER), v / sqrt(mean(v^2) + eps) * w + b (RMS); NULL weights
+ * and biases are 1 and 0.  gate [groups][cols], row g for rows/groups consecutive rows of x; scale [cols]; both may be NULL (1).
+ * stats [rows][4] fp32: written by the forward when not NULL, read by the backward.
+ * Backward: gradients of whatever output pointer is not NULL, from dx_out and du (NULL: zero); workspace of
+ * veex_residual_norm_bwd_workspace_floats(rows, cols, groups) floats (groups = 1 without gate or h); rows >= 1. */
+typedef struct VeexResidualNorm {
+  const void* x; const void* h; const void* gate; const void* scale;
+  const void* post_w; const void* post_b; const void* pre_w; const void* pre_b;
+  void* x_out; void* u; float* stats;
+  const void* dx_out; const void* du;
+  void* dx; void* dh; void* dgate; void* dscale; void* dpost_w; void* dpost_b; void* dpre_w; void* dpre_b;
+  float* workspace; long long workspace_floats;
+  long long rows, groups;
+  int32_t cols, dtype, kind;
+  float eps;
+  int32_t struct_size, reserved;
+} VeexResidualNorm;
+int veex_residual_norm_fwd(const VeexResidualNorm* d, veexStream_t s);
+long long veex_residual_norm_bwd_workspace_floats(long long rows, int cols, long long groups);
+int veex_residual_norm_bwd(const VeexResidualNorm* d, veexStream_t s);
+
+/* ------------------------------------------------------------------------------------------
  * Network level: the whole Encoder / Decoder / VAE.train_step graph as one enqueue.
  * ---------------------------------------------------------------------------------------- */
 typedef struct VeexNet VeexNet; /* host-side plan only; owns no device memory */

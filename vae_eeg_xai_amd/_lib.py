@@ -53,6 +53,36 @@ class WgradDesc(C.Structure):
     ]
 
 
+class DenseDesc(C.Structure):
+    """struct VeexDense (include/veex.h)."""
+    _fields_ = [
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p),
+        ("y", C.c_void_p), ("pre", C.c_void_p),
+        ("dy", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("db", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
+        ("rows", C.c_longlong), ("ldx", C.c_longlong),
+        ("k", C.c_int32), ("n", C.c_int32), ("dtype", C.c_int32), ("activation", C.c_int32),
+        ("rate", C.c_double), ("seed", C.c_ulonglong), ("first_row", C.c_ulonglong), ("counter", C.c_void_p),
+        ("struct_size", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class ResidualNormDesc(C.Structure):
+    """struct VeexResidualNorm (include/veex.h)."""
+    _fields_ = [
+        ("x", C.c_void_p), ("h", C.c_void_p), ("gate", C.c_void_p), ("scale", C.c_void_p),
+        ("post_w", C.c_void_p), ("post_b", C.c_void_p), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p),
+        ("x_out", C.c_void_p), ("u", C.c_void_p), ("stats", C.c_void_p),
+        ("dx_out", C.c_void_p), ("du", C.c_void_p),
+        ("dx", C.c_void_p), ("dh", C.c_void_p), ("dgate", C.c_void_p), ("dscale", C.c_void_p),
+        ("dpost_w", C.c_void_p), ("dpost_b", C.c_void_p), ("dpre_w", C.c_void_p), ("dpre_b", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_floats", C.c_longlong),
+        ("rows", C.c_longlong), ("groups", C.c_longlong),
+        ("cols", C.c_int32), ("dtype", C.c_int32), ("kind", C.c_int32), ("eps", C.c_float),
+        ("struct_size", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 _P, _I, _L, _F, _U, _D = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_ulonglong, C.c_double
 
 # name -> (restype, argtypes); every symbol include/veex.h declares
@@ -103,6 +133,14 @@ SIGNATURES = {
     "veex_column_quantiles": (_I, [_P, _I, _I, C.POINTER(_D), _I, _P, _P, _P]),
     "veex_column_medians": (_I, [_P, _I, _I, _P, _P, _P]),
     "veex_band_outside_counts": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),
+    "veex_dropout": (_I, [_P, _P, _P, _L, _I, _I, _D, _U, _U, _P, _P]),
+    "veex_dense_fwd_workspace_bytes": (_L, [C.POINTER(DenseDesc)]),
+    "veex_dense_fwd": (_I, [C.POINTER(DenseDesc), _P]),
+    "veex_dense_bwd_workspace_bytes": (_L, [C.POINTER(DenseDesc)]),
+    "veex_dense_bwd": (_I, [C.POINTER(DenseDesc), _P]),
+    "veex_residual_norm_fwd": (_I, [C.POINTER(ResidualNormDesc), _P]),
+    "veex_residual_norm_bwd_workspace_floats": (_L, [_L, _I, _L]),
+    "veex_residual_norm_bwd": (_I, [C.POINTER(ResidualNormDesc), _P]),
     "veex_net_create": (_P, [_I, _I]),
     "veex_net_destroy": (None, [_P]),
     "veex_net_param_floats": (_L, [_P]),

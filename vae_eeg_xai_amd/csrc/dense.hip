@@ -1,0 +1,425 @@
+// The Dense layer of a trunk:  y = residual + D(act(x w + b))  and its gradients  dz = D'(dy) act'(z), dx = dz w^T,
+// dw = x^T dz, db = column sums of dz.  x [M][K], w [K][N] (Keras layout), types fp32 / bf16 / fp16, sums in fp32.
+//
+// This file: the general product (any strides, alignment and size), the join of a split reduction, the dz / db pass, and
+// the host side.
+#include "dense_common.h"
+#include <algorithm>
+
+// ---------------------------------------------------------------------------------------------------------------
+// The general product: 64 x 64 tiles, 4 waves of one 32 x 32 accumulator, fp32 MFMA (a product of two 16-bit numbers is exact
+// there, so one kernel serves every type).  Operand tiles are staged through registers into [k][row] LDS; a tensor whose rows
+// are whole aligned pieces loads 8 elements at a time, others element by element.  The MFMA takes B's rows as its first operand, so
+// that a lane ends up with 4 consecutive columns of one row: one store, one block of dropout numbers.
+// ---------------------------------------------------------------------------------------------------------------
+#define DG_LD 68     // floats per LDS row: 64 + one 16-byte piece
+
+template <typename T, bool KC>
+__device__ __forceinline__ void dg_load(float (&r)[8], const DenseOperand& o, long long row0, long long rows, long long k0,
+                                        long long k_end, bool vec) {
+  // KC: k is the contiguous index: 4 threads a row, 8 k each; else the row index is: 8 threads a k, 8 rows each
+  const int t = threadIdx.x;
+  const T* p = static_cast<const T*>(o.p);
+  const long long row = row0 + (KC ? t >> 2 : 8 * (t & 7)), k = k0 + (KC ? 8 * (t & 3) : t >> 3);
+  const long long n = (row < rows && k < k_end) ? (KC ? k_end - k : rows - row) : 0;
+  const T* q = p + row * o.row_stride + k * o.k_stride;
+  if (vec && n >= 8) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 8 / V; ++c) {
+      const Piece<T, V> x = piece_load<T, V>(q + c * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) r[c * V + e] = (float)x.v[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = e < n ? (float)q[e] : 0.f;
+  }
+}
+template <bool KC>
+__device__ __forceinline__ void dg_store(float* s, const float (&r)[8]) {
+  const int t = threadIdx.x;
+  if (KC) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[(8 * (t & 3) + e) * DG_LD + (t >> 2)] = r[e];
+  } else {
+    float4* d = reinterpret_cast<float4*>(s + (t >> 3) * DG_LD + 8 * (t & 7));
+    d[0] = make_float4(r[0], r[1], r[2], r[3]);
+    d[1] = make_float4(r[4], r[5], r[6], r[7]);
+  }
+}
+
+template <typename T, bool AKC, bool BKC, bool SPLIT>
+__global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
+  __shared__ float As[2][32 * DG_LD], Bs[2][32 * DG_LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l31 = lane & 31, lh = lane >> 5, wi = wave & 1, wj = wave >> 1;
+  const int tiles_j = (g.J + 63) / 64;
+  const long long ti = blockIdx.x / tiles_j;
+  const long long i0 = ti * 64;
+  const int j0 = (int)(blockIdx.x - ti * tiles_j) * 64;
+  const long long k_begin = (long long)blockIdx.y * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
+
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  float ra[8], rb[8];
+  dg_load<T, AKC>(ra, g.a, i0, g.I, k_begin, k_end, g.vec_a);
+  dg_load<T, BKC>(rb, g.b, j0, g.J, k_begin, k_end, g.vec_b);
+  int cur = 0;
+  for (long long k0 = k_begin; k0 < k_end; k0 += 32, cur ^= 1) {
+    dg_store<AKC>(As[cur], ra);
+    dg_store<BKC>(Bs[cur], rb);
+    __syncthreads();      // (the other buffer's readers passed the barrier of the turn before)
+    if (k0 + 32 < k_end) {
+      dg_load<T, AKC>(ra, g.a, i0, g.I, k0 + 32, k_end, g.vec_a);
+      dg_load<T, BKC>(rb, g.b, j0, g.J, k0 + 32, k_end, g.vec_b);
+    }
+#pragma unroll
+    for (int s = 0; s < 16; ++s)
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Bs[cur][(2 * s + lh) * DG_LD + wj * 32 + l31],
+                                                 As[cur][(2 * s + lh) * DG_LD + wi * 32 + l31], acc, 0, 0, 0);
+  }
+  const long long i = i0 + wi * 32 + l31;
+  if (i >= g.I) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int j = j0 + wj * 32 + 8 * q + 4 * lh;
+    if (j >= g.J) continue;
+    float v[4] = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    if (SPLIT) {
+      float* s = g.slab + ((long long)blockIdx.y * g.I + i) * g.J + j;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < g.J) s[e] = v[e];
+    } else {
+      unsigned w[4] = {0u, 0u, 0u, 0u};
+      if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
+      dense_epilogue<T, 4>(g.epi, v, i, j, g.J, g.vec_e, w + (lh ? 2 : 0));
+    }
+  }
+}
+
+// Sum of the slabs in order, then the epilogue: 8 columns of one row a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
+  const int bpr = (g.J + 7) / 8;
+  const long long nb = g.I * bpr;
+  for (long long b = (long long)blockIdx.x * 256 + threadIdx.x; b < nb; b += (long long)gridDim.x * 256) {
+    const long long i = nb <= 0xFFFFFFFFll ? (long long)((unsigned)b / (unsigned)bpr) : b / bpr;
+    const int j = 8 * (int)(b - i * bpr);
+    const float* s = g.slab + i * g.J + j;
+    const long long stride = g.I * g.J;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (g.J % 4 == 0) {
+#pragma unroll 4
+      for (int z = 0; z < g.splits; ++z) {
+        const float4 x = *reinterpret_cast<const float4*>(s + z * stride);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        if (j + 4 < g.J) {
+          const float4 t = *reinterpret_cast<const float4*>(s + z * stride + 4);
+          v[4] += t.x; v[5] += t.y; v[6] += t.z; v[7] += t.w;
+        }
+      }
+    } else {
+      for (int z = 0; z < g.splits; ++z)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e < g.J) v[e] += s[z * stride + e];
+    }
+    unsigned w[4] = {0u, 0u, 0u, 0u};
+    if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
+    dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e && g.J % 8 == 0, w);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dz = D'(dy) act'(z) and the partial column sums of it (fp32, before dz is rounded): 256 columns a block as 32 threads of 8
+// columns, 8 rows at a time; each block adds a run of rows up and writes one partial row.
+// ---------------------------------------------------------------------------------------------------------------
+struct DenseDz {
+  const void *dy, *pre;
+  void* dz;              // null: only the sums
+  float* part;           // [chunks][N], null: none
+  long long rows, rows_per_chunk;
+  int n, act, vec;
+  DropArgs drop;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float s[8][256];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int j = blockIdx.x * 256 + 8 * tx, n = min(8, p.n - j);
+  const long long first = (long long)blockIdx.y * p.rows_per_chunk, last = min(p.rows, first + p.rows_per_chunk);
+  const unsigned long long base = drop_base(p.drop);
+  float sum[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+  if (n > 0) {
+    for (long long i = first + ty; i < last; i += 8) {
+      const long long at = i * p.n + j;
+      const T* dy = static_cast<const T*>(p.dy) + at;
+      const T* pre = static_cast<const T*>(p.pre) + at;
+      float d[8], z[8];
+      if (p.vec) {
+#pragma unroll
+        for (int q = 0; q < 8 / V; ++q) {
+          const Piece<T, V> a = piece_load<T, V>(dy + q * V);
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[q * V + e] = (float)a.v[e];
+          if (p.act != VEEX_ACT_NONE) {
+            const Piece<T, V> b = piece_load<T, V>(pre + q * V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[q * V + e] = (float)b.v[e];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d[e] = e < n ? (float)dy[e] : 0.f;
+          z[e] = e < n && p.act != VEEX_ACT_NONE ? (float)pre[e] : 0.f;
+        }
+      }
+      if (p.drop.cut != 0u) {
+        unsigned w[4];
+        drop_words(p.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = drop_u16(w, e) >= p.drop.cut ? d[e] * p.drop.scale : 0.f;
+      }
+      if (p.act != VEEX_ACT_NONE)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] *= dense_act_grad(z[e], p.act);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += d[e];
+      if (p.dz != nullptr) {
+        T* dz = static_cast<T*>(p.dz) + at;
+        if (p.vec) {
+#pragma unroll
+          for (int q = 0; q < 8 / V; ++q) {
+            Piece<T, V> a;
+#pragma unroll
+            for (int e = 0; e < V; ++e) a.v[e] = (T)d[q * V + e];
+            piece_store<T, V>(dz + q * V, a);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < n) dz[e] = (T)d[e];
+        }
+      }
+    }
+  }
+  if (p.part == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[ty][8 * tx + e] = sum[e];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < p.n) {
+    float a = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) a += s[q][threadIdx.x];
+    p.part[(long long)blockIdx.y * p.n + col] = a;
+  }
+}
+
+// db = the partial rows' sum, 64 columns and 16 row lanes a block
+template <typename T>
+__global__ __launch_bounds__(1024) void dense_db_kernel(const float* part, int chunks, int n, void* db) {
+  __shared__ float s[16][64];
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, col = blockIdx.x * 64 + tx;
+  float a = 0.f;
+  if (col < n)
+    for (int c = ty; c < chunks; c += 16) a += part[(long long)c * n + col];
+  s[ty][tx] = a;
+  __syncthreads();
+  if (ty == 0 && col < n) {
+    a = 0.f;
+    for (int q = 0; q < 16; ++q) a += s[q][tx];
+    static_cast<T*>(db)[col] = (T)a;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+static const int kKindFwd = 0, kKindDx = 1, kKindDw = 2;     // which of A, B have k contiguous: A only; both; neither
+
+// a tensor's pieces of 8 elements along its contiguous index (length `len`) are whole and 16-byte aligned
+static bool operand_vec(const DenseOperand& o, long long len, int elem) {
+  const long long other = o.k_stride == 1 ? o.row_stride : o.k_stride;
+  return trunk_aligned16(o.p) && other * elem % 16 == 0 && len % 8 == 0;
+}
+
+// The reduction is split where the tiles alone leave most of the 256 CUs idle: up to 512 blocks, at least 64 k each.
+static void general_split(long long I, int J, long long K, int& splits, long long& per) {
+  const long long tiles = (I + 63) / 64 * ((J + 63) / 64);
+  long long s = tiles >= 256 ? 1 : std::min<long long>(512 / tiles, (K + 63) / 64);
+  s = std::max<long long>(s, 1);
+  per = ((K + s - 1) / s + 31) / 32 * 32;
+  splits = (int)((K + per - 1) / per);
+}
+
+static long long align256(long long b) { return (b + 255) / 256 * 256; }
+
+static long long general_bytes(long long I, int J, long long K) {
+  int s; long long per;
+  general_split(I, J, K, s, per);
+  return s > 1 ? align256((long long)s * I * J * 4) : 0;
+}
+
+template <typename T>
+static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
+  general_split(g.I, g.J, g.K, g.splits, g.k_per_split);
+  g.slab = static_cast<float*>(ws);
+  g.vec_a = operand_vec(g.a, kind == kKindDw ? g.I : g.K, sizeof(T));
+  g.vec_b = operand_vec(g.b, kind == kKindDx ? g.K : g.J, sizeof(T));
+  g.vec_e = dense_epi_vec(g.epi, g.J, g.splits > 1 ? 8 : 4, sizeof(T));
+  const long long tiles = (g.I + 63) / 64 * ((g.J + 63) / 64);
+  if (tiles > 0x7FFFFFFFll) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
+  const dim3 grid((unsigned)tiles, (unsigned)g.splits);
+#define DG_GO(AK, BK)                                                                                              \
+  if (g.splits > 1) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, true>), grid, dim3(256), 0, st, g);         \
+  else hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, false>), grid, dim3(256), 0, st, g);
+  if (kind == kKindFwd) { DG_GO(true, false) }
+  else if (kind == kKindDx) { DG_GO(true, true) }
+  else { DG_GO(false, false) }
+#undef DG_GO
+  VEEX_CHECK_LAUNCH();
+  if (g.splits > 1) {
+    const long long nb = g.I * ((g.J + 7) / 8);
+    hipLaunchKernelGGL((dense_join_kernel<T>), dim3((unsigned)std::min<long long>((nb + 255) / 256, 1 << 16)), dim3(256), 0, st, g);
+    VEEX_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+// K >= 1 columns in, n >= 1 columns out, rows >= 0
+static int dense_check(const VeexDense* d, const char* who, DropArgs& drop) {
+  if (d == nullptr || (d->struct_size != 0 && d->struct_size != (int)sizeof(VeexDense))) { veex_set_error("%s: struct_size is not this library's", who); return VEEX_EINVAL; }
+  if (!trunk_dtype_ok(d->dtype) || d->activation < 0 || d->activation > VEEX_ACT_SIGMOID) { veex_set_error("%s: unknown dtype or activation", who); return VEEX_EINVAL; }
+  if (d->rows < 0 || d->rows > (1ll << 31) || d->k < 1 || d->n < 1 || d->ldx < d->k) {
+    veex_set_error("%s: 0 <= rows <= 2^31, k >= 1, n >= 1 and ldx >= k are needed", who); return VEEX_EINVAL;
+  }
+  if (!trunk_drop_args(d->rate, d->seed, d->first_row, d->counter, drop)) { veex_set_error("%s: rate %g is outside [0, 1 - 2^-17)", who, d->rate); return VEEX_EINVAL; }
+  return 0;
+}
+
+static DenseGemm dense_product(int kind, const VeexDense* d, const void* dz) {
+  DenseGemm g = {};
+  if (kind == kKindFwd) {
+    g.I = d->rows; g.J = d->n; g.K = d->k;
+    g.a = {d->x, d->ldx, 1}; g.b = {d->w, 1, d->n};
+  } else if (kind == kKindDx) {          // dx[i][j] = sum_n dz(i, n) w(j, n)
+    g.I = d->rows; g.J = d->k; g.K = d->n;
+    g.a = {dz, d->n, 1}; g.b = {d->w, d->n, 1};
+    g.epi.y = d->dx;
+  } else {                               // dw[i][j] = sum_m x(m, i) dz(m, j)
+    g.I = d->k; g.J = d->n; g.K = d->rows;
+    g.a = {d->x, 1, d->ldx}; g.b = {dz, 1, d->n};
+    g.epi.y = d->dw;
+  }
+  return g;
+}
+
+static long long product_bytes(int kind, const VeexDense* d) {
+  const DenseGemm g = dense_product(kind, d, nullptr);
+  return general_bytes(g.I, g.J, g.K);
+}
+
+static int product_launch(int kind, int dtype, const DenseGemm& g, void* ws, hipStream_t st) {
+  if (dtype == VEEX_T_F32) return general_launch<float>(kind, g, ws, st);
+  if (dtype == VEEX_T_BF16) return general_launch<bf16_t>(kind, g, ws, st);
+  return general_launch<f16_t>(kind, g, ws, st);
+}
+
+// the backward workspace: [dz] [partial column sums] [one product's slabs, used by dx and then by dw on the same stream]
+struct BwdLayout { bool dz_own; long long dz, part, prod; int chunks; long long rows_per_chunk; };
+
+static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
+  BwdLayout l = {};
+  l.dz_own = d->activation != VEEX_ACT_NONE || drop.cut != 0u;
+  const int strips = (d->n + 255) / 256;
+  const long long want = std::max<long long>(1024 / strips, 1);
+  l.rows_per_chunk = std::max<long long>(((d->rows + want - 1) / want + 7) / 8 * 8, 8);
+  l.chunks = (int)((d->rows + l.rows_per_chunk - 1) / l.rows_per_chunk);
+  l.dz = l.dz_own ? align256(d->rows * d->n * trunk_elem_bytes(d->dtype)) : 0;
+  l.part = align256((long long)l.chunks * d->n * 4);
+  l.prod = std::max(product_bytes(kKindDx, d), product_bytes(kKindDw, d));
+  return l;
+}
+
+extern "C" {
+
+long long veex_dense_fwd_workspace_bytes(const VeexDense* d) {
+  DropArgs drop;
+  if (dense_check(d, "dense", drop) != 0) return -1;
+  return d->rows == 0 ? 0 : product_bytes(kKindFwd, d);
+}
+
+int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
+  DropArgs drop;
+  if (int rc = dense_check(d, "dense", drop)) return rc;
+  if (d->x == nullptr || d->w == nullptr || d->y == nullptr) { veex_set_error("dense: x, w and y are needed"); return VEEX_EINVAL; }
+  if (d->rows == 0) return 0;
+  const long long need = product_bytes(kKindFwd, d);
+  if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need)) { veex_set_error("dense: a workspace of %lld bytes is needed", need); return VEEX_ENOMEM; }
+  DenseGemm g = dense_product(kKindFwd, d, nullptr);
+  g.epi = {d->bias, d->residual, d->y, d->pre, d->activation, drop};
+  return product_launch(kKindFwd, d->dtype, g, d->workspace, st);
+}
+
+long long veex_dense_bwd_workspace_bytes(const VeexDense* d) {
+  DropArgs drop;
+  if (dense_check(d, "dense backward", drop) != 0) return -1;
+  const BwdLayout l = bwd_layout(d, drop);
+  return l.dz + l.part + l.prod;
+}
+
+int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
+  DropArgs drop;
+  if (int rc = dense_check(d, "dense backward", drop)) return rc;
+  if (d->dy == nullptr || (d->dw != nullptr && d->x == nullptr) || (d->dx != nullptr && d->w == nullptr) ||
+      (d->activation != VEEX_ACT_NONE && d->pre == nullptr)) {
+    veex_set_error("dense backward: dy, x for dw, w for dx and pre for an activation are needed"); return VEEX_EINVAL;
+  }
+  if (d->rows == 0) { veex_set_error("dense backward: no rows"); return VEEX_EINVAL; }
+  const BwdLayout l = bwd_layout(d, drop);
+  if (l.dz + l.part + l.prod > 0 && (d->workspace == nullptr || d->workspace_bytes < l.dz + l.part + l.prod)) {
+    veex_set_error("dense backward: a workspace of %lld bytes is needed", l.dz + l.part + l.prod); return VEEX_ENOMEM;
+  }
+  char* ws = static_cast<char*>(d->workspace);
+  const void* dz = l.dz_own ? ws : d->dy;
+  if (l.dz_own || d->db != nullptr) {
+    DenseDz p = {};
+    p.dy = d->dy; p.pre = d->pre; p.dz = l.dz_own && (d->dx != nullptr || d->dw != nullptr) ? ws : nullptr;
+    p.part = d->db != nullptr ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
+    p.rows = d->rows; p.rows_per_chunk = l.rows_per_chunk; p.n = d->n; p.act = d->activation; p.drop = drop;
+    p.vec = d->n % 8 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
+    if (p.dz != nullptr || p.part != nullptr) {
+      const dim3 grid((d->n + 255) / 256, l.chunks);
+      if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_dz_kernel<float>), grid, dim3(256), 0, st, p);
+      else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_dz_kernel<bf16_t>), grid, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL((dense_dz_kernel<f16_t>), grid, dim3(256), 0, st, p);
+      VEEX_CHECK_LAUNCH();
+    }
+    if (d->db != nullptr) {
+      const dim3 grid((d->n + 63) / 64);
+      if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_db_kernel<float>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
+      else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_db_kernel<bf16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
+      else hipLaunchKernelGGL((dense_db_kernel<f16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
+      VEEX_CHECK_LAUNCH();
+    }
+  }
+  void* prod = ws + l.dz + l.part;
+  if (d->dx != nullptr)
+    if (int rc = product_launch(kKindDx, d->dtype, dense_product(kKindDx, d, dz), prod, st)) return rc;
+  if (d->dw != nullptr)
+    if (int rc = product_launch(kKindDw, d->dtype, dense_product(kKindDw, d, dz), prod, st)) return rc;
+  return 0;
+}
+
+}  // extern "C"

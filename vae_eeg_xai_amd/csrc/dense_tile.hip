@@ -1,0 +1,362 @@
+// Large Dense products on the bf16 / fp16 matrix cores:  C[i][j] = sum_k A(i, k) B(k, j), fp32 accumulate, the epilogue of
+// dense_common.h on the way out.  PL = 1: 16-bit tensors.  PL = 3: fp32 tensors, split beforehand into three bf16 terms
+// (a = a1 + a2 + a3 to 2^-27, dense_pack_kernel); a product is the six partial products a1b1, a1b2, a2b1, a1b3, a2b2, a3b1, smallest
+// first; what is left out is below 2^-25 of |a b|.
+//
+// A tile of BM x BN is computed by WM x WN waves, BK of the reduction at a time.  Operands go from memory straight into LDS
+// (16 bytes a lane, no registers in between) into the buffer that the step before has finished with, while the MFMAs of
+// this step read the other one: one barrier a step.  An operand whose k index is contiguous lies in LDS as [row][BK] and is
+// read as the MFMA wants it, 8 consecutive k a lane; one whose row index is contiguous lies as [k][128 rows] and is
+// read through the transposing LDS read.  The load writes LDS in lane order, so the bank swizzle is applied to the address
+// that a lane loads from: 16-byte piece q of an LDS row holds the tensor's piece q ^ s(row).
+//   [row][64]: s = row & 7;  [row][32]: s = (row >> 1) & 3;  [k][128]: s = (k & 3) << 2
+//
+// Needs: 16-byte aligned operands and rows; a k-contiguous operand's K a multiple of 8.  Pieces past a tensor's end
+// are sent out of the buffer's range and arrive as zeros.
+#include "dense_tile.h"
+#include <algorithm>
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float dt_f4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+#define DT_LDS __attribute__((address_space(3)))
+#define DT_OOB 0xFFFFFFF0u      // past every buffer's end
+
+__device__ __forceinline__ f32x16 dt_mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 dt_mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+template <typename T> struct DtVec;
+template <> struct DtVec<bf16_t> { typedef bf16x8 x8; };
+template <> struct DtVec<f16_t> { typedef f16x8 x8; };
+
+// One operand's ROWS x BK tiles (ROWS a multiple of 128 where the row index is contiguous)
+template <int ROWS, int BK, bool KC, int PL, int WAVES>
+struct DtOperand {
+  static constexpr int BYTES = ROWS * BK * 2;                  // of a plane's tile
+  static constexpr int LOADS = BYTES / 1024 / WAVES;           // 1024-byte loads of a wave, per plane
+  static_assert(BYTES % (1024 * WAVES) == 0, "whole loads for every wave");
+  static_assert(KC ? (BK == 64 || BK == 32) : ROWS % 128 == 0, "layouts with a swizzle");
+  static constexpr int ROWB = BK * 2;
+
+  const char* base;                // (row0, k = 0) of plane 0
+  long long ld, plane;             // bytes between rows (KC) or k's (not KC); between planes
+  long long K, rows_left;          // rows_left: rows from row0 on
+  unsigned voff[LOADS], piece_k[LOADS];
+  int wave, lane;
+
+  __device__ __forceinline__ static int swz(int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; }
+
+  __device__ __forceinline__ void init(const DtTensor& t, long long row0, long long rows, long long K_, int wave_, int lane_) {
+    wave = wave_; lane = lane_; ld = t.ld_bytes; plane = t.plane_bytes; K = K_; rows_left = rows - row0;
+    base = static_cast<const char*>(t.p) + (KC ? row0 * ld : row0 * 2);
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int at = (u * WAVES + wave) * 1024 + lane * 16;    // byte of the LDS tile that this lane fills
+      if (KC) {
+        const int row = at / ROWB, q = (at % ROWB) / 16, piece = q ^ swz(row);
+        piece_k[u] = piece * 8;
+        voff[u] = row < rows_left ? (unsigned)(row * ld) + piece * 16 : DT_OOB;
+      } else {
+        const int sub = at / (BK * 256), in = at % (BK * 256), k = in / 256, q = (in % 256) / 16, piece = q ^ ((k & 3) << 2);
+        const int row = sub * 128 + piece * 8;
+        piece_k[u] = k;
+        voff[u] = row < rows_left ? (unsigned)(k * ld) + row * 2 : DT_OOB;
+      }
+    }
+  }
+
+  // loads the BK reduction indices from k0 on (those at or past k_end arrive as zeros) into the tile at lds
+  __device__ __forceinline__ void load(DT_LDS char* lds, long long k0, long long k_end) const {
+    const bool whole = k0 + BK <= k_end;
+#pragma unroll
+    for (int pl = 0; pl < PL; ++pl) {
+      const char* p = base + pl * plane + (KC ? k0 * 2 : k0 * ld);
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)0xFFFFFFE0u, 0x00020000);
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) {
+        unsigned v = voff[u];
+        if (!whole) v = k0 + piece_k[u] < k_end ? v : DT_OOB;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DT_LDS void*)(lds + pl * BYTES + (u * WAVES + wave) * 1024), 16, v, 0, 0, 0);
+      }
+    }
+  }
+
+  // the 8 k's of lane half lh at k step ks (16 k's), of the 32 rows from `row` on (a multiple of 32)
+  template <typename V8>
+  __device__ __forceinline__ V8 frag(const DT_LDS char* lds, int pl, int row, int ks) const {
+    const int l31 = lane & 31, lh = lane >> 5;
+    if (KC) {
+      const int r = row + l31, q = (2 * ks + lh) ^ swz(r);
+      return *reinterpret_cast<const DT_LDS V8*>(lds + pl * BYTES + r * ROWB + q * 16);
+    } else {
+      const int g = lane >> 4, tq = (lane & 15) >> 2, tp = lane & 3;
+      const int k = ks * 16 + 8 * (g >> 1) + tq, piece = (row & 127) / 8 + 2 * (g & 1) + (tp >> 1);
+      const DT_LDS char* a = lds + pl * BYTES + (row >> 7) * (BK * 256) + k * 256 + 16 * (piece ^ ((k & 3) << 2)) + 8 * (tp & 1);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DT_LDS s16x4*)a);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DT_LDS s16x4*)(a + 4 * 256));     // four k's on: the same swizzle
+      return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// block -> (tile row, tile column, split): blocks go round the 8 XCDs in turn, so each XCD takes a contiguous run of tiles,
+// walked in bands of 8 tile rows: the tiles that one L2 holds at a time share 8 strips of A and a few of B
+__device__ __forceinline__ void dt_tile_of(unsigned b, unsigned ti, unsigned tj, unsigned splits, unsigned& i, unsigned& j, unsigned& z) {
+  const unsigned total = ti * tj * splits, per = total / 8, extra = total % 8;
+  const unsigned x = b % 8, s = b / 8;
+  unsigned t = x * per + min(x, extra) + s;
+  z = t / (ti * tj); t -= z * (ti * tj);
+  const unsigned band = t / (8 * tj), in = t - band * 8 * tj, h = min(8u, ti - band * 8);
+  j = in / h; i = band * 8 + in - j * h;
+}
+
+// LDS written and read by different lanes of one wave: the wave's LDS accesses complete in order, so only the compiler has to keep them so
+__device__ __forceinline__ void dt_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Split operands and infinities: an infinite operand times the other's lower terms gives NaN where fp32 gives an infinity.  A 32 x 32
+// block that holds a NaN is computed again with the fp32 MFMA from the terms' sums (which are the operands to 2^-27, and exactly them
+// where they are not finite), and its NaN elements take those values.  Finite data never come here.
+template <bool AKC, bool BKC, int MT, int NT>
+__device__ __forceinline__ void dt_mend(const DtGemm& g, f32x16 (&acc)[MT][NT], long long i0, int j0, long long k_begin, long long k_end, int lane) {
+  const int l31 = lane & 31, lh = lane >> 5;
+  auto value = [](const DtTensor& t, bool kc, long long row, long long k) -> float {
+    const char* p = static_cast<const char*>(t.p) + (kc ? row * t.ld_bytes + k * 2 : k * t.ld_bytes + row * 2);
+    return (float)*reinterpret_cast<const bf16_t*>(p) + (float)*reinterpret_cast<const bf16_t*>(p + t.plane_bytes) +
+           (float)*reinterpret_cast<const bf16_t*>(p + 2 * t.plane_bytes);
+  };
+#pragma unroll
+  for (int mi = 0; mi < MT; ++mi)
+#pragma unroll
+    for (int nj = 0; nj < NT; ++nj) {
+      bool nan = false;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) nan |= acc[mi][nj][r] != acc[mi][nj][r];
+      if (!__any(nan)) continue;
+      const long long i = i0 + mi * 32 + l31;
+      const int j = j0 + nj * 32 + l31;
+      f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll 1
+      for (long long k = k_begin; k < k_end; k += 2) {
+        const bool in = k + lh < k_end;
+        const float av = in && i < g.I ? value(g.a, AKC, i, k + lh) : 0.f, bv = in && j < g.J ? value(g.b, BKC, j, k + lh) : 0.f;
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(bv, av, s, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[mi][nj][r] = acc[mi][nj][r] != acc[mi][nj][r] ? s[r] : acc[mi][nj][r];
+    }
+}
+
+template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
+  constexpr int WAVES = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
+  typedef DtOperand<BM, BK, AKC, PL, WAVES> OpA;
+  typedef DtOperand<BN, BK, BKC, PL, WAVES> OpB;
+  typedef typename DtVec<M>::x8 V8;
+  constexpr int STAGE = PL * (OpA::BYTES + OpB::BYTES);
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  DT_LDS char* smem = (DT_LDS char*)smem_raw;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = wave / WN, wj = wave % WN;
+  unsigned ti, tj, z;
+  dt_tile_of(blockIdx.x, g.tiles_i, g.tiles_j, g.splits, ti, tj, z);
+  const long long i0 = (long long)ti * BM;
+  const int j0 = tj * BN;
+  const long long k_begin = z * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
+
+  OpA a; OpB b;
+  a.init(g.a, i0, g.I, g.K, wave, lane);
+  b.init(g.b, j0, g.J, g.K, wave, lane);
+  f32x16 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  a.load(smem, k_begin, k_end);
+  b.load(smem + PL * OpA::BYTES, k_begin, k_end);
+  int cur = 0;
+  for (long long k0 = k_begin; k0 < k_end; k0 += BK, cur ^= 1) {
+    // this step's tiles have landed, and every wave is done with the other buffer
+    __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0)
+    __syncthreads();
+    DT_LDS char* sa = smem + cur * STAGE;
+    DT_LDS char* sb = sa + PL * OpA::BYTES;
+    if (k0 + BK < k_end) {
+      DT_LDS char* na = smem + (cur ^ 1) * STAGE;
+      a.load(na, k0 + BK, k_end);
+      b.load(na + PL * OpA::BYTES, k0 + BK, k_end);
+    }
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      V8 av[PL][MT], bv[PL][NT];
+#pragma unroll
+      for (int pl = 0; pl < PL; ++pl) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) av[pl][i] = a.template frag<V8>(sa, pl, (wi * MT + i) * 32, ks);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) bv[pl][j] = b.template frag<V8>(sb, pl, (wj * NT + j) * 32, ks);
+      }
+      if (PL == 1) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = dt_mfma(bv[0][j], av[0][i], acc[i][j]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 6; ++t) {
+          constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = dt_mfma(bv[PB[t] % PL][j], av[PA[t] % PL][i], acc[i][j]);
+        }
+      }
+    }
+  }
+
+  if (PL == 3) dt_mend<AKC, BKC, MT, NT>(g, acc, i0 + wi * MT * 32, j0 + wj * NT * 32, k_begin, k_end, lane);
+
+  // The way out: each wave turns its 32-row strips round through a corner of LDS of its own (fp32, 16-byte pieces swizzled by the
+  // row), so that a lane holds 8 consecutive columns of a row and eight lanes (four for 32 columns) write a whole line.  Straight
+  // from the accumulators' layout a store would touch 32 lines.
+  constexpr int CW = NT * 32, OCT = CW / 8, RPP = 64 / OCT;      // columns, their blocks of 8, rows a pass
+  static_assert(WAVES * 32 * CW * 4 <= 2 * STAGE, "the strips fit the stages");
+  __syncthreads();                                               // every wave is done with the operand tiles
+  DT_LDS char* strip = smem + wave * 32 * CW * 4;
+  const int l31 = lane & 31, lh = lane >> 5;
+  const unsigned long long base = drop_base(g.epi.drop);
+#pragma unroll
+  for (int mi = 0; mi < MT; ++mi) {
+#pragma unroll
+    for (int nj = 0; nj < NT; ++nj)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<DT_LDS dt_f4*>(strip + l31 * CW * 4 + (((nj * 8 + 2 * q + lh) ^ (l31 & 7)) * 16)) =
+            dt_f4{acc[mi][nj][4 * q], acc[mi][nj][4 * q + 1], acc[mi][nj][4 * q + 2], acc[mi][nj][4 * q + 3]};
+    dt_wave_sync();
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += RPP) {
+      const int r = r0 + lane / OCT, o = lane % OCT;
+      const dt_f4 lo = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o) ^ (r & 7)) * 16));
+      const dt_f4 hi = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o + 1) ^ (r & 7)) * 16));
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const long long i = i0 + (wi * MT + mi) * 32 + r;
+      const int j = j0 + wj * CW + 8 * o;
+      if (i >= g.I || j >= g.J) continue;
+      if (g.slab != nullptr) {
+        float* s = g.slab + (z * g.I + i) * g.J + j;
+        if (g.J % 4 == 0) {
+          *reinterpret_cast<dt_f4*>(s) = lo;
+          if (j + 4 < g.J) *reinterpret_cast<dt_f4*>(s + 4) = hi;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j + e < g.J) s[e] = v[e];
+        }
+      } else {
+        unsigned w[4] = {0u, 0u, 0u, 0u};
+        if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
+        dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e, w);
+      }
+    }
+    dt_wave_sync();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Packing: rows of a tensor (any row stride and alignment) as 16-byte aligned rows of `cols8` = cols rounded up to 8, zeros behind
+// the last column; an fp32 tensor as its three bf16 terms in three planes.  8 columns a thread.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void dense_pack_kernel(const T* __restrict__ src, long long ld, long long rows, int cols, int cols8,
+                                                         char* __restrict__ dst, long long plane_bytes, bool vec) {
+  const int bpr = cols8 / 8;
+  const long long nb = rows * bpr;
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < nb; t += (long long)gridDim.x * 256) {
+    const long long r = nb <= 0xFFFFFFFFll ? (long long)((unsigned)t / (unsigned)bpr) : t / bpr;
+    const int c = 8 * (int)(t - r * bpr);
+    const T* p = src + r * ld + c;
+    constexpr int V = 16 / sizeof(T);
+    T x[8];
+    if (vec) {
+#pragma unroll
+      for (int q = 0; q < 8 / V; ++q) {
+        const Piece<T, V> y = piece_load<T, V>(p + q * V);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[q * V + e] = y.v[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = c + e < cols ? p[e] : (T)0.f;
+    }
+    char* d = dst + (r * cols8 + c) * 2;
+    if constexpr (sizeof(T) == 2) {
+      Piece<T, 8> y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y.v[e] = x[e];
+      piece_store<T, 8>(reinterpret_cast<T*>(d), y);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = x[e];
+      dt_store_planes(d, plane_bytes, f);
+    }
+  }
+}
+
+int dense_pack_launch(int dtype, const void* src, long long ld, long long rows, int cols, void* dst, long long plane_bytes, hipStream_t st) {
+  const int cols8 = (cols + 7) / 8 * 8;
+  const bool vec = cols % 8 == 0 && trunk_aligned16(src) && ld * trunk_elem_bytes(dtype) % 16 == 0;
+  const long long nb = rows * (cols8 / 8);
+  const dim3 grid((unsigned)std::min<long long>((nb + 255) / 256, 1 << 16));
+  char* d = static_cast<char*>(dst);
+  if (dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_pack_kernel<float>), grid, dim3(256), 0, st, static_cast<const float*>(src), ld, rows, cols, cols8, d, plane_bytes, vec);
+  else if (dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_pack_kernel<bf16_t>), grid, dim3(256), 0, st, static_cast<const bf16_t*>(src), ld, rows, cols, cols8, d, plane_bytes, vec);
+  else hipLaunchKernelGGL((dense_pack_kernel<f16_t>), grid, dim3(256), 0, st, static_cast<const f16_t*>(src), ld, rows, cols, cols8, d, plane_bytes, vec);
+  VEEX_CHECK_LAUNCH();
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int WM, int WN>
+static int dt_go(const DtGemm& gin, hipStream_t st) {
+  DtGemm g = gin;
+  g.tiles_i = (unsigned)((g.I + BM - 1) / BM); g.tiles_j = (unsigned)((g.J + BN - 1) / BN);
+  constexpr int lds = 2 * PL * (BM + BN) * BK * 2;
+  const void* fn = reinterpret_cast<const void*>(dense_tile_kernel<T, M, PL, AKC, BKC, BM, BN, BK, WM, WN>);
+  // (a function's attribute belongs to the current device: set before each launch, a host-side call of well under a microsecond)
+  if (lds > 64 * 1024 && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    veex_set_error("dense: cannot raise the dynamic LDS limit"); return VEEX_ELAUNCH;
+  }
+  hipLaunchKernelGGL((dense_tile_kernel<T, M, PL, AKC, BKC, BM, BN, BK, WM, WN>), dim3(g.tiles_i * g.tiles_j * g.splits), dim3(64 * WM * WN), lds, st, g);
+  VEEX_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, typename M, bool AKC, bool BKC>
+static int dt_pick(int tile, const DtGemm& g, hipStream_t st) {
+  if constexpr (sizeof(T) == 4) return dt_go<T, M, 3, AKC, BKC, 128, 128, 32, 2, 4>(g, st);
+  else if (tile == 256) return dt_go<T, M, 1, AKC, BKC, 256, 256, 64, 2, 4>(g, st);
+  else return dt_go<T, M, 1, AKC, BKC, 128, 128, 64, 2, 2>(g, st);
+}
+
+template <typename T, typename M>
+static int dt_kind(bool akc, bool bkc, int tile, const DtGemm& g, hipStream_t st) {
+  if (akc && bkc) return dt_pick<T, M, true, true>(tile, g, st);
+  if (akc) return dt_pick<T, M, true, false>(tile, g, st);
+  return dt_pick<T, M, false, false>(tile, g, st);
+}
+
+int dense_tile_launch(int dtype, bool akc, bool bkc, int tile, const DtGemm& g, hipStream_t st) {
+  if (dtype == VEEX_T_F32) return dt_kind<float, bf16_t>(akc, bkc, tile, g, st);
+  if (dtype == VEEX_T_BF16) return dt_kind<bf16_t, bf16_t>(akc, bkc, tile, g, st);
+  return dt_kind<f16_t, f16_t>(akc, bkc, tile, g, st);
+}

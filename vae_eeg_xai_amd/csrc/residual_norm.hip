@@ -1,0 +1,463 @@
+// The step between two blocks of a residual trunk, in one pass over the rows:
+//   n = Norm_post(h),  x_out = x + scale * gate * n,  u = Norm_pre(x_out)
+// Norm is LayerNorm (mean and variance over the row) or RMSNorm, each with an optional weight and bias; without h it is
+// u = Norm_pre(x) alone (the trunk's entry).  gate has `groups` rows, each for rows/groups consecutive rows of x (rows: one
+// gate per element; 1: one per column), scale one value per column.  Backward, with D the whole gradient at x_out:
+//   t = du * pre_w;  D = dx_out + rstd2 (t - mean(t) - rhat mean(t rhat))        rhat = (x_out - mean2) rstd2
+//   dn = D scale gate;  e = dn post_w;  dh = rstd1 (e - mean(e) - xhat mean(e xhat));  dx = D
+//   dgate = sum over the group of D scale n;  dscale = sum D gate n;  dpost_w = sum dn xhat;  dpost_b = sum dn;
+//   dpre_w = sum du rhat;  dpre_b = sum du          (RMSNorm: without the means of t and e)
+//
+// Bound: HBM.  A row lives in the registers of 1 to 16 waves (8 or 16 elements a lane), so the forward pass reads x, h and
+// gate once and writes x_out and u once; the backward pass recomputes x_out from x and h in fp32 instead of reading the
+// rounded one (the same bytes, and the gradient is that of the unrounded chain).  All statistics and sums are fp32; the
+// variance is the mean of squared deviations (two passes over registers), not a difference of moments.
+// Column sums: each block adds up its own run of rows in registers, writes one partial row per sum, and a second kernel adds
+// the partial rows in a fixed order: no atomics, the same bits every time.
+#include "trunk_common.h"
+#include "../../include/veex.h"
+#include <algorithm>
+
+struct RNormParams {
+  const void *x, *h, *gate, *scale, *post_w, *post_b, *pre_w, *pre_b;
+  void *x_out, *u;
+  float* stats;              // [rows][4]: mean1, rstd1, mean2, rstd2
+  const void *dx_out, *du;   // backward; either may be null (a zero gradient)
+  void *dx, *dh, *dgate, *dscale, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+  float* part;               // [chunks][5][cols]
+  long long rows;
+  int cols, layer;
+  float eps;
+  long long groups, rows_per_group, rows_per_chunk, chunks_per_group;
+};
+
+// sum of a (and b) over the 64 * WPR lanes of a row; red: two buffers of 2 * 16 floats, taken in turn, so that one barrier a
+// sum is enough (a wave can write a buffer again only after the barrier of the sum in between)
+template <int WPR>
+struct RowSum {
+  float* red; int rg, wave, turn;
+  __device__ __forceinline__ RowSum(float* r, int rg_, int wave_) : red(r), rg(rg_), wave(wave_), turn(0) {}
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+    if (WPR == 1) return make_float2(a, b);
+    float* r = red + turn * 32;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) { r[(rg * WPR + wave) * 2] = a; r[(rg * WPR + wave) * 2 + 1] = b; }
+    __syncthreads();
+    a = 0.f; b = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) { a += r[(rg * WPR + w) * 2]; b += r[(rg * WPR + w) * 2 + 1]; }
+    return make_float2(a, b);
+  }
+};
+
+template <typename T, int V, int C> struct RowRaw { Piece<T, V> p[C]; };
+
+template <typename T, int V, int C, int LANES>
+__device__ __forceinline__ void row_load(RowRaw<T, V, C>& r, const void* base, long long at, int lane, int cols) {
+  const T* p = static_cast<const T*>(base) + at;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = (c * LANES + lane) * V;
+    if (col < cols) r.p[c] = piece_load<T, V>(p + col);
+    else
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.p[c].v[e] = (T)0.f;
+  }
+}
+template <typename T, int V, int C, int LANES>
+__device__ __forceinline__ void row_fill(RowRaw<T, V, C>& r, float v) {
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) r.p[c].v[e] = (T)v;
+}
+template <typename T, int V, int C, int LANES>
+__device__ __forceinline__ void row_store(void* base, long long at, const float (&v)[V * C], int lane, int cols) {
+  T* p = static_cast<T*>(base) + at;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = (c * LANES + lane) * V;
+    if (col < cols) {
+      Piece<T, V> q;
+#pragma unroll
+      for (int e = 0; e < V; ++e) q.v[e] = (T)v[c * V + e];
+      piece_store<T, V>(p + col, q);
+    }
+  }
+}
+template <typename T, int V, int C, int LANES>
+__device__ __forceinline__ void row_param(RowRaw<T, V, C>& r, const void* p, float otherwise, int lane, int cols) {
+  if (p != nullptr) row_load<T, V, C, LANES>(r, p, 0, lane, cols);
+  else row_fill<T, V, C, LANES>(r, otherwise);
+}
+
+// WPR waves a row, EPL elements a lane; VEC: rows are whole 16-byte pieces
+template <typename T, int WPR, int EPL, bool VEC>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNormParams p) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V, LANES = 64 * WPR;
+  constexpr int RG = WPR > 4 ? 1 : 4 / WPR;
+  __shared__ float red[64];
+  const int lane = threadIdx.x % LANES, rg = threadIdx.x / LANES;
+  RowSum<WPR> row_sum(red, rg, (threadIdx.x >> 6) % WPR);
+  const float inv = 1.f / (float)p.cols;
+
+  RowRaw<T, V, C> scale, ow, ob, pw, pb;
+  row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
+  row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
+  row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
+  row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols);
+  row_param<T, V, C, LANES>(pb, p.pre_b, 0.f, lane, p.cols);
+
+  bool in[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) in[c] = (c * LANES + lane) * V < p.cols;
+  // mean and 1/deviation of the row v (zero outside the row)
+  auto moments = [&](const float (&v)[EPL], float& mean, float& rstd) {
+    mean = 0.f;
+    if (p.layer) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) s += v[e];
+      mean = row_sum(s, 0.f).x * inv;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) { const float d = in[e / V] ? v[e] - mean : 0.f; q = fmaf(d, d, q); }
+    rstd = 1.f / sqrtf(row_sum(q, 0.f).x * inv + p.eps);
+  };
+
+  // every row group of a block takes the same number of turns (the sums hold barriers); a turn past the end repeats the last row
+  for (long long r0 = (long long)blockIdx.x * RG; r0 < p.rows; r0 += (long long)gridDim.x * RG) {
+    const bool live = r0 + rg < p.rows;
+    const long long row = live ? r0 + rg : p.rows - 1, at = row * p.cols;
+    RowRaw<T, V, C> xr, hr, gr;
+    row_load<T, V, C, LANES>(xr, p.x, at, lane, p.cols);
+    float v[EPL], mean1 = 0.f, rstd1 = 0.f, mean2, rstd2;
+    if (p.h != nullptr) {
+      row_load<T, V, C, LANES>(hr, p.h, at, lane, p.cols);
+      if (p.gate != nullptr) row_load<T, V, C, LANES>(gr, p.gate, row / p.rows_per_group * p.cols, lane, p.cols);
+      else row_fill<T, V, C, LANES>(gr, 1.f);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) v[e] = (float)hr.p[e / V].v[e % V];
+      moments(v, mean1, rstd1);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const int c = e / V, k = e % V;
+        const float n = fmaf((v[e] - mean1) * rstd1, (float)ow.p[c].v[k], (float)ob.p[c].v[k]);
+        v[e] = in[c] ? fmaf((float)scale.p[c].v[k] * (float)gr.p[c].v[k], n, (float)xr.p[c].v[k]) : 0.f;
+      }
+      if (live) row_store<T, V, C, LANES>(p.x_out, at, v, lane, p.cols);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) v[e] = (float)xr.p[e / V].v[e % V];
+    }
+    moments(v, mean2, rstd2);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) v[e] = fmaf((v[e] - mean2) * rstd2, (float)pw.p[e / V].v[e % V], (float)pb.p[e / V].v[e % V]);
+    if (live) {
+      row_store<T, V, C, LANES>(p.u, at, v, lane, p.cols);
+      if (p.stats != nullptr && lane == 0) *reinterpret_cast<float4*>(p.stats + row * 4) = make_float4(mean1, rstd1, mean2, rstd2);
+    }
+  }
+}
+
+// One block a chunk: rows_per_chunk consecutive rows of one gate group.
+template <typename T, int WPR, int EPL, bool VEC>
+__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNormParams p) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V, LANES = 64 * WPR;
+  constexpr int RG = WPR > 4 ? 1 : 4 / WPR;
+  __shared__ float red[64];
+  __shared__ float comb[RG > 1 ? RG * LANES * EPL : 1];
+  const int lane = threadIdx.x % LANES, rg = threadIdx.x / LANES;
+  RowSum<WPR> row_sum(red, rg, (threadIdx.x >> 6) % WPR);
+  const float inv = 1.f / (float)p.cols;
+  const bool post = p.h != nullptr;
+
+  RowRaw<T, V, C> scale, ow, ob, pw, gr;
+  row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
+  row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
+  row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
+  row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols);
+  bool in[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) in[c] = (c * LANES + lane) * V < p.cols;
+
+  const long long group = blockIdx.x / p.chunks_per_group, piece = blockIdx.x - group * p.chunks_per_group;
+  const long long first = group * p.rows_per_group + piece * p.rows_per_chunk;
+  const long long last = min(first + p.rows_per_chunk, (group + 1) * p.rows_per_group);     // one past
+  const bool full_gate = p.gate != nullptr && p.rows_per_group == 1;
+  if (p.gate != nullptr) row_load<T, V, C, LANES>(gr, p.gate, group * p.cols, lane, p.cols);
+  else row_fill<T, V, C, LANES>(gr, 1.f);
+
+  float a_gate[EPL], a_ow[EPL], a_ob[EPL], a_pw[EPL], a_pb[EPL];
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) a_gate[e] = a_ow[e] = a_ob[e] = a_pw[e] = a_pb[e] = 0.f;
+
+  // (a gate per element: the chunks of one row each would leave as many partial rows as there are rows, so there the host
+  // hands out chunks of several "groups" and the gate is read with its row)
+  const long long c_first = full_gate ? blockIdx.x * p.rows_per_chunk : first;
+  const long long c_last = full_gate ? min(c_first + p.rows_per_chunk, p.rows) : last;
+  for (long long r0 = c_first; r0 < c_last; r0 += RG) {
+    const bool live = r0 + rg < c_last;
+    const long long row = live ? r0 + rg : c_last - 1, at = row * p.cols;
+    RowRaw<T, V, C> xr, hr, dor, dur;
+    row_load<T, V, C, LANES>(xr, p.x, at, lane, p.cols);
+    if (post) row_load<T, V, C, LANES>(hr, p.h, at, lane, p.cols);
+    if (p.dx_out != nullptr) row_load<T, V, C, LANES>(dor, p.dx_out, at, lane, p.cols);
+    else row_fill<T, V, C, LANES>(dor, 0.f);
+    if (p.du != nullptr) row_load<T, V, C, LANES>(dur, p.du, at, lane, p.cols);
+    else row_fill<T, V, C, LANES>(dur, 0.f);
+    if (full_gate) row_load<T, V, C, LANES>(gr, p.gate, at, lane, p.cols);
+    const float4 st = *reinterpret_cast<const float4*>(p.stats + row * 4);
+
+    float xh[EPL], n[EPL], rh[EPL], d[EPL];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      const int c = e / V, k = e % V;
+      float out = (float)xr.p[c].v[k];
+      xh[e] = n[e] = 0.f;
+      if (post) {
+        xh[e] = ((float)hr.p[c].v[k] - st.x) * st.y;
+        n[e] = fmaf(xh[e], (float)ow.p[c].v[k], (float)ob.p[c].v[k]);
+        out = fmaf((float)scale.p[c].v[k] * (float)gr.p[c].v[k], n[e], out);
+      }
+      rh[e] = in[c] ? (out - st.z) * st.w : 0.f;
+      const float du = (float)dur.p[c].v[k];
+      if (live) { a_pw[e] = fmaf(du, rh[e], a_pw[e]); a_pb[e] += du; }
+      d[e] = du * (float)pw.p[c].v[k];
+      s1 += d[e]; s2 = fmaf(d[e], rh[e], s2);
+    }
+    float2 m = row_sum(s1, s2);
+    m.x = p.layer ? m.x * inv : 0.f; m.y *= inv;
+    s1 = s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      const int c = e / V, k = e % V;
+      d[e] = fmaf(st.w, d[e] - fmaf(rh[e], m.y, m.x), (float)dor.p[c].v[k]);      // D
+    }
+    if (live && p.dx != nullptr) row_store<T, V, C, LANES>(p.dx, at, d, lane, p.cols);
+    if (post) {
+      float dg[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const int c = e / V, k = e % V;
+        const float s = (float)scale.p[c].v[k], g = (float)gr.p[c].v[k];
+        if (!in[c]) d[e] = 0.f;
+        const float dn = d[e] * (s * g);
+        dg[e] = d[e] * s * n[e];
+        if (live) {
+          a_gate[e] = fmaf(d[e] * n[e], full_gate ? g : 1.f, a_gate[e]);
+          a_ow[e] = fmaf(dn, xh[e], a_ow[e]); a_ob[e] += dn;
+        }
+        d[e] = dn * (float)ow.p[c].v[k];
+        s1 += d[e]; s2 = fmaf(d[e], in[c] ? xh[e] : 0.f, s2);
+      }
+      if (live && full_gate && p.dgate != nullptr) row_store<T, V, C, LANES>(p.dgate, at, dg, lane, p.cols);
+      m = row_sum(s1, s2);
+      m.x = p.layer ? m.x * inv : 0.f; m.y *= inv;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) d[e] = st.y * (d[e] - fmaf(xh[e], m.y, m.x));
+      if (live && p.dh != nullptr) row_store<T, V, C, LANES>(p.dh, at, d, lane, p.cols);
+    }
+  }
+
+  float* part = p.part + (long long)blockIdx.x * 5 * p.cols;
+  auto flush = [&](float (&a)[EPL], int k) {
+    if (RG > 1) {                      // the block's row groups, added in order
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) comb[(rg * LANES + lane) * EPL + e] = a[e];
+      __syncthreads();
+      if (rg != 0) return;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        a[e] = 0.f;
+        for (int g = 0; g < RG; ++g) a[e] += comb[(g * LANES + lane) * EPL + e];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * LANES + lane) * V;
+      if (col < p.cols)
+#pragma unroll
+        for (int e = 0; e < V; ++e) part[(long long)k * p.cols + col + e] = a[c * V + e];
+    }
+  };
+  if (p.dscale != nullptr || (p.dgate != nullptr && !full_gate)) flush(a_gate, 0);
+  if (p.dpost_w != nullptr) flush(a_ow, 1);
+  if (p.dpost_b != nullptr) flush(a_ob, 2);
+  if (p.dpre_w != nullptr) flush(a_pw, 3);
+  if (p.dpre_b != nullptr) flush(a_pb, 4);
+}
+
+// Column sums of the partial rows: 64 columns and 16 row lanes a block; blockIdx.y = which sum.
+template <typename T>
+__global__ __launch_bounds__(1024) void rnorm_sums_kernel(RNormParams p, long long chunks) {
+  __shared__ float s[16][64];
+  const int k = blockIdx.y, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + tx;
+  const bool ok = col < p.cols;
+  auto column = [&](long long from, long long to) -> float {       // valid in row lane 0
+    float a = 0.f;
+    if (ok)
+      for (long long c = from + ty; c < to; c += 16) a += p.part[(c * 5 + k) * p.cols + col];
+    __syncthreads();
+    s[ty][tx] = a;
+    __syncthreads();
+    a = 0.f;
+    if (ty == 0)
+      for (int i = 0; i < 16; ++i) a += s[i][tx];
+    return a;
+  };
+  if (k == 0 && p.gate != nullptr && p.rows_per_group > 1) {
+    if (p.dscale == nullptr && p.dgate == nullptr) return;
+    float ds = 0.f;
+    const float sc = p.scale != nullptr && ok ? (float)static_cast<const T*>(p.scale)[col] : 1.f;
+    for (long long g = 0; g < p.groups; ++g) {
+      const float a = column(g * p.chunks_per_group, (g + 1) * p.chunks_per_group);
+      if (ty == 0 && ok) {
+        if (p.dgate != nullptr) static_cast<T*>(p.dgate)[g * p.cols + col] = (T)(a * sc);
+        ds = fmaf(a, (float)static_cast<const T*>(p.gate)[g * p.cols + col], ds);
+      }
+    }
+    if (ty == 0 && ok && p.dscale != nullptr) static_cast<T*>(p.dscale)[col] = (T)ds;
+    return;
+  }
+  void* const outs[5] = {p.dscale, p.dpost_w, p.dpost_b, p.dpre_w, p.dpre_b};
+  T* out = static_cast<T*>(outs[k]);
+  if (out == nullptr) return;
+  const float a = column(0, chunks);
+  if (ty == 0 && ok) out[col] = (T)a;
+}
+
+// waves a row / elements a lane: the fewest lanes that hold the row at 8 elements each, up to 16 waves; wider rows take 16
+#define RNORM_BY_WIDTH(KERNEL, T, VEC, GRID, BLOCKS_OF)                                                                      \
+  do {                                                                                                                       \
+    if (p.cols <= 512) { GRID(4); hipLaunchKernelGGL((KERNEL<T, 1, 8, VEC>), dim3(grid), dim3(256), 0, st, p); }              \
+    else if (p.cols <= 1024) { GRID(2); hipLaunchKernelGGL((KERNEL<T, 2, 8, VEC>), dim3(grid), dim3(256), 0, st, p); }        \
+    else if (p.cols <= 2048) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 4, 8, VEC>), dim3(grid), dim3(256), 0, st, p); }        \
+    else if (p.cols <= 4096) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 8, 8, VEC>), dim3(grid), dim3(512), 0, st, p); }        \
+    else if (p.cols <= 8192) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 8, VEC>), dim3(grid), dim3(1024), 0, st, p); }      \
+    else { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 16, VEC>), dim3(grid), dim3(1024), 0, st, p); }                         \
+  } while (0)
+
+static bool rnorm_vec(const RNormParams& p, int dtype) {
+  if (p.cols % (16 / trunk_elem_bytes(dtype)) != 0) return false;
+  for (const void* q : {p.x, p.h, p.gate, p.scale, p.post_w, p.post_b, p.pre_w, p.pre_b, (const void*)p.x_out, (const void*)p.u,
+                        p.dx_out, p.du, (const void*)p.dx, (const void*)p.dh, (const void*)p.dgate})
+    if (!trunk_aligned16(q)) return false;
+  return true;
+}
+
+template <typename T>
+static int rnorm_fwd_launch(const RNormParams& p, bool vec, hipStream_t st) {
+  unsigned grid = 0;
+#define RNORM_FWD_GRID(RG) grid = (unsigned)std::min<long long>((p.rows + (RG) - 1) / (RG), 256 * 16)
+  if (vec) RNORM_BY_WIDTH(rnorm_fwd_kernel, T, true, RNORM_FWD_GRID, 0);
+  else RNORM_BY_WIDTH(rnorm_fwd_kernel, T, false, RNORM_FWD_GRID, 0);
+  VEEX_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hipStream_t st) {
+  const unsigned grid = (unsigned)chunks;
+#define RNORM_BWD_GRID(RG) (void)0
+  if (vec) RNORM_BY_WIDTH(rnorm_bwd_kernel, T, true, RNORM_BWD_GRID, 0);
+  else RNORM_BY_WIDTH(rnorm_bwd_kernel, T, false, RNORM_BWD_GRID, 0);
+  VEEX_CHECK_LAUNCH();
+  if (p.dgate != nullptr || p.dscale != nullptr || p.dpost_w != nullptr || p.dpost_b != nullptr || p.dpre_w != nullptr || p.dpre_b != nullptr) {
+    hipLaunchKernelGGL((rnorm_sums_kernel<T>), dim3((p.cols + 63) / 64, 5), dim3(1024), 0, st, p, chunks);
+    VEEX_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+// rows of a chunk and chunks of a launch: about 512 blocks, none across a group's end
+static long long rnorm_chunks(long long rows, long long groups, long long& per_chunk, long long& per_group) {
+  const long long t = rows / groups;
+  const long long want = std::max<long long>((rows + 511) / 512, 4);
+  if (groups == rows) { per_chunk = want; per_group = 1; return (rows + want - 1) / want; }   // (a gate per element, or one row)
+  per_group = (t + want - 1) / want;
+  per_chunk = (t + per_group - 1) / per_group;
+  per_group = (t + per_chunk - 1) / per_chunk;
+  return per_group * groups;
+}
+
+static bool rnorm_struct_ok(const VeexResidualNorm* d) {
+  if (d != nullptr && (d->struct_size == 0 || d->struct_size == (int)sizeof(VeexResidualNorm))) return true;
+  veex_set_error("residual_norm: struct_size is not this library's");
+  return false;
+}
+
+static int rnorm_check(const char* who, long long rows, int cols, long long groups, int dtype, int kind, double eps) {
+  if (!trunk_dtype_ok(dtype) || (kind != VEEX_NORM_LAYER && kind != VEEX_NORM_RMS)) { veex_set_error("%s: unknown dtype or kind", who); return VEEX_EINVAL; }
+  if (rows < 0 || cols < 1 || cols > VEEX_NORM_MAX_COLS) { veex_set_error("%s: rows >= 0 and 1 <= cols <= %d are needed", who, VEEX_NORM_MAX_COLS); return VEEX_EINVAL; }
+  if (rows > (1ll << 31)) { veex_set_error("%s: at most 2^31 rows", who); return VEEX_EINVAL; }
+  if (groups < 1 || (rows > 0 && rows % groups != 0)) { veex_set_error("%s: the gate's groups have to divide the rows", who); return VEEX_EINVAL; }
+  if (!(eps >= 0.0)) { veex_set_error("%s: eps has to be >= 0", who); return VEEX_EINVAL; }
+  return 0;
+}
+
+static void rnorm_fill(RNormParams& p, const VeexResidualNorm* d) {
+  p.x = d->x; p.h = d->h; p.gate = d->h != nullptr ? d->gate : nullptr; p.scale = d->scale;
+  p.post_w = d->post_w; p.post_b = d->post_b; p.pre_w = d->pre_w; p.pre_b = d->pre_b;
+  p.x_out = d->x_out; p.u = d->u; p.stats = d->stats;
+  p.dx_out = d->dx_out; p.du = d->du; p.dx = d->dx;
+  const bool post = d->h != nullptr;               // (without h nothing depends on the block's side)
+  p.dh = post ? d->dh : nullptr; p.dgate = p.gate != nullptr ? d->dgate : nullptr; p.dscale = post ? d->dscale : nullptr;
+  p.dpost_w = post ? d->dpost_w : nullptr; p.dpost_b = post ? d->dpost_b : nullptr; p.dpre_w = d->dpre_w; p.dpre_b = d->dpre_b;
+  p.part = d->workspace;
+  p.rows = d->rows; p.cols = d->cols; p.layer = d->kind == VEEX_NORM_LAYER; p.eps = d->eps;
+  p.groups = p.gate != nullptr ? d->groups : 1;
+  p.rows_per_group = std::max<long long>(d->rows / p.groups, 1);
+  p.rows_per_chunk = p.chunks_per_group = 1;
+}
+
+extern "C" {
+
+int veex_residual_norm_fwd(const VeexResidualNorm* d, hipStream_t st) {
+  if (!rnorm_struct_ok(d)) return VEEX_EINVAL;
+  if (d->x == nullptr || d->u == nullptr || (d->h != nullptr && d->x_out == nullptr)) {
+    veex_set_error("residual_norm: x and u (with h also x_out) are needed"); return VEEX_EINVAL;
+  }
+  if (int rc = rnorm_check("residual_norm", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps)) return rc;
+  if (d->rows == 0) return 0;
+  RNormParams p;
+  rnorm_fill(p, d);
+  p.dx_out = p.du = nullptr; p.dx = p.dh = p.dgate = nullptr;
+  const bool vec = rnorm_vec(p, d->dtype);
+  if (d->dtype == VEEX_T_F32) return rnorm_fwd_launch<float>(p, vec, st);
+  if (d->dtype == VEEX_T_BF16) return rnorm_fwd_launch<bf16_t>(p, vec, st);
+  return rnorm_fwd_launch<f16_t>(p, vec, st);
+}
+
+long long veex_residual_norm_bwd_workspace_floats(long long rows, int cols, long long groups) {
+  if (rows < 0 || cols < 1 || groups < 1 || (rows > 0 && rows % groups != 0)) return -1;
+  if (rows == 0) return 0;
+  long long a, b;
+  return rnorm_chunks(rows, groups, a, b) * 5 * cols;
+}
+
+int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
+  if (!rnorm_struct_ok(d)) return VEEX_EINVAL;
+  if (d->x == nullptr || d->stats == nullptr || d->workspace == nullptr) {
+    veex_set_error("residual_norm backward: x, stats and workspace are needed"); return VEEX_EINVAL;
+  }
+  if (int rc = rnorm_check("residual_norm backward", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps)) return rc;
+  if (d->rows == 0) { veex_set_error("residual_norm backward: no rows"); return VEEX_EINVAL; }
+  RNormParams p;
+  rnorm_fill(p, d);
+  p.x_out = p.u = nullptr;
+  const long long chunks = rnorm_chunks(p.rows, p.groups, p.rows_per_chunk, p.chunks_per_group);
+  if (d->workspace_floats < chunks * 5 * p.cols) { veex_set_error("residual_norm backward: workspace of %lld floats is needed", chunks * 5 * p.cols); return VEEX_ENOMEM; }
+  const bool vec = rnorm_vec(p, d->dtype);
+  if (d->dtype == VEEX_T_F32) return rnorm_bwd_launch<float>(p, vec, chunks, st);
+  if (d->dtype == VEEX_T_BF16) return rnorm_bwd_launch<bf16_t>(p, vec, chunks, st);
+  return rnorm_bwd_launch<f16_t>(p, vec, chunks, st);
+}
+
+}  // extern "C"

@@ -9,6 +9,7 @@
 // shuffles + one LDS pass; cross-block sums go through partial slabs (no float atomics, so
 // results are bitwise reproducible run to run).
 #include "veex_internal.h"
+#include "philox.h"
 
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
@@ -476,17 +477,10 @@ __global__ __launch_bounds__(D6_THREADS) void deconv6_bwd_kernel(
 // uses counter e>>2 and output lane e&3, so epsilon is independent of batch split / world size.
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ float philox_normal(unsigned long long e, unsigned k0, unsigned k1) {
-  unsigned c0 = (unsigned)((e >> 2) & 0xFFFFFFFFull), c1 = (unsigned)(e >> 34), c2 = 0u, c3 = 0u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const unsigned hi0 = __umulhi(0xD2511F53u, c0), lo0 = 0xD2511F53u * c0;
-    const unsigned hi1 = __umulhi(0xCD9E8D57u, c2), lo1 = 0xCD9E8D57u * c2;
-    const unsigned n0 = hi1 ^ c1 ^ k0, n1 = lo1, n2 = hi0 ^ c3 ^ k1, n3 = lo0;
-    c0 = n0; c1 = n1; c2 = n2; c3 = n3;
-    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
-  }
+  unsigned c[4] = {(unsigned)((e >> 2) & 0xFFFFFFFFull), (unsigned)(e >> 34), 0u, 0u};
+  philox4x32_10(c, k0, k1);
   const int sel = (int)(e & 3ull);
-  const unsigned ua = (sel < 2) ? c0 : c2, ub = (sel < 2) ? c1 : c3;
+  const unsigned ua = (sel < 2) ? c[0] : c[2], ub = (sel < 2) ? c[1] : c[3];
   const float u1 = ((float)ua + 0.5f) * (1.0f / 4294967296.0f);
   const float u2 = ((float)ub + 0.5f) * (1.0f / 4294967296.0f);
   // (float)ua rounds to 2^32 for the top 128 values -> u1 could be 1.0: log(1)=0, still finite

@@ -16,6 +16,9 @@ the dual mode (input gradient), veex_wgrad_gemm + veex_slab_sum (weight gradient
 can compose them under torch.autograd; ``veex::sample`` (models.py:10-22) likewise
 (veex_reparam_kl_fwd/bwd), differentiable in ``z_mean`` and ``z_log_var``.
 
+The operators of a dense trunk -- ``veex::dense``, ``veex::dropout``, ``veex::residual_norm`` -- are registered by
+trunk_ops.py, which this module imports.
+
 A ``VeexNet*`` travels as a Python int (the plan is host-only state; it owns no device memory).
 """
 from __future__ import annotations
@@ -379,6 +382,8 @@ def _deconv_backward(ctx, dy):
 
 
 conv_transpose2d.register_autograd(_deconv_backward, setup_context=_deconv_setup)
+
+from . import trunk_ops  # noqa: E402,F401  (registers torch.ops.veex.dense / dropout / residual_norm)
 
 __all__ = ["train_fwd_bwd", "forward", "encode", "decode", "attribute", "adam", "sample", "sample_bwd",
            "conv2d", "conv2d_bwd", "conv_transpose2d", "conv_transpose2d_bwd", "conv_geometry", "deconv_geometry"]
