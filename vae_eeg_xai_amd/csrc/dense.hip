@@ -2,8 +2,8 @@
 // dw = x^T dz, db = column sums of dz.  x [M][K], w [K][N] (Keras layout), types fp32 / bf16 / fp16, sums in fp32.
 //
 // This file: the general product (any strides, alignment and size), the join of a split reduction, the dz / db pass, and
-// the host side.
-#include "dense_common.h"
+// the host side, which sends large products to the 16-bit matrix cores (dense_tile.hip).
+#include "dense_tile.h"
 #include <algorithm>
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -141,7 +141,8 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
 // ---------------------------------------------------------------------------------------------------------------
 struct DenseDz {
   const void *dy, *pre;
-  void* dz;              // null: only the sums
+  void* dz;              // null: only the sums.  Rows of ld columns (the ones behind n as zeros), or fp32 as planes
+  long long ld, plane_bytes;     // plane_bytes 0: dz in the tensors' type
   float* part;           // [chunks][N], null: none
   long long rows, rows_per_chunk;
   int n, act, vec;
@@ -192,11 +193,13 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
       }
       if (p.act != VEEX_ACT_NONE)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] *= dense_act_grad(z[e], p.act);
+        for (int e = 0; e < 8; ++e) d[e] = e < n ? d[e] * dense_act_grad(z[e], p.act) : 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += d[e];
-      if (p.dz != nullptr) {
-        T* dz = static_cast<T*>(p.dz) + at;
+      if (p.dz != nullptr && p.plane_bytes != 0) {
+        dt_store_planes(static_cast<char*>(p.dz) + (i * p.ld + j) * 2, p.plane_bytes, d);
+      } else if (p.dz != nullptr) {
+        T* dz = static_cast<T*>(p.dz) + i * p.ld + j;
         if (p.vec) {
 #pragma unroll
           for (int q = 0; q < 8 / V; ++q) {
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (e < n) dz[e] = (T)d[e];
+            if (j + e < p.ld) dz[e] = (T)d[e];
         }
       }
     }
@@ -272,6 +275,19 @@ static long long general_bytes(long long I, int J, long long K) {
 }
 
 template <typename T>
+static int join_launch(const DenseGemm& g, hipStream_t st) {
+  const long long nb = g.I * ((g.J + 7) / 8);
+  hipLaunchKernelGGL((dense_join_kernel<T>), dim3((unsigned)std::min<long long>((nb + 255) / 256, 1 << 16)), dim3(256), 0, st, g);
+  VEEX_CHECK_LAUNCH();
+  return 0;
+}
+static int join_any(int dtype, const DenseGemm& g, hipStream_t st) {
+  if (dtype == VEEX_T_F32) return join_launch<float>(g, st);
+  if (dtype == VEEX_T_BF16) return join_launch<bf16_t>(g, st);
+  return join_launch<f16_t>(g, st);
+}
+
+template <typename T>
 static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
   general_split(g.I, g.J, g.K, g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
@@ -289,11 +305,7 @@ static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
   else { DG_GO(false, false) }
 #undef DG_GO
   VEEX_CHECK_LAUNCH();
-  if (g.splits > 1) {
-    const long long nb = g.I * ((g.J + 7) / 8);
-    hipLaunchKernelGGL((dense_join_kernel<T>), dim3((unsigned)std::min<long long>((nb + 255) / 256, 1 << 16)), dim3(256), 0, st, g);
-    VEEX_CHECK_LAUNCH();
-  }
+  if (g.splits > 1) return join_launch<T>(g, st);
   return 0;
 }
 
@@ -306,6 +318,52 @@ static int dense_check(const VeexDense* d, const char* who, DropArgs& drop) {
   }
   if (!trunk_drop_args(d->rate, d->seed, d->first_row, d->counter, drop)) { veex_set_error("%s: rate %g is outside [0, 1 - 2^-17)", who, d->rate); return VEEX_EINVAL; }
   return 0;
+}
+
+// ---- large products -------------------------------------------------------------------------------------------------
+// A layer whose products have at least this many multiplications goes to dense_tile.hip: below it the packing and the tiles' edges
+// cost more than the fp32 MFMA of the general product.
+static const double kTileMin16 = 1 << 25, kTileMin32 = 1 << 27;
+
+static bool uses_tiles(const VeexDense* d) {
+  const double work = (double)d->rows * d->k * d->n;
+  // a tile addresses its operand by 32 bits from its first row on: 256 rows of up to 4 MB, 64 k's of up to 16 MB
+  const long long widest = std::max<long long>(std::max<long long>(d->k, d->n), d->ldx);
+  return work >= (d->dtype == VEEX_T_F32 ? kTileMin32 : kTileMin16) && widest < (1 << 21);
+}
+
+static long long round8(long long v) { return (v + 7) / 8 * 8; }
+static int planes_of(const VeexDense* d) { return d->dtype == VEEX_T_F32 ? 3 : 1; }
+// a packed copy of a rows x cols tensor
+static long long packed_plane(long long rows, long long cols) { return align256(rows * round8(cols) * 2); }
+static long long packed_bytes(const VeexDense* d, long long rows, long long cols) { return planes_of(d) * packed_plane(rows, cols); }
+// a 16-bit tensor that the tiles can load where it lies
+static bool lies_well(const VeexDense* d, const void* p, long long ld, long long cols) {
+  return d->dtype != VEEX_T_F32 && trunk_aligned16(p) && ld % 8 == 0 && cols % 8 == 0;
+}
+
+struct TilePlan { int tile; unsigned splits; long long per; };
+
+// The tile and the split of the reduction: the fewest rounds of the chip's tile slots, weighed by a tile's time
+static TilePlan tile_plan(const VeexDense* d, long long I, long long J, long long K) {
+  TilePlan best = {};
+  double cost = 1e300;
+  const bool f32 = d->dtype == VEEX_T_F32;
+  const int bk = f32 ? 32 : 64;
+  for (int tile : {256, 128}) {
+    if (f32 && tile == 256) continue;
+    const long long tiles = (I + tile - 1) / tile * ((J + tile - 1) / tile), slots = tile == 256 || f32 ? 256 : 512;
+    for (long long s = 1; s <= 64; s *= 2) {
+      const long long per = ((K + s - 1) / s + bk - 1) / bk * bk, splits = (K + per - 1) / per;
+      if (s > 1 && per < 4 * bk) break;
+      const double rounds = (double)((tiles * splits + slots - 1) / slots);
+      const double step = tile == 256 ? 4.0 : 2.2;                  // 2^14 multiplications at a full chip's rate; two 128s share a CU
+      const double join = splits > 1 ? (double)splits * I * J / (1 << 20) * 16.0 + 300.0 : 0.0;   // slabs out and in, one more launch
+      const double c = rounds * (step * ((double)per / 64.0 + 4.0)) * 8.0 + join;
+      if (c < cost) { cost = c; best = {tile, (unsigned)splits, per}; }
+    }
+  }
+  return best;
 }
 
 static DenseGemm dense_product(int kind, const VeexDense* d, const void* dz) {
@@ -325,30 +383,76 @@ static DenseGemm dense_product(int kind, const VeexDense* d, const void* dz) {
   return g;
 }
 
+// bytes of one product's slabs
 static long long product_bytes(int kind, const VeexDense* d) {
   const DenseGemm g = dense_product(kind, d, nullptr);
-  return general_bytes(g.I, g.J, g.K);
+  if (!uses_tiles(d)) return general_bytes(g.I, g.J, g.K);
+  const TilePlan t = tile_plan(d, g.I, g.J, g.K);
+  return t.splits > 1 ? align256((long long)t.splits * g.I * g.J * 4) : 0;
 }
 
-static int product_launch(int kind, int dtype, const DenseGemm& g, void* ws, hipStream_t st) {
+static int general_any(int kind, int dtype, const DenseGemm& g, void* ws, hipStream_t st) {
   if (dtype == VEEX_T_F32) return general_launch<float>(kind, g, ws, st);
   if (dtype == VEEX_T_BF16) return general_launch<bf16_t>(kind, g, ws, st);
   return general_launch<f16_t>(kind, g, ws, st);
 }
 
-// the backward workspace: [dz] [partial column sums] [one product's slabs, used by dx and then by dw on the same stream]
-struct BwdLayout { bool dz_own; long long dz, part, prod; int chunks; long long rows_per_chunk; };
+static int tiles_any(int kind, const VeexDense* d, const DenseGemm& g, const DtTensor& a, const DtTensor& b, void* ws, hipStream_t st) {
+  const TilePlan t = tile_plan(d, g.I, g.J, g.K);
+  DtGemm q = {};
+  q.a = a; q.b = b; q.I = g.I; q.J = g.J; q.K = g.K; q.k_per_split = t.per; q.splits = t.splits;
+  q.epi = g.epi;
+  q.slab = t.splits > 1 ? static_cast<float*>(ws) : nullptr;
+  q.vec_e = dense_epi_vec(g.epi, g.J, 8, trunk_elem_bytes(d->dtype));
+  if ((double)((g.I + t.tile - 1) / t.tile) * ((g.J + t.tile - 1) / t.tile) * t.splits > 2147483647.0) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
+  if (int rc = dense_tile_launch(d->dtype, kind != kKindDw, kind == kKindDx, t.tile, q, st)) return rc;
+  if (t.splits > 1) {
+    DenseGemm j = g;
+    j.slab = q.slab; j.splits = (int)t.splits; j.vec_e = q.vec_e;
+    return join_any(d->dtype, j, st);
+  }
+  return 0;
+}
+
+// x, w or dy as the tiles load it: where it lies, or packed into *at, which moves on
+static int tile_operand(const VeexDense* d, const void* p, long long ld, long long rows, int cols, char*& at, DtTensor& t, hipStream_t st) {
+  if (lies_well(d, p, ld, cols)) { t = {p, ld * 2, 0}; return 0; }
+  const long long plane = packed_plane(rows, cols);
+  t = {at, round8(cols) * 2, plane};
+  const int rc = dense_pack_launch(d->dtype, p, ld, rows, cols, at, plane, st);
+  at += planes_of(d) * plane;
+  return rc;
+}
+static long long tile_operand_bytes(const VeexDense* d, const void* p, long long ld, long long rows, int cols) {
+  return lies_well(d, p, ld, cols) ? 0 : packed_bytes(d, rows, cols);
+}
+
+static long long fwd_bytes(const VeexDense* d) {
+  long long b = product_bytes(kKindFwd, d);
+  if (uses_tiles(d)) b += tile_operand_bytes(d, d->x, d->ldx, d->rows, d->k) + tile_operand_bytes(d, d->w, d->n, d->k, d->n);
+  return b;
+}
+
+// the backward workspace: [dz: made here, or dy packed] [partial column sums] [x, w packed] [one product's slabs, used by dx and
+// then by dw on the same stream]
+struct BwdLayout { bool dz_own, tiles; long long dz, part, packed, prod; int chunks; long long rows_per_chunk; long long total() const { return dz + part + packed + prod; } };
 
 static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
   BwdLayout l = {};
   l.dz_own = d->activation != VEEX_ACT_NONE || drop.cut != 0u;
+  l.tiles = uses_tiles(d);
   const int strips = (d->n + 255) / 256;
   const long long want = std::max<long long>(1024 / strips, 1);
   l.rows_per_chunk = std::max<long long>(((d->rows + want - 1) / want + 7) / 8 * 8, 8);
   l.chunks = (int)((d->rows + l.rows_per_chunk - 1) / l.rows_per_chunk);
-  l.dz = l.dz_own ? align256(d->rows * d->n * trunk_elem_bytes(d->dtype)) : 0;
+  if (l.tiles) {
+    l.dz = l.dz_own ? packed_bytes(d, d->rows, d->n) : tile_operand_bytes(d, d->dy, d->n, d->rows, d->n);
+    l.packed = (d->dw != nullptr ? tile_operand_bytes(d, d->x, d->ldx, d->rows, d->k) : 0) + (d->dx != nullptr ? tile_operand_bytes(d, d->w, d->n, d->k, d->n) : 0);
+  } else {
+    l.dz = l.dz_own ? align256(d->rows * d->n * trunk_elem_bytes(d->dtype)) : 0;
+  }
   l.part = align256((long long)l.chunks * d->n * 4);
-  l.prod = std::max(product_bytes(kKindDx, d), product_bytes(kKindDw, d));
+  l.prod = std::max(d->dx != nullptr ? product_bytes(kKindDx, d) : 0, d->dw != nullptr ? product_bytes(kKindDw, d) : 0);
   return l;
 }
 
@@ -357,7 +461,7 @@ extern "C" {
 long long veex_dense_fwd_workspace_bytes(const VeexDense* d) {
   DropArgs drop;
   if (dense_check(d, "dense", drop) != 0) return -1;
-  return d->rows == 0 ? 0 : product_bytes(kKindFwd, d);
+  return d->rows == 0 ? 0 : fwd_bytes(d);
 }
 
 int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
@@ -365,18 +469,24 @@ int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
   if (int rc = dense_check(d, "dense", drop)) return rc;
   if (d->x == nullptr || d->w == nullptr || d->y == nullptr) { veex_set_error("dense: x, w and y are needed"); return VEEX_EINVAL; }
   if (d->rows == 0) return 0;
-  const long long need = product_bytes(kKindFwd, d);
-  if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need)) { veex_set_error("dense: a workspace of %lld bytes is needed", need); return VEEX_ENOMEM; }
+  const long long need = fwd_bytes(d);
+  if (need > 0 && (!trunk_aligned16(d->workspace) || d->workspace == nullptr || d->workspace_bytes < need)) {
+    veex_set_error("dense: a 16-byte aligned workspace of %lld bytes is needed", need); return VEEX_ENOMEM;
+  }
   DenseGemm g = dense_product(kKindFwd, d, nullptr);
   g.epi = {d->bias, d->residual, d->y, d->pre, d->activation, drop};
-  return product_launch(kKindFwd, d->dtype, g, d->workspace, st);
+  if (!uses_tiles(d)) return general_any(kKindFwd, d->dtype, g, d->workspace, st);
+  char* at = static_cast<char*>(d->workspace);
+  DtTensor x, w;
+  if (int rc = tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, st)) return rc;
+  if (int rc = tile_operand(d, d->w, d->n, d->k, d->n, at, w, st)) return rc;
+  return tiles_any(kKindFwd, d, g, x, w, at, st);
 }
 
 long long veex_dense_bwd_workspace_bytes(const VeexDense* d) {
   DropArgs drop;
   if (dense_check(d, "dense backward", drop) != 0) return -1;
-  const BwdLayout l = bwd_layout(d, drop);
-  return l.dz + l.part + l.prod;
+  return bwd_layout(d, drop).total();
 }
 
 int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
@@ -388,14 +498,18 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
   }
   if (d->rows == 0) { veex_set_error("dense backward: no rows"); return VEEX_EINVAL; }
   const BwdLayout l = bwd_layout(d, drop);
-  if (l.dz + l.part + l.prod > 0 && (d->workspace == nullptr || d->workspace_bytes < l.dz + l.part + l.prod)) {
-    veex_set_error("dense backward: a workspace of %lld bytes is needed", l.dz + l.part + l.prod); return VEEX_ENOMEM;
+  if (l.total() > 0 && (!trunk_aligned16(d->workspace) || d->workspace == nullptr || d->workspace_bytes < l.total())) {
+    veex_set_error("dense backward: a 16-byte aligned workspace of %lld bytes is needed", l.total()); return VEEX_ENOMEM;
   }
   char* ws = static_cast<char*>(d->workspace);
-  const void* dz = l.dz_own ? ws : d->dy;
+  const bool products = d->dx != nullptr || d->dw != nullptr;
+  const void* dz = l.dz_own ? ws : d->dy;                  // the general product's
+  DtTensor dzt = {ws, round8(d->n) * 2, packed_plane(d->rows, d->n)};    // the tiles'
   if (l.dz_own || d->db != nullptr) {
     DenseDz p = {};
-    p.dy = d->dy; p.pre = d->pre; p.dz = l.dz_own && (d->dx != nullptr || d->dw != nullptr) ? ws : nullptr;
+    p.dy = d->dy; p.pre = d->pre; p.dz = l.dz_own && products ? ws : nullptr;
+    p.ld = l.tiles ? round8(d->n) : d->n;
+    p.plane_bytes = l.tiles && d->dtype == VEEX_T_F32 ? dzt.plane_bytes : 0;
     p.part = d->db != nullptr ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
     p.rows = d->rows; p.rows_per_chunk = l.rows_per_chunk; p.n = d->n; p.act = d->activation; p.drop = drop;
     p.vec = d->n % 8 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
@@ -414,11 +528,29 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
       VEEX_CHECK_LAUNCH();
     }
   }
-  void* prod = ws + l.dz + l.part;
-  if (d->dx != nullptr)
-    if (int rc = product_launch(kKindDx, d->dtype, dense_product(kKindDx, d, dz), prod, st)) return rc;
-  if (d->dw != nullptr)
-    if (int rc = product_launch(kKindDw, d->dtype, dense_product(kKindDw, d, dz), prod, st)) return rc;
+  if (!products) return 0;
+  char* at = ws + l.dz + l.part;
+  char* slabs = at + l.packed;
+  if (!l.tiles) {
+    if (d->dx != nullptr)
+      if (int rc = general_any(kKindDx, d->dtype, dense_product(kKindDx, d, dz), slabs, st)) return rc;
+    if (d->dw != nullptr)
+      if (int rc = general_any(kKindDw, d->dtype, dense_product(kKindDw, d, dz), slabs, st)) return rc;
+    return 0;
+  }
+  DtTensor x, w;
+  if (!l.dz_own) {
+    char* p = ws;
+    if (int rc = tile_operand(d, d->dy, d->n, d->rows, d->n, p, dzt, st)) return rc;
+  }
+  if (d->dx != nullptr) {
+    if (int rc = tile_operand(d, d->w, d->n, d->k, d->n, at, w, st)) return rc;
+    if (int rc = tiles_any(kKindDx, d, dense_product(kKindDx, d, nullptr), dzt, w, slabs, st)) return rc;
+  }
+  if (d->dw != nullptr) {
+    if (int rc = tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, st)) return rc;
+    if (int rc = tiles_any(kKindDw, d, dense_product(kKindDw, d, nullptr), x, dzt, slabs, st)) return rc;
+  }
   return 0;
 }
 
