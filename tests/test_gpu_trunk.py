@@ -72,6 +72,20 @@ def test_dense_sizes(ops, m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m,k,n", [(300, 1000, 520), (1030, 264, 1001), (129, 4104, 260), (260, 5000, 136), (1500, 72, 2056), (2051, 513, 259)])
+def test_dense_large(ops, m, k, n, dt):
+    """On the 16-bit matrix cores: tiles that end inside the tensors, odd sizes that are packed, split reductions."""
+    _check_dense(ops, m, k, n, dt, "silu", True, 0.1, True)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m,k,n", [(1, 65536, 1), (1, 257, 1000), (2, 700, 264), (3, 1001, 77), (5, 640, 4096), (8, 4096, 136)])
+def test_dense_few_rows(ops, m, k, n, dt):
+    _check_dense(ops, m, k, n, dt, "gelu", True, 0.2, False)
+    _check_dense(ops, m, k, n, dt, "sigmoid", False, 0.0, True)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "silu", "sigmoid"])
 @pytest.mark.parametrize("residual,rate", [(False, 0.0), (True, 0.0), (False, 0.25), (True, 0.5)])
 def test_dense_epilogues(ops, dt, act, residual, rate):

@@ -23,17 +23,21 @@ __device__ __forceinline__ void dg_load(float (&r)[8], const DenseOperand& o, lo
   const long long row = row0 + (KC ? t >> 2 : 8 * (t & 7)), k = k0 + (KC ? 8 * (t & 3) : t >> 3);
   const long long n = (row < rows && k < k_end) ? (KC ? k_end - k : rows - row) : 0;
   const T* q = p + row * o.row_stride + k * o.k_stride;
-  if (vec && n >= 8) {
+  if (vec) {                   // (n is 0 or at least 8)
     constexpr int V = 16 / sizeof(T);
+    if (n <= 0) q = p;
 #pragma unroll
     for (int c = 0; c < 8 / V; ++c) {
       const Piece<T, V> x = piece_load<T, V>(q + c * V);
 #pragma unroll
-      for (int e = 0; e < V; ++e) r[c * V + e] = (float)x.v[e];
+      for (int e = 0; e < V; ++e) r[c * V + e] = n > 0 ? (float)x.v[e] : 0.f;
     }
-  } else {
+  } else {                     // (elements past the end read the tensor's first one: eight loads at once instead of eight branches)
+    T x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = e < n ? (float)q[e] : 0.f;
+    for (int e = 0; e < 8; ++e) x[e] = *(e < n ? q + e : p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = e < n ? (float)x[e] : 0.f;
   }
 }
 template <bool KC>
@@ -100,38 +104,113 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
   }
 }
 
-// Sum of the slabs in order, then the epilogue: 8 columns of one row a thread.
-template <typename T>
+// Sum of the slabs, then the epilogue: 8 columns of one row a thread.  Where the output alone is too small to fill the chip, SL
+// threads share an output block, each adding every SL'th slab up; the SL sums are added in order.
+template <typename T, int SL>
 __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
+  constexpr int OB = 256 / SL;                    // output blocks of a workgroup
+  __shared__ float part[SL > 1 ? SL * OB * 9 : 1];
   const int bpr = (g.J + 7) / 8;
-  const long long nb = g.I * bpr;
-  for (long long b = (long long)blockIdx.x * 256 + threadIdx.x; b < nb; b += (long long)gridDim.x * 256) {
+  const long long nb = g.I * bpr, stride = g.I * g.J;
+  const int ob = threadIdx.x % OB, sl = threadIdx.x / OB;
+  for (long long b0 = (long long)blockIdx.x * OB; b0 < nb; b0 += (long long)gridDim.x * OB) {
+    const long long b = min(b0 + ob, nb - 1);     // (every thread meets the barriers)
     const long long i = nb <= 0xFFFFFFFFll ? (long long)((unsigned)b / (unsigned)bpr) : b / bpr;
     const int j = 8 * (int)(b - i * bpr);
     const float* s = g.slab + i * g.J + j;
-    const long long stride = g.I * g.J;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
     if (g.J % 4 == 0) {
-#pragma unroll 4
-      for (int z = 0; z < g.splits; ++z) {
+      const bool two = j + 4 < g.J;
+#pragma unroll 8
+      for (int z = sl; z < g.splits; z += SL) {
         const float4 x = *reinterpret_cast<const float4*>(s + z * stride);
+        const float4 t = *reinterpret_cast<const float4*>(s + z * stride + (two ? 4 : 0));
         v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        if (j + 4 < g.J) {
-          const float4 t = *reinterpret_cast<const float4*>(s + z * stride + 4);
-          v[4] += t.x; v[5] += t.y; v[6] += t.z; v[7] += t.w;
-        }
+        v[4] += t.x; v[5] += t.y; v[6] += t.z; v[7] += t.w;
       }
     } else {
-      for (int z = 0; z < g.splits; ++z)
+#pragma unroll 2
+      for (int z = sl; z < g.splits; z += SL)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (j + e < g.J) v[e] += s[z * stride + e];
+        for (int e = 0; e < 8; ++e) v[e] += s[z * stride + min(e, g.J - 1 - j)];
     }
-    unsigned w[4] = {0u, 0u, 0u, 0u};
-    if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
-    dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e && g.J % 8 == 0, w);
+    if (SL > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) part[(sl * OB + ob) * 9 + e] = v[e];
+      __syncthreads();
+      if (sl == 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = 0.f;
+          for (int q = 0; q < SL; ++q) v[e] += part[(q * OB + ob) * 9 + e];
+        }
+    }
+    if (sl == 0 && b0 + ob < nb) {
+      unsigned w[4] = {0u, 0u, 0u, 0u};
+      if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
+      dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e && g.J % 8 == 0, w);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows (up to 8): the weights are read once and everything else is small, so the bound is their bandwidth.  A thread owns V
+// columns (16 bytes of a 16-byte aligned row of w, else one) and every KL'th k of the block's range, 8 loads in flight; KL threads a
+// column meet in LDS.  Blocks split k until there are some thousand of them.  w [K][N] as it lies; x through LDS, as fp32.
+// ---------------------------------------------------------------------------------------------------------------
+#define DF_KB 256        // k's of x in LDS at a time
+template <typename T, int R, bool VEC>
+__global__ __launch_bounds__(256) void dense_few_rows_kernel(DenseGemm g) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+  constexpr int CL = VEC ? 16 : 64, KL = 256 / CL;          // column threads, k threads: 256 bytes of a row, or 64 elements
+  __shared__ float xs[R][DF_KB];
+  __shared__ float part[KL][CL * V + 1];
+  const int cl = threadIdx.x % CL, kl = threadIdx.x / CL;
+  const int j = blockIdx.x * CL * V + cl * V;
+  const bool ok = j < g.J;                                   // (VEC: J is a multiple of V)
+  const T* x = static_cast<const T*>(g.a.p);
+  const T* w = static_cast<const T*>(g.b.p) + (ok ? j : 0);
+  const long long k_begin = blockIdx.y * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
+  float acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[r][e] = 0.f;
+  for (long long k0 = k_begin; k0 < k_end; k0 += DF_KB) {
+    const int n = (int)min((long long)DF_KB, k_end - k0);
+    __syncthreads();
+    for (int t = threadIdx.x; t < R * DF_KB; t += 256) {
+      const int r = t / DF_KB, k = t % DF_KB;
+      xs[r][k] = r < g.I && k < n ? (float)x[r * g.a.row_stride + k0 + k] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int k = kl; k < n; k += KL) {
+      const Piece<T, V> p = piece_load<T, V>(w + (k0 + k) * g.b.k_stride);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float a = xs[r][k];
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[r][e] = fmaf(a, (float)p.v[e], acc[r][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[kl][cl * V + e] = acc[r][e];
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (r < g.I && c < CL * V && blockIdx.x * CL * V + c < g.J) {
+      float a = 0.f;
+#pragma unroll
+      for (int q = 0; q < KL; ++q) a += part[q][c];
+      g.slab[((long long)blockIdx.y * g.I + r) * g.J + blockIdx.x * CL * V + c] = a;
+    }
   }
 }
 
@@ -144,6 +223,7 @@ struct DenseDz {
   void* dz;              // null: only the sums.  Rows of ld columns (the ones behind n as zeros), or fp32 as planes
   long long ld, plane_bytes;     // plane_bytes 0: dz in the tensors' type
   float* part;           // [chunks][N], null: none
+  void* db;              // with one chunk: the sums themselves, instead of part
   long long rows, rows_per_chunk;
   int n, act, vec;
   DropArgs drop;
@@ -216,7 +296,7 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
       }
     }
   }
-  if (p.part == nullptr) return;
+  if (p.part == nullptr && p.db == nullptr) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) s[ty][8 * tx + e] = sum[e];
   __syncthreads();
@@ -225,7 +305,8 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
     float a = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) a += s[q][threadIdx.x];
-    p.part[(long long)blockIdx.y * p.n + col] = a;
+    if (p.db != nullptr) static_cast<T*>(p.db)[col] = (T)a;
+    else p.part[(long long)blockIdx.y * p.n + col] = a;
   }
 }
 
@@ -277,7 +358,12 @@ static long long general_bytes(long long I, int J, long long K) {
 template <typename T>
 static int join_launch(const DenseGemm& g, hipStream_t st) {
   const long long nb = g.I * ((g.J + 7) / 8);
-  hipLaunchKernelGGL((dense_join_kernel<T>), dim3((unsigned)std::min<long long>((nb + 255) / 256, 1 << 16)), dim3(256), 0, st, g);
+#define DJ_GO(SL) hipLaunchKernelGGL((dense_join_kernel<T, SL>), dim3((unsigned)std::min<long long>((nb + 256 / SL - 1) / (256 / SL), 1 << 16)), dim3(256), 0, st, g)
+  // shared output blocks while there are fewer than two workgroups a CU: 100 slabs of 100 columns 34 -> 5 us
+  if (nb >= 512 * 256 || g.splits < 8) DJ_GO(1);
+  else if (nb >= 512 * 32 || g.splits < 32) DJ_GO(8);
+  else DJ_GO(32);
+#undef DJ_GO
   VEEX_CHECK_LAUNCH();
   return 0;
 }
@@ -320,6 +406,49 @@ static int dense_check(const VeexDense* d, const char* who, DropArgs& drop) {
   return 0;
 }
 
+// ---- few rows -------------------------------------------------------------------------------------------------------
+static const int kFewRows = 8;
+
+template <typename T>
+static bool few_vec(const DenseGemm& g) { return operand_vec(g.b, g.J, sizeof(T)); }
+
+// about 1024 blocks, at least 64 k's each
+static void few_split(const DenseGemm& g, bool vec, int elem, int& splits, long long& per) {
+  const long long strips = vec ? (g.J * elem + 255) / 256 : (g.J + 63) / 64;
+  const long long s = std::max<long long>(std::min<long long>((1023 + strips) / strips, g.K / 64), 1);
+  per = (g.K + s - 1) / s;
+  splits = (int)((g.K + per - 1) / per);
+}
+
+template <typename T>
+static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
+  const bool vec = few_vec<T>(g);
+  few_split(g, vec, sizeof(T), g.splits, g.k_per_split);
+  g.slab = static_cast<float*>(ws);
+  g.vec_e = dense_epi_vec(g.epi, g.J, 8, sizeof(T));
+  const dim3 grid((unsigned)(vec ? (g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64), (unsigned)g.splits);
+#define DF_GO(R)                                                                                              \
+  if (vec) hipLaunchKernelGGL((dense_few_rows_kernel<T, R, true>), grid, dim3(256), 0, st, g);                 \
+  else hipLaunchKernelGGL((dense_few_rows_kernel<T, R, false>), grid, dim3(256), 0, st, g);
+  if (g.I == 1) { DF_GO(1) }
+  else if (g.I == 2) { DF_GO(2) }
+  else if (g.I <= 4) { DF_GO(4) }
+  else { DF_GO(8) }
+#undef DF_GO
+  VEEX_CHECK_LAUNCH();
+  return join_launch<T>(g, st);
+}
+
+// the weights are worth a second launch to join: from 2^16 of them on (below, one tile of the general product is as quick)
+static bool few_rows(const VeexDense* d) { return d->rows <= kFewRows && (long long)d->k * d->n >= (1 << 16); }
+
+static long long few_bytes(const VeexDense* d, const DenseGemm& g) {
+  const int elem = trunk_elem_bytes(d->dtype);
+  int s; long long per;
+  few_split(g, operand_vec(g.b, g.J, elem), elem, s, per);
+  return align256((long long)s * g.I * g.J * 4);
+}
+
 // ---- large products -------------------------------------------------------------------------------------------------
 // A layer whose products have at least this many multiplications goes to dense_tile.hip: below it the packing and the tiles' edges
 // cost more than the fp32 MFMA of the general product.
@@ -327,6 +456,7 @@ static const double kTileMin16 = 1 << 25, kTileMin32 = 1 << 27;
 
 static bool uses_tiles(const VeexDense* d) {
   const double work = (double)d->rows * d->k * d->n;
+  if (d->rows <= kFewRows) return false;
   // a tile addresses its operand by 32 bits from its first row on: 256 rows of up to 4 MB, 64 k's of up to 16 MB
   const long long widest = std::max<long long>(std::max<long long>(d->k, d->n), d->ldx);
   return work >= (d->dtype == VEEX_T_F32 ? kTileMin32 : kTileMin16) && widest < (1 << 21);
@@ -386,6 +516,7 @@ static DenseGemm dense_product(int kind, const VeexDense* d, const void* dz) {
 // bytes of one product's slabs
 static long long product_bytes(int kind, const VeexDense* d) {
   const DenseGemm g = dense_product(kind, d, nullptr);
+  if (kind == kKindFwd && few_rows(d)) return few_bytes(d, g);
   if (!uses_tiles(d)) return general_bytes(g.I, g.J, g.K);
   const TilePlan t = tile_plan(d, g.I, g.J, g.K);
   return t.splits > 1 ? align256((long long)t.splits * g.I * g.J * 4) : 0;
@@ -443,7 +574,8 @@ static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
   l.tiles = uses_tiles(d);
   const int strips = (d->n + 255) / 256;
   const long long want = std::max<long long>(1024 / strips, 1);
-  l.rows_per_chunk = std::max<long long>(((d->rows + want - 1) / want + 7) / 8 * 8, 8);
+  // (up to 64 rows one chunk: eight turns, and no second launch to add partial rows)
+  l.rows_per_chunk = d->rows <= 64 ? 64 : std::max<long long>(((d->rows + want - 1) / want + 7) / 8 * 8, 8);
   l.chunks = (int)((d->rows + l.rows_per_chunk - 1) / l.rows_per_chunk);
   if (l.tiles) {
     l.dz = l.dz_own ? packed_bytes(d, d->rows, d->n) : tile_operand_bytes(d, d->dy, d->n, d->rows, d->n);
@@ -475,6 +607,11 @@ int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
   }
   DenseGemm g = dense_product(kKindFwd, d, nullptr);
   g.epi = {d->bias, d->residual, d->y, d->pre, d->activation, drop};
+  if (few_rows(d)) {
+    if (d->dtype == VEEX_T_F32) return few_launch<float>(g, d->workspace, st);
+    if (d->dtype == VEEX_T_BF16) return few_launch<bf16_t>(g, d->workspace, st);
+    return few_launch<f16_t>(g, d->workspace, st);
+  }
   if (!uses_tiles(d)) return general_any(kKindFwd, d->dtype, g, d->workspace, st);
   char* at = static_cast<char*>(d->workspace);
   DtTensor x, w;
@@ -510,17 +647,18 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
     p.dy = d->dy; p.pre = d->pre; p.dz = l.dz_own && products ? ws : nullptr;
     p.ld = l.tiles ? round8(d->n) : d->n;
     p.plane_bytes = l.tiles && d->dtype == VEEX_T_F32 ? dzt.plane_bytes : 0;
-    p.part = d->db != nullptr ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
+    p.db = l.chunks == 1 ? d->db : nullptr;
+    p.part = d->db != nullptr && l.chunks > 1 ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
     p.rows = d->rows; p.rows_per_chunk = l.rows_per_chunk; p.n = d->n; p.act = d->activation; p.drop = drop;
     p.vec = d->n % 8 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
-    if (p.dz != nullptr || p.part != nullptr) {
+    if (p.dz != nullptr || d->db != nullptr) {
       const dim3 grid((d->n + 255) / 256, l.chunks);
       if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_dz_kernel<float>), grid, dim3(256), 0, st, p);
       else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_dz_kernel<bf16_t>), grid, dim3(256), 0, st, p);
       else hipLaunchKernelGGL((dense_dz_kernel<f16_t>), grid, dim3(256), 0, st, p);
       VEEX_CHECK_LAUNCH();
     }
-    if (d->db != nullptr) {
+    if (p.part != nullptr) {
       const dim3 grid((d->n + 63) / 64);
       if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_db_kernel<float>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
       else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_db_kernel<bf16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
