@@ -10,7 +10,7 @@
 // The general product: 64 x 64 tiles, 4 waves of one 32 x 32 accumulator, fp32 MFMA (a product of two 16-bit numbers is exact
 // there, so one kernel serves every type).  Operand tiles are staged through registers into [k][row] LDS; a tensor whose rows
 // are whole aligned pieces loads 8 elements at a time, others element by element.  The MFMA takes B's rows as its first operand, so
-// that a lane ends up with 4 consecutive columns of one row: one store, one block of dropout numbers.
+// that a lane ends up with 4 consecutive columns of one row.
 // ---------------------------------------------------------------------------------------------------------------
 #define DG_LD 68     // floats per LDS row: 64 + one 16-byte piece
 
@@ -84,32 +84,46 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Bs[cur][(2 * s + lh) * DG_LD + wj * 32 + l31],
                                                  As[cur][(2 * s + lh) * DG_LD + wi * 32 + l31], acc, 0, 0, 0);
   }
-  const long long i = i0 + wi * 32 + l31;
-  if (i >= g.I) return;
+  // The way out, as in dense_tile.hip: each wave turns its 32 x 32 block round in LDS, so that a lane holds 8 columns of a row
+  __syncthreads();
+  float* strip = (wave < 2 ? As[wave] : Bs[wave - 2]);         // 32 rows of 36 floats
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int j = j0 + wj * 32 + 8 * q + 4 * lh;
-    if (j >= g.J) continue;
-    float v[4] = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<float4*>(strip + l31 * 36 + 8 * q + 4 * lh) = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+  __syncthreads();
+  const unsigned long long base = drop_base(g.epi.drop);
+#pragma unroll 1
+  for (int r = lane >> 2; r < 32; r += 16) {
+    const long long i = i0 + wi * 32 + r;
+    const int j = j0 + wj * 32 + 8 * (lane & 3);
+    if (i >= g.I || j >= g.J) continue;
+    const float4 lo = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3)), hi = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3) + 4);
+    float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     if (SPLIT) {
       float* s = g.slab + ((long long)blockIdx.y * g.I + i) * g.J + j;
+      if (g.J % 4 == 0) {
+        *reinterpret_cast<float4*>(s) = lo;
+        if (j + 4 < g.J) *reinterpret_cast<float4*>(s + 4) = hi;
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e < g.J) s[e] = v[e];
+        for (int e = 0; e < 8; ++e)
+          if (j + e < g.J) s[e] = v[e];
+      }
     } else {
       unsigned w[4] = {0u, 0u, 0u, 0u};
-      if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
-      dense_epilogue<T, 4>(g.epi, v, i, j, g.J, g.vec_e, w + (lh ? 2 : 0));
+      if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
+      dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e, w);
     }
   }
 }
 
 // Sum of the slabs, then the epilogue: 8 columns of one row a thread.  Where the output alone is too small to fill the chip, SL
-// threads share an output block, each adding every SL'th slab up; the SL sums are added in order.
+// threads share an output block, each adding every SL'th slab up; the SL sums are added in a fixed order.
 template <typename T, int SL>
 __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
-  constexpr int OB = 256 / SL;                    // output blocks of a workgroup
-  __shared__ float part[SL > 1 ? SL * OB * 9 : 1];
+  constexpr int OB = 256 / SL;                    // output blocks of a workgroup; a wave holds all of them (SL > 1), 64 / OB times
+  static_assert(SL == 1 || OB <= 64, "");
+  __shared__ float part[SL > 1 ? 4 * OB * 9 : 1];
   const int bpr = (g.J + 7) / 8;
   const long long nb = g.I * bpr, stride = g.I * g.J;
   const int ob = threadIdx.x % OB, sl = threadIdx.x / OB;
@@ -137,21 +151,23 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
         for (int e = 0; e < 8; ++e) v[e] += s[z * stride + min(e, g.J - 1 - j)];
     }
     if (SL > 1) {
-      __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[(sl * OB + ob) * 9 + e] = v[e];
+      for (int o = OB; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += __shfl_xor(v[e], o);
+      __syncthreads();
+      if ((threadIdx.x & 63) < OB)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[((threadIdx.x >> 6) * OB + ob) * 9 + e] = v[e];
       __syncthreads();
       if (sl == 0)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = 0.f;
-          for (int q = 0; q < SL; ++q) v[e] += part[(q * OB + ob) * 9 + e];
-        }
+        for (int e = 0; e < 8; ++e) v[e] = part[ob * 9 + e] + part[(OB + ob) * 9 + e] + (part[(2 * OB + ob) * 9 + e] + part[(3 * OB + ob) * 9 + e]);
     }
     if (sl == 0 && b0 + ob < nb) {
       unsigned w[4] = {0u, 0u, 0u, 0u};
       if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
-      dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e && g.J % 8 == 0, w);
+      dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e, w);
     }
   }
 }
@@ -271,9 +287,7 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[e] = drop_u16(w, e) >= p.drop.cut ? d[e] * p.drop.scale : 0.f;
       }
-      if (p.act != VEEX_ACT_NONE)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = e < n ? d[e] * dense_act_grad(z[e], p.act) : 0.f;
+      if (p.act != VEEX_ACT_NONE) dense_act_grad<T, 8>(d, z, p.act);        // (finite at the zeros behind the last column)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += d[e];
       if (p.dz != nullptr && p.plane_bytes != 0) {
@@ -379,7 +393,7 @@ static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
   g.slab = static_cast<float*>(ws);
   g.vec_a = operand_vec(g.a, kind == kKindDw ? g.I : g.K, sizeof(T));
   g.vec_b = operand_vec(g.b, kind == kKindDx ? g.K : g.J, sizeof(T));
-  g.vec_e = dense_epi_vec(g.epi, g.J, g.splits > 1 ? 8 : 4, sizeof(T));
+  g.vec_e = dense_epi_vec(g.epi, g.J, 8, sizeof(T));
   const long long tiles = (g.I + 63) / 64 * ((g.J + 63) / 64);
   if (tiles > 0x7FFFFFFFll) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
   const dim3 grid((unsigned)tiles, (unsigned)g.splits);

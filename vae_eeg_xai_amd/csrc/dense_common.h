@@ -16,29 +16,87 @@ struct DenseEpi {
   DropArgs drop;         // cut 0: none
 };
 
+// The activations, W values at a time with the choice outside the loops: a small kernel's time is largely the fetch of its code, and
+// an activation's code chosen per value, times the unrolled values, was most of it (512x28x4096 fp32: 22 us so, 8 us now).
+//
+// A 16-bit result keeps 11 bits at most, so there the hardware's exp2 and reciprocal (1 ulp) serve; fp32 takes the accurate expf
+// and division.  gelu needs Phi(z) = erfc(-z / sqrt 2) / 2: with x = |z| / sqrt 2 and t = 1 / (1 + p x), erfc(x) = P(t) t exp(-x^2), P
+// fitted here to exp(x^2) erfc(x) / t on 0 <= x <= 9.5 for the least largest relative error (7.3e-7 with 7 coefficients, 1.7e-8
+// with 9; fp32 rounding brings the latter to 3.5e-7).  The derivative's exp(-z^2 / 2) is the same exponential.
+template <typename T> __device__ __forceinline__ float act_exp(float x) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(x * 1.44269504f);
+  else return expf(x);
+}
+template <typename T> __device__ __forceinline__ float act_rcp(float x) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(x);
+  else return 1.f / x;
+}
+// Phi(z), and e = exp(-z^2 / 2)
+template <typename T> __device__ __forceinline__ float act_phi(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678f, t = act_rcp<T>(fmaf(0.37f, x, 1.f));
+  float q;
+  if constexpr (sizeof(T) == 2) {
+    q = -0.142551705f;
+    q = fmaf(q, t, 0.435660362f); q = fmaf(q, t, -0.186432138f); q = fmaf(q, t, 0.31740576f);
+    q = fmaf(q, t, 0.152655855f); q = fmaf(q, t, 0.214882717f); q = fmaf(q, t, 0.20837988f);
+  } else {
+    q = 0.0619231425f;
+    q = fmaf(q, t, -0.303273201f); q = fmaf(q, t, 0.486842126f); q = fmaf(q, t, -0.285312116f); q = fmaf(q, t, 0.310802102f);
+    q = fmaf(q, t, 0.106520303f); q = fmaf(q, t, 0.206254035f); q = fmaf(q, t, 0.207429841f); q = fmaf(q, t, 0.208813742f);
+  }
+  e = act_exp<T>(-0.5f * z * z);
+  q *= 0.5f * t * e;
+  return z > 0.f ? 1.f - q : q;
+}
+
 // A relu unit passes a NaN on (a comparison with it is false), as the formula's where(z < 0, 0, z) does.
-__device__ __forceinline__ float dense_act(float z, int act) {
+template <typename T, int W>
+__device__ __forceinline__ void dense_act(float (&v)[W], int act) {
   switch (act) {
-    case VEEX_ACT_RELU: return z < 0.f ? 0.f : z;
-    case VEEX_ACT_GELU: return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
-    case VEEX_ACT_SILU: return z * (1.f / (1.f + expf(-z)));
-    case VEEX_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
-    default: return z;
+    case VEEX_ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+      break;
+    case VEEX_ACT_GELU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) { float x; v[e] *= act_phi<T>(v[e], x); }
+      break;
+    case VEEX_ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] *= act_rcp<T>(1.f + act_exp<T>(-v[e]));
+      break;
+    case VEEX_ACT_SIGMOID:
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = act_rcp<T>(1.f + act_exp<T>(-v[e]));
+      break;
+    default: break;
   }
 }
-// d act / dz; for relu, s may be z or the kept output (both are <= 0 exactly where nothing passes)
-__device__ __forceinline__ float dense_act_grad(float s, int act) {
+// d[e] *= d act / dz at s[e]; for relu, s may be z or the kept output (both are <= 0 exactly where nothing passes)
+template <typename T, int W>
+__device__ __forceinline__ void dense_act_grad(float (&d)[W], const float (&s)[W], int act) {
   switch (act) {
-    case VEEX_ACT_RELU: return s <= 0.f ? 0.f : 1.f;
-    case VEEX_ACT_GELU: return 0.5f * (1.f + erff(s * 0.70710678118654752f)) + s * expf(-0.5f * s * s) * 0.39894228040143268f;
-    case VEEX_ACT_SILU: { const float e = 1.f / (1.f + expf(-s)); return e * (1.f + s * (1.f - e)); }
-    case VEEX_ACT_SIGMOID: { const float e = 1.f / (1.f + expf(-s)); return e * (1.f - e); }
-    default: return 1.f;
+    case VEEX_ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) d[e] = s[e] <= 0.f ? 0.f : d[e];
+      break;
+    case VEEX_ACT_GELU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) { float x; const float phi = act_phi<T>(s[e], x); d[e] *= fmaf(s[e] * 0.39894228f, x, phi); }
+      break;
+    case VEEX_ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < W; ++e) { const float x = act_rcp<T>(1.f + act_exp<T>(-s[e])); d[e] *= x * fmaf(s[e], 1.f - x, 1.f); }
+      break;
+    case VEEX_ACT_SIGMOID:
+#pragma unroll
+      for (int e = 0; e < W; ++e) { const float x = act_rcp<T>(1.f + act_exp<T>(-s[e])); d[e] *= x * (1.f - x); }
+      break;
+    default: break;
   }
 }
 
-// Columns j .. j + W - 1 (W = 4 or 8, j a multiple of W) of row i.  half words: u16 of column j + e is words[(e0 + e) >> 1]'s
-// half (e & 1), where e0 = j & 7 (the caller passes the Philox words of the block of 8 that holds them).
+// Columns j .. j + W - 1 (W = 8, j a multiple of 8) of row i; words: the row's dropout words of that block.
 template <typename T, int W>
 __device__ __forceinline__ void dense_epilogue(const DenseEpi& ep, float (&v)[W], long long i, int j, int J, bool vec,
                                                const unsigned* words) {
@@ -78,8 +136,10 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& ep, float (&v)[W]
   }
   float o[W];
 #pragma unroll
+  for (int e = 0; e < W; ++e) o[e] = v[e];
+  dense_act<T, W>(o, ep.act);
+#pragma unroll
   for (int e = 0; e < W; ++e) {
-    o[e] = dense_act(v[e], ep.act);
     if (ep.drop.cut != 0u) {
       const unsigned u = (e & 1) ? words[e >> 1] >> 16 : words[e >> 1] & 0xFFFFu;
       o[e] = u >= ep.drop.cut ? o[e] * ep.drop.scale : 0.f;

@@ -224,31 +224,34 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
 
   if (PL == 3) dt_mend<AKC, BKC, MT, NT>(g, acc, i0 + wi * MT * 32, j0 + wj * NT * 32, k_begin, k_end, lane);
 
-  // The way out: each wave turns its 32-row strips round through a corner of LDS of its own (fp32, 16-byte pieces swizzled by the
+  // The way out: each wave turns 64 rows at a time round through a corner of LDS of its own (fp32, 16-byte pieces swizzled by the
   // row), so that a lane holds 8 consecutive columns of a row and eight lanes (four for 32 columns) write a whole line.  Straight
   // from the accumulators' layout a store would touch 32 lines.
   constexpr int CW = NT * 32, OCT = CW / 8, RPP = 64 / OCT;      // columns, their blocks of 8, rows a pass
-  static_assert(WAVES * 32 * CW * 4 <= 2 * STAGE, "the strips fit the stages");
+  constexpr int SM = MT < 2 ? MT : 2;                            // 32-row blocks a strip holds
+  static_assert(WAVES * SM * 32 * CW * 4 <= 2 * STAGE && MT % SM == 0, "the strips fit the stages");
   __syncthreads();                                               // every wave is done with the operand tiles
-  DT_LDS char* strip = smem + wave * 32 * CW * 4;
+  DT_LDS char* strip = smem + wave * SM * 32 * CW * 4;
   const int l31 = lane & 31, lh = lane >> 5;
   const unsigned long long base = drop_base(g.epi.drop);
 #pragma unroll
-  for (int mi = 0; mi < MT; ++mi) {
+  for (int m0 = 0; m0 < MT; m0 += SM) {
 #pragma unroll
-    for (int nj = 0; nj < NT; ++nj)
+    for (int mi = m0; mi < m0 + SM; ++mi)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<DT_LDS dt_f4*>(strip + l31 * CW * 4 + (((nj * 8 + 2 * q + lh) ^ (l31 & 7)) * 16)) =
-            dt_f4{acc[mi][nj][4 * q], acc[mi][nj][4 * q + 1], acc[mi][nj][4 * q + 2], acc[mi][nj][4 * q + 3]};
+      for (int nj = 0; nj < NT; ++nj)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<DT_LDS dt_f4*>(strip + ((mi - m0) * 32 + l31) * CW * 4 + (((nj * 8 + 2 * q + lh) ^ (l31 & 7)) * 16)) =
+              dt_f4{acc[mi][nj][4 * q], acc[mi][nj][4 * q + 1], acc[mi][nj][4 * q + 2], acc[mi][nj][4 * q + 3]};
     dt_wave_sync();
 #pragma unroll 1
-    for (int r0 = 0; r0 < 32; r0 += RPP) {
+    for (int r0 = 0; r0 < 32 * SM; r0 += RPP) {
       const int r = r0 + lane / OCT, o = lane % OCT;
       const dt_f4 lo = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o) ^ (r & 7)) * 16));
       const dt_f4 hi = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o + 1) ^ (r & 7)) * 16));
       float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      const long long i = i0 + (wi * MT + mi) * 32 + r;
+      const long long i = i0 + (wi * MT + m0) * 32 + r;
       const int j = j0 + wj * CW + 8 * o;
       if (i >= g.I || j >= g.J) continue;
       if (g.slab != nullptr) {
