@@ -9,7 +9,8 @@
 // read as the MFMA wants it, 8 consecutive k a lane; one whose row index is contiguous lies as [k][128 rows] and is
 // read through the transposing LDS read.  The load writes LDS in lane order, so the bank swizzle is applied to the address
 // that a lane loads from: 16-byte piece q of an LDS row holds the tensor's piece q ^ s(row).
-//   [row][64]: s = row & 7;  [row][32]: s = (row >> 1) & 3;  [k][128]: s = (k & 3) << 2
+//   [row][64]: s = (row >> 1) & 7;  [row][32]: s = (row >> 2) & 3;  [k][128]: s = (k & 3) << 2
+// (16 lanes read at a time, 256 bytes: 16 consecutive rows of one piece have to fall on 16 different ones)
 //
 // Needs: 16-byte aligned operands and rows; a k-contiguous operand's K a multiple of 8.  Pieces past a tensor's end
 // are sent out of the buffer's range and arrive as zeros.
@@ -19,9 +20,19 @@
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float dt_f4 __attribute__((ext_vector_type(4)));
+typedef unsigned dt_u4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 #define DT_LDS __attribute__((address_space(3)))
+#ifndef DT_L_BK
+#define DT_L_BK 32
+#define DT_L_ST 4
+#define DT_S_BK 32
+#define DT_S_ST 4
+#define DT_S_W 2, 2
+#define DT_X3_ST 3
+#define DT_X3_W 2, 4
+#endif
 #define DT_OOB 0xFFFFFFF0u      // past every buffer's end
 
 __device__ __forceinline__ f32x16 dt_mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -37,6 +48,7 @@ struct DtOperand {
   static constexpr int LOADS = BYTES / 1024 / WAVES;           // 1024-byte loads of a wave, per plane
   static_assert(BYTES % (1024 * WAVES) == 0, "whole loads for every wave");
   static_assert(KC ? (BK == 64 || BK == 32) : ROWS % 128 == 0, "layouts with a swizzle");
+  static constexpr int COUNT = PL * LOADS;                     // loads of a wave, a stage
   static constexpr int ROWB = BK * 2;
 
   const char* base;                // (row0, k = 0) of plane 0
@@ -45,7 +57,7 @@ struct DtOperand {
   unsigned voff[LOADS], piece_k[LOADS];
   int wave, lane;
 
-  __device__ __forceinline__ static int swz(int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; }
+  __device__ __forceinline__ static int swz(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
 
   __device__ __forceinline__ void init(const DtTensor& t, long long row0, long long rows, long long K_, int wave_, int lane_) {
     wave = wave_; lane = lane_; ld = t.ld_bytes; plane = t.plane_bytes; K = K_; rows_left = rows - row0;
@@ -66,20 +78,16 @@ struct DtOperand {
     }
   }
 
-  // loads the BK reduction indices from k0 on (those at or past k_end arrive as zeros) into the tile at lds
-  __device__ __forceinline__ void load(DT_LDS char* lds, long long k0, long long k_end) const {
-    const bool whole = k0 + BK <= k_end;
-#pragma unroll
-    for (int pl = 0; pl < PL; ++pl) {
-      const char* p = base + pl * plane + (KC ? k0 * 2 : k0 * ld);
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)0xFFFFFFE0u, 0x00020000);
-#pragma unroll
-      for (int u = 0; u < LOADS; ++u) {
-        unsigned v = voff[u];
-        if (!whole) v = k0 + piece_k[u] < k_end ? v : DT_OOB;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DT_LDS void*)(lds + pl * BYTES + (u * WAVES + wave) * 1024), 16, v, 0, 0, 0);
-      }
-    }
+  // load c (of COUNT) of the tile that holds the BK reduction indices from k0 on (those at or past k_end arrive as zeros)
+  __device__ __forceinline__ void load(int c, DT_LDS char* lds, long long k0, long long k_end) const {
+    const int pl = c / LOADS, u = c % LOADS;
+    const uint64_t at = reinterpret_cast<uint64_t>(base + pl * plane + (KC ? k0 * 2 : k0 * ld));
+    const dt_u4 r = {(unsigned)at, (unsigned)(at >> 32) & 0xFFFFu, 0xFFFFFFE0u, 0x00020000u};
+    const unsigned v = k0 + piece_k[u] < k_end ? voff[u] : DT_OOB;
+    // (asm: the compiler's own load into LDS makes it wait for that load before the next LDS read of whatever buffer, which
+    // leaves nothing in flight.  No register is written, and m0 only here; the wait is the one before the barrier.)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 : : "s"((unsigned)(uintptr_t)(lds + pl * BYTES + (u * WAVES + wave) * 1024)), "v"(v), "s"(r) : "memory");
   }
 
   // the 8 k's of lane half lh at k step ks (16 k's), of the 32 rows from `row` on (a multiple of 32)
@@ -152,7 +160,7 @@ __device__ __forceinline__ void dt_mend(const DtGemm& g, f32x16 (&acc)[MT][NT], 
     }
 }
 
-template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int WM, int WN>
+template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int ST, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
   constexpr int WAVES = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
   typedef DtOperand<BM, BK, AKC, PL, WAVES> OpA;
@@ -180,45 +188,66 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  a.load(smem, k_begin, k_end);
-  b.load(smem + PL * OpA::BYTES, k_begin, k_end);
-  int cur = 0;
-  for (long long k0 = k_begin; k0 < k_end; k0 += BK, cur ^= 1) {
-    // this step's tiles have landed, and every wave is done with the other buffer
-    __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0)
-    __syncthreads();
-    DT_LDS char* sa = smem + cur * STAGE;
-    DT_LDS char* sb = sa + PL * OpA::BYTES;
-    if (k0 + BK < k_end) {
-      DT_LDS char* na = smem + (cur ^ 1) * STAGE;
-      a.load(na, k0 + BK, k_end);
-      b.load(na + PL * OpA::BYTES, k0 + BK, k_end);
+  // ST stages in a ring: while step t is computed, the loads of the ST - 1 steps behind it are on their way (past the end they
+  // fetch nothing, so that the count of loads in flight stays the same)
+  constexpr int COUNT = OpA::COUNT + OpB::COUNT, KS = BK / 16, PER = (COUNT + KS - 1) / KS, MF = MT * NT * (PL == 1 ? 1 : 6);
+  static_assert(ST >= 3 && KS % 2 == 0, "");
+  auto load = [&](int c, int stage, long long k0) {
+    if (c < OpA::COUNT) a.load(c, smem + stage * STAGE, k0, k_end);
+    else if (c < COUNT) b.load(c - OpA::COUNT, smem + stage * STAGE + PL * OpA::BYTES, k0, k_end);
+  };
+  V8 av[2][PL][MT], bv[2][PL][NT];
+  auto read = [&](int buf, const DT_LDS char* st, int ks) {
+#pragma unroll
+    for (int pl = 0; pl < PL; ++pl) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) bv[buf][pl][j] = b.template frag<V8>(st + PL * OpA::BYTES, pl, (wj * NT + j) * 32, ks);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) av[buf][pl][i] = a.template frag<V8>(st, pl, (wi * MT + i) * 32, ks);
     }
+  };
 #pragma unroll
-    for (int ks = 0; ks < BK / 16; ++ks) {
-      V8 av[PL][MT], bv[PL][NT];
+  for (int t = 0; t < ST - 1; ++t)
 #pragma unroll
-      for (int pl = 0; pl < PL; ++pl) {
+    for (int c = 0; c < COUNT; ++c) load(c, t, k_begin + t * BK);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((ST - 2) * COUNT) : "memory");
+  read(0, smem, 0);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) av[pl][i] = a.template frag<V8>(sa, pl, (wi * MT + i) * 32, ks);
+  for (int c = 0; c < PER; ++c) load(c, ST - 1, k_begin + (ST - 1) * BK);
+  int cur = 0;
+  for (long long k0 = k_begin; k0 < k_end; k0 += BK) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) bv[pl][j] = b.template frag<V8>(sb, pl, (wj * NT + j) * 32, ks);
-      }
-      if (PL == 1) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = dt_mfma(bv[0][j], av[0][i], acc[i][j]);
+    for (int ks = 0; ks < KS; ++ks) {
+      // the operands of the k step after this one are read before this one's MFMAs are issued; before the first of the next
+      // stage: that stage has landed, and every wave has read what it needs of this one, which is loaded again from here on
+      int stage; long long at; int c0;
+      if (ks < KS - 1) {
+        read((ks + 1) & 1, smem + cur * STAGE, ks + 1);
+        stage = cur == 0 ? ST - 1 : cur - 1; at = k0 + (ST - 1) * BK; c0 = (ks + 1) * PER;
       } else {
-#pragma unroll
-        for (int t = 0; t < 6; ++t) {
-          constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = dt_mfma(bv[PB[t] % PL][j], av[PA[t] % PL][i], acc[i][j]);
-        }
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((ST - 2) * COUNT) : "memory");
+        stage = cur; at = k0 + ST * BK; c0 = 0;
+        cur = cur == ST - 1 ? 0 : cur + 1;
+        read(0, smem + cur * STAGE, 0);          // (behind the last step: what is read is not used)
       }
+      __builtin_amdgcn_sched_barrier(0);
+      // the loads go out one by one between the MFMAs: a wave's instructions issue in order, and a burst of loads holds up
+      // everything behind it until the memory path has taken them
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        const int t = m / (MT * NT), i = m % (MT * NT) / NT, j = m % NT;
+        constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};       // smallest terms first
+        const int pa = PL == 1 ? 0 : PA[t], pb = PL == 1 ? 0 : PB[t];
+        acc[i][j] = dt_mfma(bv[ks & 1][pb % PL][j], av[ks & 1][pa % PL][i], acc[i][j]);
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          if (m == (c + 1) * MF / (PER + 1)) {
+            __builtin_amdgcn_sched_barrier(0);
+            load(c0 + c, stage, at);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -229,8 +258,9 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
   // from the accumulators' layout a store would touch 32 lines.
   constexpr int CW = NT * 32, OCT = CW / 8, RPP = 64 / OCT;      // columns, their blocks of 8, rows a pass
   constexpr int SM = MT < 2 ? MT : 2;                            // 32-row blocks a strip holds
-  static_assert(WAVES * SM * 32 * CW * 4 <= 2 * STAGE && MT % SM == 0, "the strips fit the stages");
-  __syncthreads();                                               // every wave is done with the operand tiles
+  static_assert(WAVES * SM * 32 * CW * 4 <= ST * STAGE && MT % SM == 0, "the strips fit the stages");
+  // every wave is done with the operand tiles, and no load is on its way into them
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
   DT_LDS char* strip = smem + wave * SM * 32 * CW * 4;
   const int l31 = lane & 31, lh = lane >> 5;
   const unsigned long long base = drop_base(g.epi.drop);
@@ -329,26 +359,27 @@ int dense_pack_launch(int dtype, const void* src, long long ld, long long rows, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int WM, int WN>
+template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int ST, int WM, int WN>
 static int dt_go(const DtGemm& gin, hipStream_t st) {
   DtGemm g = gin;
   g.tiles_i = (unsigned)((g.I + BM - 1) / BM); g.tiles_j = (unsigned)((g.J + BN - 1) / BN);
-  constexpr int lds = 2 * PL * (BM + BN) * BK * 2;
-  const void* fn = reinterpret_cast<const void*>(dense_tile_kernel<T, M, PL, AKC, BKC, BM, BN, BK, WM, WN>);
+  constexpr int lds = ST * PL * (BM + BN) * BK * 2;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  const void* fn = reinterpret_cast<const void*>(dense_tile_kernel<T, M, PL, AKC, BKC, BM, BN, BK, ST, WM, WN>);
   // (a function's attribute belongs to the current device: set before each launch, a host-side call of well under a microsecond)
   if (lds > 64 * 1024 && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     veex_set_error("dense: cannot raise the dynamic LDS limit"); return VEEX_ELAUNCH;
   }
-  hipLaunchKernelGGL((dense_tile_kernel<T, M, PL, AKC, BKC, BM, BN, BK, WM, WN>), dim3(g.tiles_i * g.tiles_j * g.splits), dim3(64 * WM * WN), lds, st, g);
+  hipLaunchKernelGGL((dense_tile_kernel<T, M, PL, AKC, BKC, BM, BN, BK, ST, WM, WN>), dim3(g.tiles_i * g.tiles_j * g.splits), dim3(64 * WM * WN), lds, st, g);
   VEEX_CHECK_LAUNCH();
   return 0;
 }
 
 template <typename T, typename M, bool AKC, bool BKC>
 static int dt_pick(int tile, const DtGemm& g, hipStream_t st) {
-  if constexpr (sizeof(T) == 4) return dt_go<T, M, 3, AKC, BKC, 128, 128, 32, 2, 4>(g, st);
-  else if (tile == 256) return dt_go<T, M, 1, AKC, BKC, 256, 256, 64, 2, 4>(g, st);
-  else return dt_go<T, M, 1, AKC, BKC, 128, 128, 64, 2, 2>(g, st);
+  if constexpr (sizeof(T) == 4) return dt_go<T, M, 3, AKC, BKC, 128, 128, 32, DT_X3_ST, DT_X3_W>(g, st);
+  else if (tile == 256) return dt_go<T, M, 1, AKC, BKC, 256, 256, DT_L_BK, DT_L_ST, 2, 4>(g, st);
+  else return dt_go<T, M, 1, AKC, BKC, 128, 128, DT_S_BK, DT_S_ST, DT_S_W>(g, st);
 }
 
 template <typename T, typename M>
