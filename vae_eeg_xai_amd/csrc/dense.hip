@@ -92,10 +92,12 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
     *reinterpret_cast<float4*>(strip + l31 * 36 + 8 * q + 4 * lh) = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
   __syncthreads();
   const unsigned long long base = drop_base(g.epi.drop);
+  const int j = j0 + wj * 32 + 8 * (lane & 3);
+  float bias[8];
+  if (!SPLIT) dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
 #pragma unroll 1
   for (int r = lane >> 2; r < 32; r += 16) {
     const long long i = i0 + wi * 32 + r;
-    const int j = j0 + wj * 32 + 8 * (lane & 3);
     if (i >= g.I || j >= g.J) continue;
     const float4 lo = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3)), hi = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3) + 4);
     float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
     } else {
       unsigned w[4] = {0u, 0u, 0u, 0u};
       if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
-      dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e, w);
+      dense_epilogue<T>(g.epi, v, bias, i * g.J + j, g.J - j, g.vec_e, w);
     }
   }
 }
@@ -167,7 +169,9 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
     if (sl == 0 && b0 + ob < nb) {
       unsigned w[4] = {0u, 0u, 0u, 0u};
       if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
-      dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e, w);
+      float bias[8];
+      dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
+      dense_epilogue<T>(g.epi, v, bias, i * g.J + j, g.J - j, g.vec_e, w);
     }
   }
 }
@@ -245,68 +249,51 @@ struct DenseDz {
   DropArgs drop;
 };
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
-  constexpr int V = 16 / sizeof(T);
   __shared__ float s[8][256];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int j = blockIdx.x * 256 + 8 * tx, n = min(8, p.n - j);
   const long long first = (long long)blockIdx.y * p.rows_per_chunk, last = min(p.rows, first + p.rows_per_chunk);
   const unsigned long long base = drop_base(p.drop);
+  const T* const dy = static_cast<const T*>(p.dy) + j;
+  const T* const pre = static_cast<const T*>(p.pre) + j;
   float sum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[e] = 0.f;
   if (n > 0) {
-    for (long long i = first + ty; i < last; i += 8) {
-      const long long at = i * p.n + j;
-      const T* dy = static_cast<const T*>(p.dy) + at;
-      const T* pre = static_cast<const T*>(p.pre) + at;
-      float d[8], z[8];
-      if (p.vec) {
+    constexpr int RB = 2;                 // rows in flight a thread
+    for (long long i0 = first + ty; i0 < last; i0 += 8 * RB) {
+      Raw8<T> d[RB], z[RB];
 #pragma unroll
-        for (int q = 0; q < 8 / V; ++q) {
-          const Piece<T, V> a = piece_load<T, V>(dy + q * V);
-#pragma unroll
-          for (int e = 0; e < V; ++e) d[q * V + e] = (float)a.v[e];
-          if (p.act != VEEX_ACT_NONE) {
-            const Piece<T, V> b = piece_load<T, V>(pre + q * V);
-#pragma unroll
-            for (int e = 0; e < V; ++e) z[q * V + e] = (float)b.v[e];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d[e] = e < n ? (float)dy[e] : 0.f;
-          z[e] = e < n && p.act != VEEX_ACT_NONE ? (float)pre[e] : 0.f;
-        }
+      for (int q = 0; q < RB; ++q) {
+        const long long at = min(i0 + 8 * q, last - 1) * p.n;
+        load_raw<T>(d[q], dy + at, n, VEC);
+        if (p.act != VEEX_ACT_NONE) load_raw<T>(z[q], pre + at, n, VEC);
       }
-      if (p.drop.cut != 0u) {
-        unsigned w[4];
-        drop_words(p.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = drop_u16(w, e) >= p.drop.cut ? d[e] * p.drop.scale : 0.f;
-      }
-      if (p.act != VEEX_ACT_NONE) dense_act_grad<T, 8>(d, z, p.act);        // (finite at the zeros behind the last column)
+      for (int q = 0; q < RB; ++q) {
+        const long long i = i0 + 8 * q;
+        if (i >= last) continue;
+        float g[8], x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += d[e];
-      if (p.dz != nullptr && p.plane_bytes != 0) {
-        dt_store_planes(static_cast<char*>(p.dz) + (i * p.ld + j) * 2, p.plane_bytes, d);
-      } else if (p.dz != nullptr) {
-        T* dz = static_cast<T*>(p.dz) + i * p.ld + j;
-        if (p.vec) {
+        for (int e = 0; e < 8; ++e) { g[e] = VEC || e < n ? (float)d[q].v[e] : 0.f; x[e] = (float)z[q].v[e]; }
+        if (p.drop.cut != 0u) {
+          unsigned w[4];
+          drop_words(p.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
 #pragma unroll
-          for (int q = 0; q < 8 / V; ++q) {
-            Piece<T, V> a;
-#pragma unroll
-            for (int e = 0; e < V; ++e) a.v[e] = (T)d[q * V + e];
-            piece_store<T, V>(dz + q * V, a);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (j + e < p.ld) dz[e] = (T)d[e];
+          for (int e = 0; e < 8; ++e) g[e] = drop_u16(w, e) >= p.drop.cut ? g[e] * p.drop.scale : 0.f;
         }
+        if (p.act != VEEX_ACT_NONE) {
+          dense_act_grad<T, 8>(g, x, p.act);
+          if (!VEC)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = e < n ? g[e] : 0.f;       // (behind the last column z repeats another element)
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += g[e];
+        if (p.dz != nullptr && p.plane_bytes != 0) dt_store_planes(static_cast<char*>(p.dz) + (i * p.ld + j) * 2, p.plane_bytes, g);
+        else if (p.dz != nullptr) store8<T>(static_cast<T*>(p.dz) + i * p.ld + j, g, (int)(p.ld - j), VEC);
       }
     }
   }
@@ -393,7 +380,7 @@ static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
   g.slab = static_cast<float*>(ws);
   g.vec_a = operand_vec(g.a, kind == kKindDw ? g.I : g.K, sizeof(T));
   g.vec_b = operand_vec(g.b, kind == kKindDx ? g.K : g.J, sizeof(T));
-  g.vec_e = dense_epi_vec(g.epi, g.J, 8, sizeof(T));
+  g.vec_e = dense_epi_vec(g.epi, g.J);
   const long long tiles = (g.I + 63) / 64 * ((g.J + 63) / 64);
   if (tiles > 0x7FFFFFFFll) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
   const dim3 grid((unsigned)tiles, (unsigned)g.splits);
@@ -439,7 +426,7 @@ static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
   const bool vec = few_vec<T>(g);
   few_split(g, vec, sizeof(T), g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
-  g.vec_e = dense_epi_vec(g.epi, g.J, 8, sizeof(T));
+  g.vec_e = dense_epi_vec(g.epi, g.J);
   const dim3 grid((unsigned)(vec ? (g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64), (unsigned)g.splits);
 #define DF_GO(R)                                                                                              \
   if (vec) hipLaunchKernelGGL((dense_few_rows_kernel<T, R, true>), grid, dim3(256), 0, st, g);                 \
@@ -486,27 +473,35 @@ static bool lies_well(const VeexDense* d, const void* p, long long ld, long long
   return d->dtype != VEEX_T_F32 && trunk_aligned16(p) && ld % 8 == 0 && cols % 8 == 0;
 }
 
-struct TilePlan { int tile; unsigned splits; long long per; };
+struct TilePlan { int tile, bm, bn; unsigned splits; long long per; };
 
 // The tile and the split of the reduction: the fewest rounds of the chip's tile slots, weighed by a tile's time
 static TilePlan tile_plan(const VeexDense* d, long long I, long long J, long long K) {
   TilePlan best = {};
   double cost = 1e300;
   const bool f32 = d->dtype == VEEX_T_F32;
-  const int bk = f32 ? 32 : 64;
-  for (int tile : {256, 128}) {
-    if (f32 && tile == 256) continue;
-    const long long tiles = (I + tile - 1) / tile * ((J + tile - 1) / tile), slots = tile == 256 || f32 ? 256 : 512;
+  const int bk = 32;
+  struct Shape { int code, bm, bn, slots; double step; };
+  static const Shape shapes16[] = {{0, 256, 256, 256, 0.93}, {1, 256, 128, 256, 0.53}, {2, 128, 128, 256, 0.33}};
+  static const Shape shapes32[] = {{1, 256, 128, 256, 2.4}, {2, 128, 128, 256, 1.3}};
+  for (int q = 0; q < (f32 ? 2 : 3); ++q) {
+    const Shape& sh = f32 ? shapes32[q] : shapes16[q];
+#ifdef DT_FORCE
+    if (sh.code != DT_FORCE) continue;
+#endif
+    const long long tiles = (I + sh.bm - 1) / sh.bm * ((J + sh.bn - 1) / sh.bn);
     for (long long s = 1; s <= 64; s *= 2) {
       const long long per = ((K + s - 1) / s + bk - 1) / bk * bk, splits = (K + per - 1) / per;
       if (s > 1 && per < 4 * bk) break;
-      const double rounds = (double)((tiles * splits + slots - 1) / slots);
-      const double step = tile == 256 ? 4.0 : 2.2;                  // 2^14 multiplications at a full chip's rate; two 128s share a CU
-      const double join = splits > 1 ? (double)splits * I * J / (1 << 20) * 16.0 + 300.0 : 0.0;   // slabs out and in, one more launch
-      const double c = rounds * (step * ((double)per / 64.0 + 4.0)) * 8.0 + join;
-      if (c < cost) { cost = c; best = {tile, (unsigned)splits, per}; }
+      const double rounds = (double)((tiles * splits + sh.slots - 1) / sh.slots);
+      const double join = splits > 1 ? (double)splits * I * J * 8.0 / 4.0e6 + 4.0 : 0.0;   // slabs out and in, one more launch
+      const double c = rounds * sh.step * ((double)per / 32.0 + 3.0) + join;
+      if (c < cost) { cost = c; best = {sh.code, sh.bm, sh.bn, (unsigned)splits, per}; }
     }
   }
+#ifdef DT_SAY
+  printf("I %lld J %lld K %lld: tile %d splits %u\n", I, J, K, best.tile, best.splits);
+#endif
   return best;
 }
 
@@ -548,8 +543,8 @@ static int tiles_any(int kind, const VeexDense* d, const DenseGemm& g, const DtT
   q.a = a; q.b = b; q.I = g.I; q.J = g.J; q.K = g.K; q.k_per_split = t.per; q.splits = t.splits;
   q.epi = g.epi;
   q.slab = t.splits > 1 ? static_cast<float*>(ws) : nullptr;
-  q.vec_e = dense_epi_vec(g.epi, g.J, 8, trunk_elem_bytes(d->dtype));
-  if ((double)((g.I + t.tile - 1) / t.tile) * ((g.J + t.tile - 1) / t.tile) * t.splits > 2147483647.0) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
+  q.vec_e = dense_epi_vec(g.epi, g.J);
+  if ((double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits > 2147483647.0) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
   if (int rc = dense_tile_launch(d->dtype, kind != kKindDw, kind == kKindDx, t.tile, q, st)) return rc;
   if (t.splits > 1) {
     DenseGemm j = g;
@@ -667,9 +662,13 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
     p.vec = d->n % 8 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
     if (p.dz != nullptr || d->db != nullptr) {
       const dim3 grid((d->n + 255) / 256, l.chunks);
-      if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_dz_kernel<float>), grid, dim3(256), 0, st, p);
-      else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_dz_kernel<bf16_t>), grid, dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((dense_dz_kernel<f16_t>), grid, dim3(256), 0, st, p);
+#define DZ_GO(T)                                                                                              \
+  if (p.vec) hipLaunchKernelGGL((dense_dz_kernel<T, true>), grid, dim3(256), 0, st, p);                        \
+  else hipLaunchKernelGGL((dense_dz_kernel<T, false>), grid, dim3(256), 0, st, p);
+      if (d->dtype == VEEX_T_F32) { DZ_GO(float) }
+      else if (d->dtype == VEEX_T_BF16) { DZ_GO(bf16_t) }
+      else { DZ_GO(f16_t) }
+#undef DZ_GO
       VEEX_CHECK_LAUNCH();
     }
     if (p.part != nullptr) {

@@ -96,81 +96,80 @@ __device__ __forceinline__ void dense_act_grad(float (&d)[W], const float (&s)[W
   }
 }
 
-// Columns j .. j + W - 1 (W = 8, j a multiple of 8) of row i; words: the row's dropout words of that block.
-template <typename T, int W>
-__device__ __forceinline__ void dense_epilogue(const DenseEpi& ep, float (&v)[W], long long i, int j, int J, bool vec,
-                                               const unsigned* words) {
-  const T* bias = static_cast<const T*>(ep.bias);
-  const T* res = static_cast<const T*>(ep.res);
-  T* y = static_cast<T*>(ep.y);
-  T* pre = static_cast<T*>(ep.pre);
-  const long long at = i * J + j;
-  constexpr int V = W * (int)sizeof(T) <= 16 ? W : 16 / (int)sizeof(T);
-  const int n = min(W, J - j);
-  if (n <= 0) return;
-  float r[W];
-#pragma unroll
-  for (int e = 0; e < W; ++e) r[e] = 0.f;
+// Eight elements at p (n of them inside the row), as they lie; vec: as 16-byte pieces.  Kept apart from their conversion, so that
+// several loads are on their way before the first is waited for.
+template <typename T> struct Raw8 { T v[8]; };
+template <typename T>
+__device__ __forceinline__ void load_raw(Raw8<T>& r, const T* p, int n, bool vec) {
+  constexpr int V = 16 / (int)sizeof(T);
   if (vec) {
-    if (bias != nullptr)
 #pragma unroll
-      for (int q = 0; q < W / V; ++q) {
-        const Piece<T, V> b = piece_load<T, V>(bias + j + q * V);
+    for (int q = 0; q < 8 / V; ++q) {
+      const Piece<T, V> b = piece_load<T, V>(p + q * V);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[q * V + e] += (float)b.v[e];
-      }
-    if (res != nullptr)
-#pragma unroll
-      for (int q = 0; q < W / V; ++q) {
-        const Piece<T, V> b = piece_load<T, V>(res + at + q * V);
-#pragma unroll
-        for (int e = 0; e < V; ++e) r[q * V + e] = (float)b.v[e];
-      }
+      for (int e = 0; e < V; ++e) r.v[q * V + e] = b.v[e];
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < W; ++e)
-      if (e < n) {
-        if (bias != nullptr) v[e] += (float)bias[j + e];
-        if (res != nullptr) r[e] = (float)res[at + e];
-      }
+    for (int e = 0; e < 8; ++e) r.v[e] = p[e < n ? e : 0];
   }
-  float o[W];
+}
+template <typename T>
+__device__ __forceinline__ void load8(float (&r)[8], const T* p, int n, bool vec) {
+  Raw8<T> x;
+  load_raw<T>(x, p, n, vec);
 #pragma unroll
-  for (int e = 0; e < W; ++e) o[e] = v[e];
-  dense_act<T, W>(o, ep.act);
+  for (int e = 0; e < 8; ++e) r[e] = (float)x.v[e];
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&s)[8], int n, bool vec) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (vec) {
 #pragma unroll
-  for (int e = 0; e < W; ++e) {
-    if (ep.drop.cut != 0u) {
-      const unsigned u = (e & 1) ? words[e >> 1] >> 16 : words[e >> 1] & 0xFFFFu;
-      o[e] = u >= ep.drop.cut ? o[e] * ep.drop.scale : 0.f;
+    for (int q = 0; q < 8 / V; ++q) {
+      Piece<T, V> b;
+#pragma unroll
+      for (int e = 0; e < V; ++e) b.v[e] = (T)s[q * V + e];
+      piece_store<T, V>(p + q * V, b);
     }
-    o[e] += r[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (T)s[e];
   }
-  auto put = [&](T* dst, const float (&s)[W]) {
-    if (vec) {
-#pragma unroll
-      for (int q = 0; q < W / V; ++q) {
-        Piece<T, V> p;
-#pragma unroll
-        for (int e = 0; e < V; ++e) p.v[e] = (T)s[q * V + e];
-        piece_store<T, V>(dst + at + q * V, p);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; ++e)
-        if (e < n) dst[at + e] = (T)s[e];
-    }
-  };
-  if (pre != nullptr) put(pre, v);
-  put(y, o);
 }
 
-// every tensor of the epilogue can be moved in pieces of W elements
-inline bool dense_epi_vec(const DenseEpi& ep, int J, int W, int elem) {
-  if (J % W != 0) return false;
-  const uintptr_t mask = (uintptr_t)(W * elem < 16 ? W * elem : 16) - 1;
+// Columns j .. j + 7 (j a multiple of 8, n of them inside the row) of row i, `at` = i * J + j: v = acc, b = the bias there (zeros
+// without one), words = the row's dropout words of that block.  A thread that walks down rows loads b once.
+template <typename T>
+__device__ __forceinline__ void dense_bias(const DenseEpi& ep, float (&b)[8], int j, int J, bool vec) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) b[e] = 0.f;
+  if (ep.bias != nullptr && j < J) load8<T>(b, static_cast<const T*>(ep.bias) + j, J - j, vec);
+}
+template <typename T>
+__device__ __forceinline__ void dense_epilogue(const DenseEpi& ep, float (&v)[8], const float (&b)[8], long long at, int n, bool vec,
+                                               const unsigned* words) {
+  float r[8];
+  if (ep.res != nullptr) load8<T>(r, static_cast<const T*>(ep.res) + at, n, vec);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += b[e];
+  if (ep.pre != nullptr) store8<T>(static_cast<T*>(ep.pre) + at, v, n, vec);
+  dense_act<T, 8>(v, ep.act);
+  if (ep.drop.cut != 0u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = drop_u16(words, e) >= ep.drop.cut ? v[e] * ep.drop.scale : 0.f;
+  if (ep.res != nullptr)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
+  store8<T>(static_cast<T*>(ep.y) + at, v, n, vec);
+}
+
+// every tensor of the epilogue can be moved in 16-byte pieces of blocks of 8 columns
+inline bool dense_epi_vec(const DenseEpi& ep, int J) {
+  if (J % 8 != 0) return false;
   for (const void* q : {ep.bias, ep.res, (const void*)ep.y, (const void*)ep.pre})
-    if (reinterpret_cast<uintptr_t>(q) & mask) return false;
+    if (!trunk_aligned16(q)) return false;
   return true;
 }
 

@@ -24,15 +24,6 @@ typedef unsigned dt_u4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 #define DT_LDS __attribute__((address_space(3)))
-#ifndef DT_L_BK
-#define DT_L_BK 32
-#define DT_L_ST 4
-#define DT_S_BK 32
-#define DT_S_ST 4
-#define DT_S_W 2, 2
-#define DT_X3_ST 3
-#define DT_X3_W 2, 4
-#endif
 #define DT_OOB 0xFFFFFFF0u      // past every buffer's end
 
 __device__ __forceinline__ f32x16 dt_mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -191,7 +182,7 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
   // ST stages in a ring: while step t is computed, the loads of the ST - 1 steps behind it are on their way (past the end they
   // fetch nothing, so that the count of loads in flight stays the same)
   constexpr int COUNT = OpA::COUNT + OpB::COUNT, KS = BK / 16, PER = (COUNT + KS - 1) / KS, MF = MT * NT * (PL == 1 ? 1 : 6);
-  static_assert(ST >= 3 && KS % 2 == 0, "");
+  static_assert(ST >= 2 && KS % 2 == 0, "");
   auto load = [&](int c, int stage, long long k0) {
     if (c < OpA::COUNT) a.load(c, smem + stage * STAGE, k0, k_end);
     else if (c < COUNT) b.load(c - OpA::COUNT, smem + stage * STAGE + PL * OpA::BYTES, k0, k_end);
@@ -257,13 +248,16 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
   // row), so that a lane holds 8 consecutive columns of a row and eight lanes (four for 32 columns) write a whole line.  Straight
   // from the accumulators' layout a store would touch 32 lines.
   constexpr int CW = NT * 32, OCT = CW / 8, RPP = 64 / OCT;      // columns, their blocks of 8, rows a pass
-  constexpr int SM = MT < 2 ? MT : 2;                            // 32-row blocks a strip holds
+  constexpr int SM = MT < 2 || WAVES * 64 * CW * 4 > ST * STAGE ? 1 : 2;                            // 32-row blocks a strip holds
   static_assert(WAVES * SM * 32 * CW * 4 <= ST * STAGE && MT % SM == 0, "the strips fit the stages");
   // every wave is done with the operand tiles, and no load is on its way into them
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
   DT_LDS char* strip = smem + wave * SM * 32 * CW * 4;
   const int l31 = lane & 31, lh = lane >> 5;
   const unsigned long long base = drop_base(g.epi.drop);
+  const int o = lane % OCT, j = j0 + wj * CW + 8 * o;
+  float bias[8];
+  if (g.slab == nullptr) dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
 #pragma unroll
   for (int m0 = 0; m0 < MT; m0 += SM) {
 #pragma unroll
@@ -275,29 +269,27 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
           *reinterpret_cast<DT_LDS dt_f4*>(strip + ((mi - m0) * 32 + l31) * CW * 4 + (((nj * 8 + 2 * q + lh) ^ (l31 & 7)) * 16)) =
               dt_f4{acc[mi][nj][4 * q], acc[mi][nj][4 * q + 1], acc[mi][nj][4 * q + 2], acc[mi][nj][4 * q + 3]};
     dt_wave_sync();
-#pragma unroll 1
-    for (int r0 = 0; r0 < 32 * SM; r0 += RPP) {
-      const int r = r0 + lane / OCT, o = lane % OCT;
+    long long i = i0 + (wi * MT + m0) * 32 + lane / OCT, at = i * g.J + j;
+#pragma unroll 2
+    for (int r = lane / OCT; r < 32 * SM; r += RPP, i += RPP, at += (long long)RPP * g.J) {
       const dt_f4 lo = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o) ^ (r & 7)) * 16));
       const dt_f4 hi = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o + 1) ^ (r & 7)) * 16));
-      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      const long long i = i0 + (wi * MT + m0) * 32 + r;
-      const int j = j0 + wj * CW + 8 * o;
       if (i >= g.I || j >= g.J) continue;
       if (g.slab != nullptr) {
-        float* s = g.slab + (z * g.I + i) * g.J + j;
+        float* s = g.slab + z * g.I * g.J + at;
         if (g.J % 4 == 0) {
           *reinterpret_cast<dt_f4*>(s) = lo;
           if (j + 4 < g.J) *reinterpret_cast<dt_f4*>(s + 4) = hi;
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (j + e < g.J) s[e] = v[e];
+            if (j + e < g.J) s[e] = e < 4 ? lo[e & 3] : hi[e & 3];
         }
       } else {
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         unsigned w[4] = {0u, 0u, 0u, 0u};
         if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
-        dense_epilogue<T, 8>(g.epi, v, i, j, g.J, g.vec_e, w);
+        dense_epilogue<T>(g.epi, v, bias, at, g.J - j, g.vec_e, w);
       }
     }
     dt_wave_sync();
@@ -377,9 +369,14 @@ static int dt_go(const DtGemm& gin, hipStream_t st) {
 
 template <typename T, typename M, bool AKC, bool BKC>
 static int dt_pick(int tile, const DtGemm& g, hipStream_t st) {
-  if constexpr (sizeof(T) == 4) return dt_go<T, M, 3, AKC, BKC, 128, 128, 32, DT_X3_ST, DT_X3_W>(g, st);
-  else if (tile == 256) return dt_go<T, M, 1, AKC, BKC, 256, 256, DT_L_BK, DT_L_ST, 2, 4>(g, st);
-  else return dt_go<T, M, 1, AKC, BKC, 128, 128, DT_S_BK, DT_S_ST, DT_S_W>(g, st);
+  if constexpr (sizeof(T) == 4) {
+    if (tile == 1) return dt_go<T, M, 3, AKC, BKC, 256, 128, 32, 2, 4, 2>(g, st);
+    return dt_go<T, M, 3, AKC, BKC, 128, 128, 32, 3, 2, 4>(g, st);
+  } else {
+    if (tile == 0) return dt_go<T, M, 1, AKC, BKC, 256, 256, 32, 4, 2, 4>(g, st);
+    if (tile == 1) return dt_go<T, M, 1, AKC, BKC, 256, 128, 64, 3, 4, 2>(g, st);
+    return dt_go<T, M, 1, AKC, BKC, 128, 128, 64, 4, 2, 4>(g, st);
+  }
 }
 
 template <typename T, typename M>
