@@ -128,30 +128,39 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNo
     rstd = 1.f / sqrtf(row_sum(q, 0.f).x * inv + p.eps);
   };
 
-  // every row group of a block takes the same number of turns (the sums hold barriers); a turn past the end repeats the last row
-  for (long long r0 = (long long)blockIdx.x * RG; r0 < p.rows; r0 += (long long)gridDim.x * RG) {
+  // Every row group of a block takes the same number of turns (the sums hold barriers); a turn past the end repeats the last row.
+  // The next turn's rows are on their way while this one's are worked on: a turn is a chain of load, two to four sums across the
+  // waves and store, and the chip has too few rows in flight to hide it otherwise.
+  struct In { RowRaw<T, V, C> x, h, g; };
+  auto fetch = [&](In& r, long long row) {
+    row = min(row, p.rows - 1);
+    row_load<T, V, C, LANES>(r.x, p.x, row * p.cols, lane, p.cols);
+    if (p.h != nullptr) row_load<T, V, C, LANES>(r.h, p.h, row * p.cols, lane, p.cols);
+    if (p.gate != nullptr) row_load<T, V, C, LANES>(r.g, p.gate, row / p.rows_per_group * p.cols, lane, p.cols);
+    else row_fill<T, V, C, LANES>(r.g, 1.f);
+  };
+  const long long step = (long long)gridDim.x * RG;
+  In in_now, in_next;
+  fetch(in_now, (long long)blockIdx.x * RG + rg);
+  for (long long r0 = (long long)blockIdx.x * RG; r0 < p.rows; r0 += step) {
     const bool live = r0 + rg < p.rows;
     const long long row = live ? r0 + rg : p.rows - 1, at = row * p.cols;
-    RowRaw<T, V, C> xr, hr, gr;
-    row_load<T, V, C, LANES>(xr, p.x, at, lane, p.cols);
+    if (r0 + step < p.rows) fetch(in_next, r0 + step + rg);
     float v[EPL], mean1 = 0.f, rstd1 = 0.f, mean2, rstd2;
     if (p.h != nullptr) {
-      row_load<T, V, C, LANES>(hr, p.h, at, lane, p.cols);
-      if (p.gate != nullptr) row_load<T, V, C, LANES>(gr, p.gate, row / p.rows_per_group * p.cols, lane, p.cols);
-      else row_fill<T, V, C, LANES>(gr, 1.f);
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) v[e] = (float)hr.p[e / V].v[e % V];
+      for (int e = 0; e < EPL; ++e) v[e] = (float)in_now.h.p[e / V].v[e % V];
       moments(v, mean1, rstd1);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         const int c = e / V, k = e % V;
         const float n = fmaf((v[e] - mean1) * rstd1, (float)ow.p[c].v[k], (float)ob.p[c].v[k]);
-        v[e] = in[c] ? fmaf((float)scale.p[c].v[k] * (float)gr.p[c].v[k], n, (float)xr.p[c].v[k]) : 0.f;
+        v[e] = in[c] ? fmaf((float)scale.p[c].v[k] * (float)in_now.g.p[c].v[k], n, (float)in_now.x.p[c].v[k]) : 0.f;
       }
       if (live) row_store<T, V, C, LANES>(p.x_out, at, v, lane, p.cols);
     } else {
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) v[e] = (float)xr.p[e / V].v[e % V];
+      for (int e = 0; e < EPL; ++e) v[e] = (float)in_now.x.p[e / V].v[e % V];
     }
     moments(v, mean2, rstd2);
 #pragma unroll
@@ -160,6 +169,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNo
       row_store<T, V, C, LANES>(p.u, at, v, lane, p.cols);
       if (p.stats != nullptr && lane == 0) *reinterpret_cast<float4*>(p.stats + row * 4) = make_float4(mean1, rstd1, mean2, rstd2);
     }
+    in_now = in_next;
   }
 }
 
@@ -199,19 +209,28 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
   // hands out chunks of several "groups" and the gate is read with its row)
   const long long c_first = full_gate ? blockIdx.x * p.rows_per_chunk : first;
   const long long c_last = full_gate ? min(c_first + p.rows_per_chunk, p.rows) : last;
+  struct In { RowRaw<T, V, C> x, h, dout, du, g; float4 st; };
+  auto fetch = [&](In& r, long long row) {
+    row = min(row, c_last - 1);
+    const long long at = row * p.cols;
+    row_load<T, V, C, LANES>(r.x, p.x, at, lane, p.cols);
+    if (post) row_load<T, V, C, LANES>(r.h, p.h, at, lane, p.cols);
+    if (p.dx_out != nullptr) row_load<T, V, C, LANES>(r.dout, p.dx_out, at, lane, p.cols);
+    else row_fill<T, V, C, LANES>(r.dout, 0.f);
+    if (p.du != nullptr) row_load<T, V, C, LANES>(r.du, p.du, at, lane, p.cols);
+    else row_fill<T, V, C, LANES>(r.du, 0.f);
+    if (full_gate) row_load<T, V, C, LANES>(r.g, p.gate, at, lane, p.cols);
+    else r.g = gr;
+    r.st = *reinterpret_cast<const float4*>(p.stats + row * 4);
+  };
+  In in_now, in_next;
+  if (c_first < c_last) fetch(in_now, c_first + rg);
   for (long long r0 = c_first; r0 < c_last; r0 += RG) {
     const bool live = r0 + rg < c_last;
     const long long row = live ? r0 + rg : c_last - 1, at = row * p.cols;
-    RowRaw<T, V, C> xr, hr, dor, dur;
-    row_load<T, V, C, LANES>(xr, p.x, at, lane, p.cols);
-    if (post) row_load<T, V, C, LANES>(hr, p.h, at, lane, p.cols);
-    if (p.dx_out != nullptr) row_load<T, V, C, LANES>(dor, p.dx_out, at, lane, p.cols);
-    else row_fill<T, V, C, LANES>(dor, 0.f);
-    if (p.du != nullptr) row_load<T, V, C, LANES>(dur, p.du, at, lane, p.cols);
-    else row_fill<T, V, C, LANES>(dur, 0.f);
-    if (full_gate) row_load<T, V, C, LANES>(gr, p.gate, at, lane, p.cols);
-    const float4 st = *reinterpret_cast<const float4*>(p.stats + row * 4);
-
+    if (r0 + RG < c_last) fetch(in_next, r0 + RG + rg);          // (as in the forward kernel)
+    const RowRaw<T, V, C>&xr = in_now.x, &hr = in_now.h, &dor = in_now.dout, &dur = in_now.du, &gr = in_now.g;
+    const float4 st = in_now.st;
     float xh[EPL], n[EPL], rh[EPL], d[EPL];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -262,6 +281,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
       for (int e = 0; e < EPL; ++e) d[e] = st.y * (d[e] - fmaf(xh[e], m.y, m.x));
       if (live && p.dh != nullptr) row_store<T, V, C, LANES>(p.dh, at, d, lane, p.cols);
     }
+    in_now = in_next;
   }
 
   float* part = p.part + (long long)blockIdx.x * 5 * p.cols;
@@ -293,44 +313,45 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
   if (p.dpre_b != nullptr) flush(a_pb, 4);
 }
 
-// Column sums of the partial rows: 64 columns and 16 row lanes a block; blockIdx.y = which sum.
+// Column sums of the partial rows, 64 columns and 16 row lanes a block.  blockIdx.y 0: dscale (each chunk's sum times its group's
+// gate), 1 to 4: the vectors, 5 on: the gate rows of a grouped gate.
 template <typename T>
 __global__ __launch_bounds__(1024) void rnorm_sums_kernel(RNormParams p, long long chunks) {
   __shared__ float s[16][64];
-  const int k = blockIdx.y, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int col = blockIdx.x * 64 + tx;
-  const bool ok = col < p.cols;
-  auto column = [&](long long from, long long to) -> float {       // valid in row lane 0
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int col = blockIdx.x * 64 + tx, lc = min(col, p.cols - 1);
+  const bool grouped = p.gate != nullptr && p.rows_per_group > 1;
+  const T* gate = static_cast<const T*>(p.gate);
+  auto column = [&](int k, long long from, long long to, bool weigh) -> float {       // valid in row lane 0
     float a = 0.f;
-    if (ok)
-      for (long long c = from + ty; c < to; c += 16) a += p.part[(c * 5 + k) * p.cols + col];
+    const float* part = p.part + (long long)k * p.cols + lc;
+#pragma unroll 8
+    for (long long c = from + ty; c < to; c += 16) {
+      const float v = part[c * 5 * p.cols];
+      a = weigh ? fmaf(v, (float)gate[c / p.chunks_per_group * p.cols + lc], a) : a + v;
+    }
     __syncthreads();
     s[ty][tx] = a;
     __syncthreads();
     a = 0.f;
     if (ty == 0)
+#pragma unroll
       for (int i = 0; i < 16; ++i) a += s[i][tx];
     return a;
   };
-  if (k == 0 && p.gate != nullptr && p.rows_per_group > 1) {
-    if (p.dscale == nullptr && p.dgate == nullptr) return;
-    float ds = 0.f;
-    const float sc = p.scale != nullptr && ok ? (float)static_cast<const T*>(p.scale)[col] : 1.f;
-    for (long long g = 0; g < p.groups; ++g) {
-      const float a = column(g * p.chunks_per_group, (g + 1) * p.chunks_per_group);
-      if (ty == 0 && ok) {
-        if (p.dgate != nullptr) static_cast<T*>(p.dgate)[g * p.cols + col] = (T)(a * sc);
-        ds = fmaf(a, (float)static_cast<const T*>(p.gate)[g * p.cols + col], ds);
-      }
+  if (blockIdx.y >= 5) {
+    const float sc = p.scale != nullptr ? (float)static_cast<const T*>(p.scale)[lc] : 1.f;
+    for (long long g = blockIdx.y - 5; g < p.groups; g += gridDim.y - 5) {
+      const float a = column(0, g * p.chunks_per_group, (g + 1) * p.chunks_per_group, false);
+      if (ty == 0 && col < p.cols) static_cast<T*>(p.dgate)[g * p.cols + col] = (T)(a * sc);
     }
-    if (ty == 0 && ok && p.dscale != nullptr) static_cast<T*>(p.dscale)[col] = (T)ds;
     return;
   }
   void* const outs[5] = {p.dscale, p.dpost_w, p.dpost_b, p.dpre_w, p.dpre_b};
-  T* out = static_cast<T*>(outs[k]);
+  T* out = static_cast<T*>(outs[blockIdx.y]);
   if (out == nullptr) return;
-  const float a = column(0, chunks);
-  if (ty == 0 && ok) out[col] = (T)a;
+  const float a = column(blockIdx.y, 0, chunks, blockIdx.y == 0 && grouped);
+  if (ty == 0 && col < p.cols) out[col] = (T)a;
 }
 
 // waves a row / elements a lane: the fewest lanes that hold the row at 8 elements each, up to 16 waves; wider rows take 16
@@ -370,7 +391,8 @@ static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hi
   else RNORM_BY_WIDTH(rnorm_bwd_kernel, T, false, RNORM_BWD_GRID, 0);
   VEEX_CHECK_LAUNCH();
   if (p.dgate != nullptr || p.dscale != nullptr || p.dpost_w != nullptr || p.dpost_b != nullptr || p.dpre_w != nullptr || p.dpre_b != nullptr) {
-    hipLaunchKernelGGL((rnorm_sums_kernel<T>), dim3((p.cols + 63) / 64, 5), dim3(1024), 0, st, p, chunks);
+    const long long gate_rows = p.dgate != nullptr && p.rows_per_group > 1 ? std::min<long long>(p.groups, 1024) : 0;
+    hipLaunchKernelGGL((rnorm_sums_kernel<T>), dim3((p.cols + 63) / 64, (unsigned)(5 + gate_rows)), dim3(1024), 0, st, p, chunks);
     VEEX_CHECK_LAUNCH();
   }
   return 0;

@@ -61,6 +61,12 @@ void check_drop(const char* what, const Tensor& x, double rate, int64_t first_ro
 // the counter's word as a forward call saw it, for the backward pass: the caller may advance it in between
 Tensor word_now(const Tensor& counter, bool used) { return counter.defined() && used ? counter.detach().add(0) : Tensor(); }
 
+// Below autograd while a backward pass records none itself (its ops' autograd kernels, which only refuse, cost some microseconds)
+struct BelowUnlessRecording {
+  std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+  BelowUnlessRecording() { if (!at::GradMode::is_enabled()) below.emplace(); }
+};
+
 // ------------------------------------------------------------------------------------------------ dropout
 Tensor dropout_fwd(const Tensor& x_in, double rate, int64_t seed, int64_t first_row, const OptTensor& residual_in, const OptTensor& counter) {
   const c10::DeviceGuard guard(x_in.device());
@@ -223,6 +229,7 @@ struct Dense : torch::autograd::Function<Dense> {
     if (need_x || need_w || need_b) {
       static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("veex::dense_bwd", "").typed<decltype(dense_bwd)>();
       const auto saved = ctx->get_saved_variables();
+      const BelowUnlessRecording below;
       auto [dx, dw, db] = op.call(grads[0], saved[0], saved[1], opt(saved[2]), ctx->saved_data["activation"].toInt(), ctx->saved_data["rate"].toDouble(),
                                   ctx->saved_data["seed"].toInt(), ctx->saved_data["first_row"].toInt(), opt(saved[3]), need_x, need_w, need_b);
       if (need_x) out[0] = dx;
@@ -341,6 +348,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const auto s = ctx->get_saved_variables();
     std::array<bool, 8> need;
     for (int i = 0, given = 0; i < 8; ++i) need[i] = s[i].defined() && ctx->needs_input_grad(given++);   // (counts the tensors given)
+    const BelowUnlessRecording below;
     const auto g = op.call(s[0], opt(s[1]), opt(s[2]), opt(s[3]), opt(s[4]), opt(s[5]), opt(s[6]), opt(s[7]), ctx->saved_data["groups"].toInt(),
                            ctx->saved_data["kind"].toInt(), ctx->saved_data["eps"].toDouble(), s[8], opt(dx_out), opt(du), need);
     for (int i = 0; i < 8; ++i)
