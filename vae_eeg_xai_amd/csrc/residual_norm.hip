@@ -31,6 +31,21 @@ struct RNormParams {
   long long groups, rows_per_group, rows_per_chunk, chunks_per_group;
 };
 
+// Sum over a wave's 64 lanes, in every lane: neighbours, pairs, quads and eights through DPP, the four rows of 16 through lane swaps.
+// (A shuffle goes through LDS, some hundred cycles a step; six steps twice or more a row were a third of these kernels' time.)
+__device__ __forceinline__ float rn_wave_sum(float x) {
+#define RN_DPP(CTRL) x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xF, 0xF, true))
+  RN_DPP(0xB1);       // quad_perm [1,0,3,2]
+  RN_DPP(0x4E);       // quad_perm [2,3,0,1]
+  RN_DPP(0x141);      // row_half_mirror
+  RN_DPP(0x140);      // row_mirror
+#undef RN_DPP
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+
 // sum of a (and b) over the 64 * WPR lanes of a row; red: two buffers of 2 * 16 floats, taken in turn, so that one barrier a
 // sum is enough (a wave can write a buffer again only after the barrier of the sum in between)
 template <int WPR>
@@ -38,8 +53,7 @@ struct RowSum {
   float* red; int rg, wave, turn;
   __device__ __forceinline__ RowSum(float* r, int rg_, int wave_) : red(r), rg(rg_), wave(wave_), turn(0) {}
   __device__ __forceinline__ float2 operator()(float a, float b) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+    a = rn_wave_sum(a); b = rn_wave_sum(b);
     if (WPR == 1) return make_float2(a, b);
     float* r = red + turn * 32;
     turn ^= 1;
@@ -65,6 +79,13 @@ __device__ __forceinline__ void row_load(RowRaw<T, V, C>& r, const void* base, l
 #pragma unroll
       for (int e = 0; e < V; ++e) r.p[c].v[e] = (T)0.f;
   }
+}
+template <typename T, int V, int C>
+__device__ __forceinline__ void row_copy(RowRaw<T, V, C>& a, const RowRaw<T, V, C>& b) {
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) a.p[c].v[e] = b.p[c].v[e];
 }
 template <typename T, int V, int C, int LANES>
 __device__ __forceinline__ void row_fill(RowRaw<T, V, C>& r, float v) {
@@ -169,12 +190,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNo
       row_store<T, V, C, LANES>(p.u, at, v, lane, p.cols);
       if (p.stats != nullptr && lane == 0) *reinterpret_cast<float4*>(p.stats + row * 4) = make_float4(mean1, rstd1, mean2, rstd2);
     }
-    in_now = in_next;
+    row_copy(in_now.x, in_next.x); row_copy(in_now.h, in_next.h); row_copy(in_now.g, in_next.g);
   }
 }
 
-// One block a chunk: rows_per_chunk consecutive rows of one gate group.
-template <typename T, int WPR, int EPL, bool VEC>
+// One block a chunk: rows_per_chunk consecutive rows of one gate group.  BIAS: a bias learns too (two more sums a column).
+template <typename T, int WPR, int EPL, bool VEC, bool BIAS>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNormParams p) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V, LANES = 64 * WPR;
   constexpr int RG = WPR > 4 ? 1 : 4 / WPR;
@@ -201,9 +222,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
   if (p.gate != nullptr) row_load<T, V, C, LANES>(gr, p.gate, group * p.cols, lane, p.cols);
   else row_fill<T, V, C, LANES>(gr, 1.f);
 
-  float a_gate[EPL], a_ow[EPL], a_ob[EPL], a_pw[EPL], a_pb[EPL];
+  float a_gate[EPL], a_ow[EPL], a_pw[EPL], a_ob[BIAS ? EPL : 1], a_pb[BIAS ? EPL : 1];
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) a_gate[e] = a_ow[e] = a_ob[e] = a_pw[e] = a_pb[e] = 0.f;
+  for (int e = 0; e < EPL; ++e) {
+    a_gate[e] = a_ow[e] = a_pw[e] = 0.f;
+    if (BIAS) a_ob[e] = a_pb[e] = 0.f;
+  }
 
   // (a gate per element: the chunks of one row each would leave as many partial rows as there are rows, so there the host
   // hands out chunks of several "groups" and the gate is read with its row)
@@ -220,7 +244,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
     if (p.du != nullptr) row_load<T, V, C, LANES>(r.du, p.du, at, lane, p.cols);
     else row_fill<T, V, C, LANES>(r.du, 0.f);
     if (full_gate) row_load<T, V, C, LANES>(r.g, p.gate, at, lane, p.cols);
-    else r.g = gr;
+    else row_copy(r.g, gr);
     r.st = *reinterpret_cast<const float4*>(p.stats + row * 4);
   };
   In in_now, in_next;
@@ -231,21 +255,23 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
     if (r0 + RG < c_last) fetch(in_next, r0 + RG + rg);          // (as in the forward kernel)
     const RowRaw<T, V, C>&xr = in_now.x, &hr = in_now.h, &dor = in_now.dout, &dur = in_now.du, &gr = in_now.g;
     const float4 st = in_now.st;
-    float xh[EPL], n[EPL], rh[EPL], d[EPL];
+    float xh[EPL], rh[EPL], d[EPL];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
       const int c = e / V, k = e % V;
       float out = (float)xr.p[c].v[k];
-      xh[e] = n[e] = 0.f;
+      xh[e] = 0.f;
       if (post) {
         xh[e] = ((float)hr.p[c].v[k] - st.x) * st.y;
-        n[e] = fmaf(xh[e], (float)ow.p[c].v[k], (float)ob.p[c].v[k]);
-        out = fmaf((float)scale.p[c].v[k] * (float)gr.p[c].v[k], n[e], out);
+        out = fmaf((float)scale.p[c].v[k] * (float)gr.p[c].v[k], fmaf(xh[e], (float)ow.p[c].v[k], (float)ob.p[c].v[k]), out);
       }
       rh[e] = in[c] ? (out - st.z) * st.w : 0.f;
       const float du = (float)dur.p[c].v[k];
-      if (live) { a_pw[e] = fmaf(du, rh[e], a_pw[e]); a_pb[e] += du; }
+      if (live) {
+        a_pw[e] = fmaf(du, rh[e], a_pw[e]);
+        if (BIAS) a_pb[e] += du;
+      }
       d[e] = du * (float)pw.p[c].v[k];
       s1 += d[e]; s2 = fmaf(d[e], rh[e], s2);
     }
@@ -259,29 +285,36 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
     }
     if (live && p.dx != nullptr) row_store<T, V, C, LANES>(p.dx, at, d, lane, p.cols);
     if (post) {
-      float dg[EPL];
+      if (live && full_gate && p.dgate != nullptr) {
+        float dg[EPL];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+          dg[e] = d[e] * (float)scale.p[e / V].v[e % V] * fmaf(xh[e], (float)ow.p[e / V].v[e % V], (float)ob.p[e / V].v[e % V]);
+        row_store<T, V, C, LANES>(p.dgate, at, dg, lane, p.cols);
+      }
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         const int c = e / V, k = e % V;
-        const float s = (float)scale.p[c].v[k], g = (float)gr.p[c].v[k];
+        const float s = (float)scale.p[c].v[k], g = (float)gr.p[c].v[k], n = fmaf(xh[e], (float)ow.p[c].v[k], (float)ob.p[c].v[k]);
         if (!in[c]) d[e] = 0.f;
         const float dn = d[e] * (s * g);
-        dg[e] = d[e] * s * n[e];
         if (live) {
-          a_gate[e] = fmaf(d[e] * n[e], full_gate ? g : 1.f, a_gate[e]);
-          a_ow[e] = fmaf(dn, xh[e], a_ow[e]); a_ob[e] += dn;
+          a_gate[e] = fmaf(d[e] * n, full_gate ? g : 1.f, a_gate[e]);
+          a_ow[e] = fmaf(dn, xh[e], a_ow[e]);
+          if (BIAS) a_ob[e] += dn;
         }
         d[e] = dn * (float)ow.p[c].v[k];
         s1 += d[e]; s2 = fmaf(d[e], in[c] ? xh[e] : 0.f, s2);
       }
-      if (live && full_gate && p.dgate != nullptr) row_store<T, V, C, LANES>(p.dgate, at, dg, lane, p.cols);
       m = row_sum(s1, s2);
       m.x = p.layer ? m.x * inv : 0.f; m.y *= inv;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) d[e] = st.y * (d[e] - fmaf(xh[e], m.y, m.x));
       if (live && p.dh != nullptr) row_store<T, V, C, LANES>(p.dh, at, d, lane, p.cols);
     }
-    in_now = in_next;
+    row_copy(in_now.x, in_next.x); row_copy(in_now.h, in_next.h); row_copy(in_now.dout, in_next.dout);
+    row_copy(in_now.du, in_next.du); row_copy(in_now.g, in_next.g);
+    in_now.st = in_next.st;
   }
 
   float* part = p.part + (long long)blockIdx.x * 5 * p.cols;
@@ -308,9 +341,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
   };
   if (p.dscale != nullptr || (p.dgate != nullptr && !full_gate)) flush(a_gate, 0);
   if (p.dpost_w != nullptr) flush(a_ow, 1);
-  if (p.dpost_b != nullptr) flush(a_ob, 2);
+  if constexpr (BIAS) if (p.dpost_b != nullptr) flush(a_ob, 2);
   if (p.dpre_w != nullptr) flush(a_pw, 3);
-  if (p.dpre_b != nullptr) flush(a_pb, 4);
+  if constexpr (BIAS) if (p.dpre_b != nullptr) flush(a_pb, 4);
 }
 
 // Column sums of the partial rows, 64 columns and 16 row lanes a block.  blockIdx.y 0: dscale (each chunk's sum times its group's
@@ -355,14 +388,14 @@ __global__ __launch_bounds__(1024) void rnorm_sums_kernel(RNormParams p, long lo
 }
 
 // waves a row / elements a lane: the fewest lanes that hold the row at 8 elements each, up to 16 waves; wider rows take 16
-#define RNORM_BY_WIDTH(KERNEL, T, VEC, GRID, BLOCKS_OF)                                                                      \
+#define RNORM_BY_WIDTH(KERNEL, GRID, T, ...)                                                                      \
   do {                                                                                                                       \
-    if (p.cols <= 512) { GRID(4); hipLaunchKernelGGL((KERNEL<T, 1, 8, VEC>), dim3(grid), dim3(256), 0, st, p); }              \
-    else if (p.cols <= 1024) { GRID(2); hipLaunchKernelGGL((KERNEL<T, 2, 8, VEC>), dim3(grid), dim3(256), 0, st, p); }        \
-    else if (p.cols <= 2048) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 4, 8, VEC>), dim3(grid), dim3(256), 0, st, p); }        \
-    else if (p.cols <= 4096) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 8, 8, VEC>), dim3(grid), dim3(512), 0, st, p); }        \
-    else if (p.cols <= 8192) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 8, VEC>), dim3(grid), dim3(1024), 0, st, p); }      \
-    else { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 16, VEC>), dim3(grid), dim3(1024), 0, st, p); }                         \
+    if (p.cols <= 512) { GRID(4); hipLaunchKernelGGL((KERNEL<T, 1, 8, __VA_ARGS__>), dim3(grid), dim3(256), 0, st, p); }              \
+    else if (p.cols <= 1024) { GRID(2); hipLaunchKernelGGL((KERNEL<T, 2, 8, __VA_ARGS__>), dim3(grid), dim3(256), 0, st, p); }        \
+    else if (p.cols <= 2048) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 4, 8, __VA_ARGS__>), dim3(grid), dim3(256), 0, st, p); }        \
+    else if (p.cols <= 4096) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 8, 8, __VA_ARGS__>), dim3(grid), dim3(512), 0, st, p); }        \
+    else if (p.cols <= 8192) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 8, __VA_ARGS__>), dim3(grid), dim3(1024), 0, st, p); }      \
+    else { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 16, __VA_ARGS__>), dim3(grid), dim3(1024), 0, st, p); }                         \
   } while (0)
 
 static bool rnorm_vec(const RNormParams& p, int dtype) {
@@ -377,8 +410,8 @@ template <typename T>
 static int rnorm_fwd_launch(const RNormParams& p, bool vec, hipStream_t st) {
   unsigned grid = 0;
 #define RNORM_FWD_GRID(RG) grid = (unsigned)std::min<long long>((p.rows + (RG) - 1) / (RG), 256 * 16)
-  if (vec) RNORM_BY_WIDTH(rnorm_fwd_kernel, T, true, RNORM_FWD_GRID, 0);
-  else RNORM_BY_WIDTH(rnorm_fwd_kernel, T, false, RNORM_FWD_GRID, 0);
+  if (vec) RNORM_BY_WIDTH(rnorm_fwd_kernel, RNORM_FWD_GRID, T, true);
+  else RNORM_BY_WIDTH(rnorm_fwd_kernel, RNORM_FWD_GRID, T, false);
   VEEX_CHECK_LAUNCH();
   return 0;
 }
@@ -387,8 +420,11 @@ template <typename T>
 static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hipStream_t st) {
   const unsigned grid = (unsigned)chunks;
 #define RNORM_BWD_GRID(RG) (void)0
-  if (vec) RNORM_BY_WIDTH(rnorm_bwd_kernel, T, true, RNORM_BWD_GRID, 0);
-  else RNORM_BY_WIDTH(rnorm_bwd_kernel, T, false, RNORM_BWD_GRID, 0);
+  const bool bias = p.dpost_b != nullptr || p.dpre_b != nullptr;
+  if (vec && bias) RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, true, true);
+  else if (vec) RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, true, false);
+  else if (bias) RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, false, true);
+  else RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, false, false);
   VEEX_CHECK_LAUNCH();
   if (p.dgate != nullptr || p.dscale != nullptr || p.dpost_w != nullptr || p.dpost_b != nullptr || p.dpre_w != nullptr || p.dpre_b != nullptr) {
     const long long gate_rows = p.dgate != nullptr && p.rows_per_group > 1 ? std::min<long long>(p.groups, 1024) : 0;
@@ -398,10 +434,10 @@ static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hi
   return 0;
 }
 
-// rows of a chunk and chunks of a launch: about 512 blocks, none across a group's end
-static long long rnorm_chunks(long long rows, long long groups, long long& per_chunk, long long& per_group) {
-  const long long t = rows / groups;
-  const long long want = std::max<long long>((rows + 511) / 512, 4);
+// rows of a chunk and chunks of a launch: about as many blocks as the chip holds, none across a group's end
+static long long rnorm_chunks(long long rows, int cols, long long groups, long long& per_chunk, long long& per_group) {
+  const long long t = rows / groups, blocks = cols > 2048 ? 256 : 512;       // (resident at once: 8 waves a CU)
+  const long long want = std::max<long long>((rows + blocks - 1) / blocks, 4);
   if (groups == rows) { per_chunk = want; per_group = 1; return (rows + want - 1) / want; }   // (a gate per element, or one row)
   per_group = (t + want - 1) / want;
   per_chunk = (t + per_group - 1) / per_group;
@@ -461,7 +497,7 @@ long long veex_residual_norm_bwd_workspace_floats(long long rows, int cols, long
   if (rows < 0 || cols < 1 || groups < 1 || (rows > 0 && rows % groups != 0)) return -1;
   if (rows == 0) return 0;
   long long a, b;
-  return rnorm_chunks(rows, groups, a, b) * 5 * cols;
+  return rnorm_chunks(rows, cols, groups, a, b) * 5 * cols;
 }
 
 int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
@@ -474,7 +510,7 @@ int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
   RNormParams p;
   rnorm_fill(p, d);
   p.x_out = p.u = nullptr;
-  const long long chunks = rnorm_chunks(p.rows, p.groups, p.rows_per_chunk, p.chunks_per_group);
+  const long long chunks = rnorm_chunks(p.rows, p.cols, p.groups, p.rows_per_chunk, p.chunks_per_group);
   if (d->workspace_floats < chunks * 5 * p.cols) { veex_set_error("residual_norm backward: workspace of %lld floats is needed", chunks * 5 * p.cols); return VEEX_ENOMEM; }
   const bool vec = rnorm_vec(p, d->dtype);
   if (d->dtype == VEEX_T_F32) return rnorm_bwd_launch<float>(p, vec, chunks, st);
