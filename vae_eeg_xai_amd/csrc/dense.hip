@@ -14,46 +14,63 @@
 // ---------------------------------------------------------------------------------------------------------------
 #define DG_LD 68     // floats per LDS row: 64 + one 16-byte piece
 
-template <typename T, bool KC>
-__device__ __forceinline__ void dg_load(float (&r)[8], const DenseOperand& o, long long row0, long long rows, long long k0,
-                                        long long k_end, bool vec) {
-  // KC: k is the contiguous index: 4 threads a row, 8 k each; else the row index is: 8 threads a k, 8 rows each
-  const int t = threadIdx.x;
-  const T* p = static_cast<const T*>(o.p);
-  const long long row = row0 + (KC ? t >> 2 : 8 * (t & 7)), k = k0 + (KC ? 8 * (t & 3) : t >> 3);
-  const long long n = (row < rows && k < k_end) ? (KC ? k_end - k : rows - row) : 0;
-  const T* q = p + row * o.row_stride + k * o.k_stride;
-  if (vec) {                   // (n is 0 or at least 8)
-    constexpr int V = 16 / sizeof(T);
-    if (n <= 0) q = p;
+// One operand's 64 x 32 tiles, 8 elements a thread.  Whole pieces: 8 neighbours of the contiguous index (k: 4 threads a row, else 8
+// threads a k).  Otherwise single elements with neighbouring threads on neighbouring addresses (32 threads along k, 8 rows apart,
+// or 64 threads along the rows, 4 k's apart): eight at once from each thread's own place would touch eight times the lines.
+template <typename T, bool KC, bool vec>
+struct DgOperand {
+  const T *at, *safe;           // this thread's first element of the next tile; what a thread outside the tensor reads
+  long long rs, ks, rows_left, k_left;      // strides; rows and k's from this thread's first element on
+  __device__ __forceinline__ void init(const DenseOperand& o, long long row0, long long rows, long long k0, long long k_end) {
+    const int t = threadIdx.x;
+    rs = o.row_stride; ks = o.k_stride;
+    const int r = vec ? (KC ? t >> 2 : 8 * (t & 7)) : (KC ? t >> 5 : t & 63);
+    const int k = vec ? (KC ? 8 * (t & 3) : t >> 3) : (KC ? t & 31 : t >> 6);
+    rows_left = rows - row0 - r; k_left = k_end - k0 - k;
+    safe = static_cast<const T*>(o.p);
+    at = safe + (row0 + r) * rs + (k0 + k) * ks;
+  }
+  __device__ __forceinline__ void load(float (&r)[8]) {
+    if (vec) {
+      constexpr int V = 16 / sizeof(T);
+      const bool in = rows_left > 0 && k_left > 0;
+      const T* q = in ? at : safe;
 #pragma unroll
-    for (int c = 0; c < 8 / V; ++c) {
-      const Piece<T, V> x = piece_load<T, V>(q + c * V);
+      for (int c = 0; c < 8 / V; ++c) {
+        const Piece<T, V> x = piece_load<T, V>(q + c * V);
 #pragma unroll
-      for (int e = 0; e < V; ++e) r[c * V + e] = n > 0 ? (float)x.v[e] : 0.f;
+        for (int e = 0; e < V; ++e) r[c * V + e] = in ? (float)x.v[e] : 0.f;
+      }
+    } else {
+      T x[8];
+      bool in[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        in[e] = KC ? rows_left > 8 * e && k_left > 0 : rows_left > 0 && k_left > 4 * e;
+        x[e] = *(in[e] ? at + e * (KC ? 8 * rs : 4 * ks) : safe);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = in[e] ? (float)x[e] : 0.f;
     }
-  } else {                     // (elements past the end read the tensor's first one: eight loads at once instead of eight branches)
-    T x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = *(e < n ? q + e : p);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = e < n ? (float)x[e] : 0.f;
+    at += 32 * ks; k_left -= 32;
   }
-}
-template <bool KC>
-__device__ __forceinline__ void dg_store(float* s, const float (&r)[8]) {
-  const int t = threadIdx.x;
-  if (KC) {
+  __device__ __forceinline__ void store(float* s, const float (&r)[8]) const {
+    const int t = threadIdx.x;
+    if (!vec) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[(8 * (t & 3) + e) * DG_LD + (t >> 2)] = r[e];
-  } else {
-    float4* d = reinterpret_cast<float4*>(s + (t >> 3) * DG_LD + 8 * (t & 7));
-    d[0] = make_float4(r[0], r[1], r[2], r[3]);
-    d[1] = make_float4(r[4], r[5], r[6], r[7]);
+      for (int e = 0; e < 8; ++e) s[KC ? (t & 31) * DG_LD + (t >> 5) + 8 * e : ((t >> 6) + 4 * e) * DG_LD + (t & 63)] = r[e];
+    } else if (KC) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[(8 * (t & 3) + e) * DG_LD + (t >> 2)] = r[e];
+    } else {
+      float4* d = reinterpret_cast<float4*>(s + (t >> 3) * DG_LD + 8 * (t & 7));
+      d[0] = make_float4(r[0], r[1], r[2], r[3]);
+      d[1] = make_float4(r[4], r[5], r[6], r[7]);
+    }
   }
-}
+};
 
-template <typename T, bool AKC, bool BKC, bool SPLIT>
+template <typename T, bool AKC, bool BKC, bool SPLIT, bool VEC>
 __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
   __shared__ float As[2][32 * DG_LD], Bs[2][32 * DG_LD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -68,16 +85,20 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
   float ra[8], rb[8];
-  dg_load<T, AKC>(ra, g.a, i0, g.I, k_begin, k_end, g.vec_a);
-  dg_load<T, BKC>(rb, g.b, j0, g.J, k_begin, k_end, g.vec_b);
+  DgOperand<T, AKC, VEC> a;
+  DgOperand<T, BKC, VEC> b;
+  a.init(g.a, i0, g.I, k_begin, k_end);
+  b.init(g.b, j0, g.J, k_begin, k_end);
+  a.load(ra);
+  b.load(rb);
   int cur = 0;
   for (long long k0 = k_begin; k0 < k_end; k0 += 32, cur ^= 1) {
-    dg_store<AKC>(As[cur], ra);
-    dg_store<BKC>(Bs[cur], rb);
+    a.store(As[cur], ra);
+    b.store(Bs[cur], rb);
     __syncthreads();      // (the other buffer's readers passed the barrier of the turn before)
     if (k0 + 32 < k_end) {
-      dg_load<T, AKC>(ra, g.a, i0, g.I, k0 + 32, k_end, g.vec_a);
-      dg_load<T, BKC>(rb, g.b, j0, g.J, k0 + 32, k_end, g.vec_b);
+      a.load(ra);
+      b.load(rb);
     }
 #pragma unroll
     for (int s = 0; s < 16; ++s)
@@ -311,19 +332,21 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
   }
 }
 
-// db = the partial rows' sum, 64 columns and 16 row lanes a block
+// db = the partial rows' sum, 32 columns and 32 row lanes a block
 template <typename T>
 __global__ __launch_bounds__(1024) void dense_db_kernel(const float* part, int chunks, int n, void* db) {
-  __shared__ float s[16][64];
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, col = blockIdx.x * 64 + tx;
+  __shared__ float s[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
+  const float* p = part + min(col, n - 1);
   float a = 0.f;
-  if (col < n)
-    for (int c = ty; c < chunks; c += 16) a += part[(long long)c * n + col];
+#pragma unroll 8
+  for (int c = ty; c < chunks; c += 32) a += p[(long long)c * n];
   s[ty][tx] = a;
   __syncthreads();
   if (ty == 0 && col < n) {
     a = 0.f;
-    for (int q = 0; q < 16; ++q) a += s[q][tx];
+#pragma unroll
+    for (int q = 0; q < 32; ++q) a += s[q][tx];
     static_cast<T*>(db)[col] = (T)a;
   }
 }
@@ -378,15 +401,16 @@ template <typename T>
 static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
   general_split(g.I, g.J, g.K, g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
-  g.vec_a = operand_vec(g.a, kind == kKindDw ? g.I : g.K, sizeof(T));
-  g.vec_b = operand_vec(g.b, kind == kKindDx ? g.K : g.J, sizeof(T));
+  const bool vec = operand_vec(g.a, kind == kKindDw ? g.I : g.K, sizeof(T)) && operand_vec(g.b, kind == kKindDx ? g.K : g.J, sizeof(T));
   g.vec_e = dense_epi_vec(g.epi, g.J);
   const long long tiles = (g.I + 63) / 64 * ((g.J + 63) / 64);
   if (tiles > 0x7FFFFFFFll) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
   const dim3 grid((unsigned)tiles, (unsigned)g.splits);
-#define DG_GO(AK, BK)                                                                                              \
-  if (g.splits > 1) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, true>), grid, dim3(256), 0, st, g);         \
-  else hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, false>), grid, dim3(256), 0, st, g);
+#define DG_GO(AK, BK)                                                                                                             \
+  if (g.splits > 1 && vec) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, true, true>), grid, dim3(256), 0, st, g);           \
+  else if (g.splits > 1) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, true, false>), grid, dim3(256), 0, st, g);            \
+  else if (vec) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, false, true>), grid, dim3(256), 0, st, g);                     \
+  else hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, false, false>), grid, dim3(256), 0, st, g);
   if (kind == kKindFwd) { DG_GO(true, false) }
   else if (kind == kKindDx) { DG_GO(true, true) }
   else { DG_GO(false, false) }
@@ -451,16 +475,19 @@ static long long few_bytes(const VeexDense* d, const DenseGemm& g) {
 }
 
 // ---- large products -------------------------------------------------------------------------------------------------
-// A layer whose products have at least this many multiplications goes to dense_tile.hip: below it the packing and the tiles' edges
-// cost more than the fp32 MFMA of the general product.
-static const double kTileMin16 = 1 << 25, kTileMin32 = 1 << 27;
+// Which products go to dense_tile.hip.  16-bit types: all that need no packing (16x1024x1024 9.0 us on the general product, 8.5 on
+// the tiles; 512^3 15.3, 8.4), packed ones from 2^24 multiplications on (257x255x259 14.8, 12.6; 512x28x4096 forward 6.6, 8.8).
+// fp32, which is packed and multiplied six times: from 1.5e9 on (1000^3 34, 32; 2048x1024x1024 53, 43; 4096x1024x1024 90, 60) and 128
+// rows (64x4096x4096 34, 55).
+static bool lies_well(const VeexDense* d, const void* p, long long ld, long long cols);
 
 static bool uses_tiles(const VeexDense* d) {
-  const double work = (double)d->rows * d->k * d->n;
-  if (d->rows <= kFewRows) return false;
   // a tile addresses its operand by 32 bits from its first row on: 256 rows of up to 4 MB, 64 k's of up to 16 MB
   const long long widest = std::max<long long>(std::max<long long>(d->k, d->n), d->ldx);
-  return work >= (d->dtype == VEEX_T_F32 ? kTileMin32 : kTileMin16) && widest < (1 << 21);
+  if (widest >= (1 << 21)) return false;
+  const double work = (double)d->rows * d->k * d->n;
+  if (d->dtype == VEEX_T_F32) return work >= 1.5e9 && d->rows >= 128;
+  return work >= (1 << 24) || (lies_well(d, d->x, d->ldx, d->k) && lies_well(d, d->w, d->n, d->n) && lies_well(d, d->dy, d->n, d->n));
 }
 
 static long long round8(long long v) { return (v + 7) / 8 * 8; }
@@ -554,14 +581,13 @@ static int tiles_any(int kind, const VeexDense* d, const DenseGemm& g, const DtT
   return 0;
 }
 
-// x, w or dy as the tiles load it: where it lies, or packed into *at, which moves on
-static int tile_operand(const VeexDense* d, const void* p, long long ld, long long rows, int cols, char*& at, DtTensor& t, hipStream_t st) {
-  if (lies_well(d, p, ld, cols)) { t = {p, ld * 2, 0}; return 0; }
+// x, w or dy as the tiles load it: where it lies, or packed into *at, which moves on (the job is added to the list)
+static void tile_operand(const VeexDense* d, const void* p, long long ld, long long rows, int cols, char*& at, DtTensor& t, DtPack* jobs, int& n) {
+  if (lies_well(d, p, ld, cols)) { t = {p, ld * 2, 0}; return; }
   const long long plane = packed_plane(rows, cols);
   t = {at, round8(cols) * 2, plane};
-  const int rc = dense_pack_launch(d->dtype, p, ld, rows, cols, at, plane, st);
+  jobs[n++] = {p, at, ld, rows, plane, cols};
   at += planes_of(d) * plane;
-  return rc;
 }
 static long long tile_operand_bytes(const VeexDense* d, const void* p, long long ld, long long rows, int cols) {
   return lies_well(d, p, ld, cols) ? 0 : packed_bytes(d, rows, cols);
@@ -623,9 +649,12 @@ int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
   }
   if (!uses_tiles(d)) return general_any(kKindFwd, d->dtype, g, d->workspace, st);
   char* at = static_cast<char*>(d->workspace);
-  DtTensor x, w;
-  if (int rc = tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, st)) return rc;
-  if (int rc = tile_operand(d, d->w, d->n, d->k, d->n, at, w, st)) return rc;
+  DtTensor x = {}, w = {};
+  DtPack jobs[2];
+  int n = 0;
+  tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, jobs, n);
+  tile_operand(d, d->w, d->n, d->k, d->n, at, w, jobs, n);
+  if (int rc = dense_pack_launch(d->dtype, jobs, n, st)) return rc;
   return tiles_any(kKindFwd, d, g, x, w, at, st);
 }
 
@@ -672,7 +701,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
       VEEX_CHECK_LAUNCH();
     }
     if (p.part != nullptr) {
-      const dim3 grid((d->n + 63) / 64);
+      const dim3 grid((d->n + 31) / 32);
       if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_db_kernel<float>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
       else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_db_kernel<bf16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
       else hipLaunchKernelGGL((dense_db_kernel<f16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
@@ -689,19 +718,20 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
       if (int rc = general_any(kKindDw, d->dtype, dense_product(kKindDw, d, dz), slabs, st)) return rc;
     return 0;
   }
-  DtTensor x, w;
+  DtTensor x = {}, w = {};
+  DtPack jobs[3];
+  int n = 0;
   if (!l.dz_own) {
     char* p = ws;
-    if (int rc = tile_operand(d, d->dy, d->n, d->rows, d->n, p, dzt, st)) return rc;
+    tile_operand(d, d->dy, d->n, d->rows, d->n, p, dzt, jobs, n);
   }
-  if (d->dx != nullptr) {
-    if (int rc = tile_operand(d, d->w, d->n, d->k, d->n, at, w, st)) return rc;
+  if (d->dx != nullptr) tile_operand(d, d->w, d->n, d->k, d->n, at, w, jobs, n);
+  if (d->dw != nullptr) tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, jobs, n);
+  if (int rc = dense_pack_launch(d->dtype, jobs, n, st)) return rc;
+  if (d->dx != nullptr)
     if (int rc = tiles_any(kKindDx, d, dense_product(kKindDx, d, nullptr), dzt, w, slabs, st)) return rc;
-  }
-  if (d->dw != nullptr) {
-    if (int rc = tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, st)) return rc;
+  if (d->dw != nullptr)
     if (int rc = tiles_any(kKindDw, d, dense_product(kKindDw, d, nullptr), x, dzt, slabs, st)) return rc;
-  }
   return 0;
 }
 

@@ -185,7 +185,7 @@ struct DenseGemm {
   float* slab;           // [splits][I][J] when splits > 1
   int splits;
   long long k_per_split;
-  int vec_a, vec_b, vec_e;
+  int vec_e;             // the epilogue's tensors move in 16-byte pieces of 8 columns
 };
 
 #endif

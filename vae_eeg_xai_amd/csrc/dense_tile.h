@@ -19,7 +19,9 @@ struct DtGemm {
 
 // akc / bkc: that operand's k index is its contiguous one.  tile: 256 or 128 (16-bit types)
 int dense_tile_launch(int dtype, bool akc, bool bkc, int tile, const DtGemm& g, hipStream_t st);
-int dense_pack_launch(int dtype, const void* src, long long ld, long long rows, int cols, void* dst, long long plane_bytes, hipStream_t st);
+// up to three packings in one launch
+struct DtPack { const void* src; void* dst; long long ld, rows, plane_bytes; int cols; };
+int dense_pack_launch(int dtype, const DtPack* jobs, int n, hipStream_t st);
 
 // Eight fp32 values as their three bf16 terms: f = t1 + t2 + t3 to 2^-27 (each term rounds what the ones before left; the
 // differences are exact).  A value that is not finite, or that rounds to an infinity, is its first term alone.

@@ -300,12 +300,19 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
 // Packing: rows of a tensor (any row stride and alignment) as 16-byte aligned rows of `cols8` = cols rounded up to 8, zeros behind
 // the last column; an fp32 tensor as its three bf16 terms in three planes.  8 columns a thread.
 // ---------------------------------------------------------------------------------------------------------------
+struct DtPackJobs { DtPack job[3]; unsigned first[4]; int vec[3]; };     // first: a job's first workgroup; the last one's end
+
 template <typename T>
-__global__ __launch_bounds__(256) void dense_pack_kernel(const T* __restrict__ src, long long ld, long long rows, int cols, int cols8,
-                                                         char* __restrict__ dst, long long plane_bytes, bool vec) {
-  const int bpr = cols8 / 8;
-  const long long nb = rows * bpr;
-  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < nb; t += (long long)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void dense_pack_kernel(DtPackJobs jobs) {
+  const int q = blockIdx.x < jobs.first[1] ? 0 : blockIdx.x < jobs.first[2] ? 1 : 2;
+  const DtPack& o = jobs.job[q];
+  const T* __restrict__ src = static_cast<const T*>(o.src);
+  char* __restrict__ dst = static_cast<char*>(o.dst);
+  const long long ld = o.ld, plane_bytes = o.plane_bytes;
+  const int cols = o.cols, cols8 = (cols + 7) / 8 * 8, bpr = cols8 / 8;
+  const bool vec = jobs.vec[q];
+  const long long nb = o.rows * bpr, step = (long long)(jobs.first[q + 1] - jobs.first[q]) * 256;
+  for (long long t = (long long)(blockIdx.x - jobs.first[q]) * 256 + threadIdx.x; t < nb; t += step) {
     const long long r = nb <= 0xFFFFFFFFll ? (long long)((unsigned)t / (unsigned)bpr) : t / bpr;
     const int c = 8 * (int)(t - r * bpr);
     const T* p = src + r * ld + c;
@@ -320,7 +327,9 @@ __global__ __launch_bounds__(256) void dense_pack_kernel(const T* __restrict__ s
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = c + e < cols ? p[e] : (T)0.f;
+      for (int e = 0; e < 8; ++e) x[e] = p[c + e < cols ? e : 0];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = c + e < cols ? x[e] : (T)0.f;
     }
     char* d = dst + (r * cols8 + c) * 2;
     if constexpr (sizeof(T) == 2) {
@@ -337,15 +346,20 @@ __global__ __launch_bounds__(256) void dense_pack_kernel(const T* __restrict__ s
   }
 }
 
-int dense_pack_launch(int dtype, const void* src, long long ld, long long rows, int cols, void* dst, long long plane_bytes, hipStream_t st) {
-  const int cols8 = (cols + 7) / 8 * 8;
-  const bool vec = cols % 8 == 0 && trunk_aligned16(src) && ld * trunk_elem_bytes(dtype) % 16 == 0;
-  const long long nb = rows * (cols8 / 8);
-  const dim3 grid((unsigned)std::min<long long>((nb + 255) / 256, 1 << 16));
-  char* d = static_cast<char*>(dst);
-  if (dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_pack_kernel<float>), grid, dim3(256), 0, st, static_cast<const float*>(src), ld, rows, cols, cols8, d, plane_bytes, vec);
-  else if (dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_pack_kernel<bf16_t>), grid, dim3(256), 0, st, static_cast<const bf16_t*>(src), ld, rows, cols, cols8, d, plane_bytes, vec);
-  else hipLaunchKernelGGL((dense_pack_kernel<f16_t>), grid, dim3(256), 0, st, static_cast<const f16_t*>(src), ld, rows, cols, cols8, d, plane_bytes, vec);
+int dense_pack_launch(int dtype, const DtPack* jobs, int n, hipStream_t st) {
+  if (n == 0) return 0;
+  DtPackJobs j = {};
+  for (int q = 0; q < 3; ++q) {
+    j.first[q + 1] = j.first[q];
+    if (q >= n) continue;
+    j.job[q] = jobs[q];
+    j.vec[q] = jobs[q].cols % 8 == 0 && trunk_aligned16(jobs[q].src) && jobs[q].ld * trunk_elem_bytes(dtype) % 16 == 0;
+    j.first[q + 1] += (unsigned)std::min<long long>((jobs[q].rows * ((jobs[q].cols + 7) / 8) + 255) / 256, 1 << 16);
+  }
+  const dim3 grid(j.first[3]);
+  if (dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_pack_kernel<float>), grid, dim3(256), 0, st, j);
+  else if (dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_pack_kernel<bf16_t>), grid, dim3(256), 0, st, j);
+  else hipLaunchKernelGGL((dense_pack_kernel<f16_t>), grid, dim3(256), 0, st, j);
   VEEX_CHECK_LAUNCH();
   return 0;
 }
