@@ -266,7 +266,7 @@ int veex_band_outside_counts(const float* z, int N, int L, int nb, const double*
  * (16-bit number of (r, c) >= cut).  The number is half word c & 1 of word (c & 7) >> 1 of Philox-4x32-10 with key = seed and
  * counter (c >> 3, 0x44524F50, row low, row high), row = first_row + counter[0] + r: it does not depend on how a batch is
  * split over calls.  The mask is never stored: the backward pass is the same call on dy without residual.  residual and
- * counter (a DEVICE word read when the kernel runs) may be NULL; y may be x. */
+ * counter (a DEVICE word read when the kernel runs) may be NULL. */
 int veex_dropout(const void* x, const void* residual, void* y, long long rows, int cols, int dtype, double rate,
                  unsigned long long seed, unsigned long long first_row, const unsigned long long* counter, veexStream_t s);
 
@@ -282,7 +282,7 @@ int veex_dropout(const void* x, const void* residual, void* y, long long rows, i
  * Backward: dz = D'(dy) act'(z), dx = dz w^T, dw = x^T dz, db = column sums of dz; each of dx, dw, db may be NULL.  pre is what
  * the forward wrote there; for VEEX_ACT_RELU without residual it may be the forward's y instead (y > 0 exactly where an element
  * was kept and z > 0), for VEEX_ACT_NONE it is not read.  d(residual) is dy.
- * Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned,
+ * rows <= 2^31, k and n <= 2^30.  Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned,
  * of at least the bytes that the _workspace function of the direction returns for the same struct (host only; -1: bad). */
 typedef struct VeexDense {
   const void* x; const void* w; const void* bias; const void* residual;

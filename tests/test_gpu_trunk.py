@@ -72,7 +72,7 @@ def test_dense_sizes(ops, m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,k,n", [(300, 1000, 520), (1030, 264, 1001), (129, 4104, 260), (260, 5000, 136), (1500, 72, 2056), (2051, 513, 259)])
+@pytest.mark.parametrize("m,k,n", [(300, 1000, 520), (1030, 264, 1001), (129, 4104, 260), (260, 5000, 136), (1500, 72, 2056), (2051, 513, 259), (1500, 1032, 1104), (1303, 1001, 1207)])
 def test_dense_large(ops, m, k, n, dt):
     """On the 16-bit matrix cores: tiles that end inside the tensors, odd sizes that are packed, split reductions."""
     _check_dense(ops, m, k, n, dt, "silu", True, 0.1, True)
@@ -122,8 +122,8 @@ def test_dense_strides_alignment_and_shapes(ops, dt):
     b = _rand(g, 40, dtype=dtype).cuda()
     base = ops.dense(wide[:, 8:72].contiguous(), w, b, "gelu")
     assert torch.equal(ops.dense(wide[:, 8:72], w, b, "gelu"), base)                       # row stride 200, 16-byte aligned
-    off = wide[:, 9:73]
-    assert torch.equal(ops.dense(off, w, b, "gelu"), ops.dense(off.contiguous(), w, b, "gelu"))
+    e = 2 * ref.dense_bounds(dtype, wide[:, 9:73].double().cpu(), w.double().cpu(), b.double().cpu(), "gelu", None, None, None)[0]
+    ref.within(ops.dense(wide[:, 9:73], w, b, "gelu"), ops.dense(wide[:, 9:73].contiguous(), w, b, "gelu").double().cpu(), e)      # another kernel may serve it
     xt = wide[:, :64].t().contiguous().t()
     assert torch.equal(ops.dense(xt, w, b, "gelu"), ops.dense(wide[:, :64].contiguous(), w, b, "gelu"))
     wt = w.t().contiguous().t()
@@ -143,6 +143,38 @@ def test_dense_strides_alignment_and_shapes(ops, dt):
     assert torch.equal(d1, d2)
 
 
+def test_dense_fp16_sums_beyond_its_range(ops):
+    """z past 65504: y is an infinity (or 0 on the other side), and the gradient is the activation's limit, not NaN."""
+    x = torch.full((16, 64), 100.0, dtype=torch.float16, device="cuda")
+    w = torch.full((64, 16), 20.0, dtype=torch.float16, device="cuda")
+    w[:, 8:] = -20.0
+    for act in ("gelu", "silu", "relu"):
+        xs = x.clone().requires_grad_()
+        y = ops.dense(xs, w, None, act)
+        assert bool(torch.isinf(y[:, :8]).all()) and not y[:, 8:].any()
+        dx, = torch.autograd.grad(y, xs, torch.ones_like(y))
+        assert torch.equal(dx, torch.full_like(dx, 160.0))
+
+
+def test_low_level_ops_refuse_what_does_not_fit(ops):
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(8, 6, device="cuda")
+    y = torch.zeros(4, 6, device="cuda")
+    for bad in (lambda: ops.dense_fwd(x, torch.zeros(9, 6, device="cuda"), None, 0, None, 0.0, 0, 0, None, False),
+                lambda: ops.dense_fwd(x, w, torch.zeros(5, device="cuda"), 0, None, 0.0, 0, 0, None, False),
+                lambda: ops.dense_fwd(x, w.cpu(), None, 0, None, 0.0, 0, 0, None, False),
+                lambda: ops.dense_bwd(y[:3], x, w, None, 0, 0.0, 0, 0, None, True, True, True),
+                lambda: ops.dense_bwd(y, x, w, None, 1, 0.0, 0, 0, None, True, True, True),
+                lambda: ops.dense_bwd(y, x, w, y[:, :5], 1, 0.0, 0, 0, None, True, True, True),
+                lambda: ops.dropout_fwd(x, 0.5, 1, 0, w, None),
+                lambda: ops.residual_norm_fwd(x, x[:3], None, None, None, None, None, None, 1, 0, 1e-3, False),
+                lambda: ops.residual_norm_fwd(x, x, torch.zeros(3, 8, device="cuda"), None, None, None, None, None, 3, 0, 1e-3, False),
+                lambda: ops.residual_norm_bwd(x, x, None, None, None, None, None, None, 1, 0, 1e-3, torch.zeros(3, 4, device="cuda"), x, x, [True] * 8)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        ops.dense_fwd(x, w, None, 9, None, 0.0, 0, 0, None, False)
+
+
 def test_dense_no_rows(ops):
     x, w, b = torch.zeros(0, 16, device="cuda", requires_grad=True), torch.ones(16, 8, device="cuda", requires_grad=True), torch.ones(8, device="cuda", requires_grad=True)
     y = ops.dense(x, w, b, "relu", None, 0.5, 1)
@@ -155,7 +187,7 @@ def test_dense_no_rows(ops):
 def test_dense_infinities_and_nan_stay_in_their_rows(ops, dt):
     """A NaN row gives a NaN row, an infinity no finite value where it weighs in; no other row changes; relu passes NaN on."""
     dtype = TYPES[dt]
-    for m, k, n in ((40, 48, 56), (512, 256, 256)):
+    for m, k, n in ((40, 48, 56), (512, 256, 256), (1024, 1200, 1280)):        # the last: fp32 by split terms
         g = torch.Generator().manual_seed(2)
         x, w = _rand(g, m, k, dtype=dtype), _rand(g, k, n, dtype=dtype, scale=0.2)
         w[:, 3] = w[:, 3].abs() + torch.finfo(dtype).eps
@@ -481,10 +513,12 @@ def test_captured_training_pass_replays_with_fresh_numbers(ops):
     assert not torch.equal(seen[0], seen[1])
 
 
-def test_two_captured_graphs_share_nothing(ops):
+@pytest.mark.parametrize("dt,m,k,n", [("f32", 100, 640, 72), ("f32", 1, 6400, 100), ("f32", 1408, 1100, 1000), ("bf16", 300, 2048, 264), ("bf16", 301, 2047, 263)])
+def test_two_captured_graphs_share_nothing(ops, dt, m, k, n):
+    """The general product split, few rows, split fp32 terms, tiles with a split reduction, tiles of packed operands."""
     g = torch.Generator().manual_seed(15)
-    x = torch.randn(100, 640, generator=g).cuda()
-    w1, w2 = (torch.randn(640, 72, generator=g).cuda() for _ in range(2))
+    x = torch.randn(m, k, generator=g).to(TYPES[dt]).cuda()
+    w1, w2 = (torch.randn(k, n, generator=g).to(TYPES[dt]).cuda() for _ in range(2))
     want = ops.dense(x, w1, None, "gelu"), ops.dense(x, w2, None, "gelu")
     torch.cuda.synchronize()
     graphs, outs = [], []

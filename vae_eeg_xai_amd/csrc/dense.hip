@@ -123,15 +123,9 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
     const float4 lo = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3)), hi = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3) + 4);
     float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     if (SPLIT) {
-      float* s = g.slab + ((long long)blockIdx.y * g.I + i) * g.J + j;
-      if (g.J % 4 == 0) {
-        *reinterpret_cast<float4*>(s) = lo;
-        if (j + 4 < g.J) *reinterpret_cast<float4*>(s + 4) = hi;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (j + e < g.J) s[e] = v[e];
-      }
+      float* s = g.slab + ((long long)blockIdx.y * g.I + i) * slab_ld(g.J) + j;
+      *reinterpret_cast<float4*>(s) = lo;
+      if (j + 4 < g.J) *reinterpret_cast<float4*>(s + 4) = hi;
     } else {
       unsigned w[4] = {0u, 0u, 0u, 0u};
       if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
@@ -148,30 +142,23 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
   static_assert(SL == 1 || OB <= 64, "");
   __shared__ float part[SL > 1 ? 4 * OB * 9 : 1];
   const int bpr = (g.J + 7) / 8;
-  const long long nb = g.I * bpr, stride = g.I * g.J;
+  const long long nb = g.I * bpr, stride = g.I * slab_ld(g.J);
   const int ob = threadIdx.x % OB, sl = threadIdx.x / OB;
   for (long long b0 = (long long)blockIdx.x * OB; b0 < nb; b0 += (long long)gridDim.x * OB) {
     const long long b = min(b0 + ob, nb - 1);     // (every thread meets the barriers)
     const long long i = nb <= 0xFFFFFFFFll ? (long long)((unsigned)b / (unsigned)bpr) : b / bpr;
     const int j = 8 * (int)(b - i * bpr);
-    const float* s = g.slab + i * g.J + j;
+    const float* s = g.slab + i * slab_ld(g.J) + j;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    if (g.J % 4 == 0) {
-      const bool two = j + 4 < g.J;
+    const int second = j + 4 < g.J ? 4 : 0;
 #pragma unroll 8
-      for (int z = sl; z < g.splits; z += SL) {
-        const float4 x = *reinterpret_cast<const float4*>(s + z * stride);
-        const float4 t = *reinterpret_cast<const float4*>(s + z * stride + (two ? 4 : 0));
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        v[4] += t.x; v[5] += t.y; v[6] += t.z; v[7] += t.w;
-      }
-    } else {
-#pragma unroll 2
-      for (int z = sl; z < g.splits; z += SL)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += s[z * stride + min(e, g.J - 1 - j)];
+    for (int z = sl; z < g.splits; z += SL) {
+      const float4 x = *reinterpret_cast<const float4*>(s + z * stride);
+      const float4 t = *reinterpret_cast<const float4*>(s + z * stride + second);
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      v[4] += t.x; v[5] += t.y; v[6] += t.z; v[7] += t.w;
     }
     if (SL > 1) {
 #pragma unroll
@@ -250,7 +237,7 @@ __global__ __launch_bounds__(256) void dense_few_rows_kernel(DenseGemm g) {
       float a = 0.f;
 #pragma unroll
       for (int q = 0; q < KL; ++q) a += part[q][c];
-      g.slab[((long long)blockIdx.y * g.I + r) * g.J + blockIdx.x * CL * V + c] = a;
+      g.slab[((long long)blockIdx.y * g.I + r) * slab_ld(g.J) + blockIdx.x * CL * V + c] = a;
     }
   }
 }
@@ -362,10 +349,11 @@ static bool operand_vec(const DenseOperand& o, long long len, int elem) {
   return trunk_aligned16(o.p) && other * elem % 16 == 0 && len % 8 == 0;
 }
 
-// The reduction is split where the tiles alone leave most of the 256 CUs idle: up to 512 blocks, at least 64 k each.
+// The reduction is split where the tiles are fewer than two a CU: up to 512 blocks, at least 64 k each (1001x1003x1005 fp32 52 us
+// with one a CU, 41 with two, 38 with three, where 640^3 goes from 17 to 19).
 static void general_split(long long I, int J, long long K, int& splits, long long& per) {
   const long long tiles = (I + 63) / 64 * ((J + 63) / 64);
-  long long s = tiles >= 256 ? 1 : std::min<long long>(512 / tiles, (K + 63) / 64);
+  long long s = tiles >= 512 ? 1 : std::min<long long>(512 / tiles, (K + 63) / 64);
   s = std::max<long long>(s, 1);
   per = ((K + s - 1) / s + 31) / 32 * 32;
   splits = (int)((K + per - 1) / per);
@@ -376,7 +364,7 @@ static long long align256(long long b) { return (b + 255) / 256 * 256; }
 static long long general_bytes(long long I, int J, long long K) {
   int s; long long per;
   general_split(I, J, K, s, per);
-  return s > 1 ? align256((long long)s * I * J * 4) : 0;
+  return s > 1 ? align256(s * I * slab_ld(J) * 4) : 0;
 }
 
 template <typename T>
@@ -420,12 +408,11 @@ static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
   return 0;
 }
 
-// K >= 1 columns in, n >= 1 columns out, rows >= 0
 static int dense_check(const VeexDense* d, const char* who, DropArgs& drop) {
   if (d == nullptr || (d->struct_size != 0 && d->struct_size != (int)sizeof(VeexDense))) { veex_set_error("%s: struct_size is not this library's", who); return VEEX_EINVAL; }
   if (!trunk_dtype_ok(d->dtype) || d->activation < 0 || d->activation > VEEX_ACT_SIGMOID) { veex_set_error("%s: unknown dtype or activation", who); return VEEX_EINVAL; }
-  if (d->rows < 0 || d->rows > (1ll << 31) || d->k < 1 || d->n < 1 || d->ldx < d->k) {
-    veex_set_error("%s: 0 <= rows <= 2^31, k >= 1, n >= 1 and ldx >= k are needed", who); return VEEX_EINVAL;
+  if (d->rows < 0 || d->rows > (1ll << 31) || d->k < 1 || d->k > (1 << 30) || d->n < 1 || d->n > (1 << 30) || d->ldx < d->k) {
+    veex_set_error("%s: 0 <= rows <= 2^31, 1 <= k, n <= 2^30 and ldx >= k are needed", who); return VEEX_EINVAL;
   }
   if (!trunk_drop_args(d->rate, d->seed, d->first_row, d->counter, drop)) { veex_set_error("%s: rate %g is outside [0, 1 - 2^-17)", who, d->rate); return VEEX_EINVAL; }
   return 0;
@@ -439,7 +426,7 @@ static bool few_vec(const DenseGemm& g) { return operand_vec(g.b, g.J, sizeof(T)
 
 // about 1024 blocks, at least 64 k's each
 static void few_split(const DenseGemm& g, bool vec, int elem, int& splits, long long& per) {
-  const long long strips = vec ? (g.J * elem + 255) / 256 : (g.J + 63) / 64;
+  const long long strips = vec ? ((long long)g.J * elem + 255) / 256 : (g.J + 63) / 64;
   const long long s = std::max<long long>(std::min<long long>((1023 + strips) / strips, g.K / 64), 1);
   per = (g.K + s - 1) / s;
   splits = (int)((g.K + per - 1) / per);
@@ -451,7 +438,7 @@ static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
   few_split(g, vec, sizeof(T), g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
   g.vec_e = dense_epi_vec(g.epi, g.J);
-  const dim3 grid((unsigned)(vec ? (g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64), (unsigned)g.splits);
+  const dim3 grid((unsigned)(vec ? ((long long)g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64), (unsigned)g.splits);
 #define DF_GO(R)                                                                                              \
   if (vec) hipLaunchKernelGGL((dense_few_rows_kernel<T, R, true>), grid, dim3(256), 0, st, g);                 \
   else hipLaunchKernelGGL((dense_few_rows_kernel<T, R, false>), grid, dim3(256), 0, st, g);
@@ -471,12 +458,12 @@ static long long few_bytes(const VeexDense* d, const DenseGemm& g) {
   const int elem = trunk_elem_bytes(d->dtype);
   int s; long long per;
   few_split(g, operand_vec(g.b, g.J, elem), elem, s, per);
-  return align256((long long)s * g.I * g.J * 4);
+  return align256(s * g.I * slab_ld(g.J) * 4);
 }
 
 // ---- large products -------------------------------------------------------------------------------------------------
 // Which products go to dense_tile.hip.  16-bit types: all that need no packing (16x1024x1024 9.0 us on the general product, 8.5 on
-// the tiles; 512^3 15.3, 8.4), packed ones from 2^24 multiplications on (257x255x259 14.8, 12.6; 512x28x4096 forward 6.6, 8.8).
+// the tiles; 512^3 15.3, 8.4), packed ones from 2^26 multiplications on (257x255x259 10, 12.5; 385x383x387 13, 13.7).
 // fp32, which is packed and multiplied six times: from 1.5e9 on (1000^3 34, 32; 2048x1024x1024 53, 43; 4096x1024x1024 90, 60) and 128
 // rows (64x4096x4096 34, 55).
 static bool lies_well(const VeexDense* d, const void* p, long long ld, long long cols);
@@ -487,7 +474,7 @@ static bool uses_tiles(const VeexDense* d) {
   if (widest >= (1 << 21)) return false;
   const double work = (double)d->rows * d->k * d->n;
   if (d->dtype == VEEX_T_F32) return work >= 1.5e9 && d->rows >= 128;
-  return work >= (1 << 24) || (lies_well(d, d->x, d->ldx, d->k) && lies_well(d, d->w, d->n, d->n) && lies_well(d, d->dy, d->n, d->n));
+  return work >= (1 << 26) || (lies_well(d, d->x, d->ldx, d->k) && lies_well(d, d->w, d->n, d->n) && lies_well(d, d->dy, d->n, d->n));
 }
 
 static long long round8(long long v) { return (v + 7) / 8 * 8; }
@@ -513,9 +500,6 @@ static TilePlan tile_plan(const VeexDense* d, long long I, long long J, long lon
   static const Shape shapes32[] = {{1, 256, 128, 256, 2.4}, {2, 128, 128, 256, 1.3}};
   for (int q = 0; q < (f32 ? 2 : 3); ++q) {
     const Shape& sh = f32 ? shapes32[q] : shapes16[q];
-#ifdef DT_FORCE
-    if (sh.code != DT_FORCE) continue;
-#endif
     const long long tiles = (I + sh.bm - 1) / sh.bm * ((J + sh.bn - 1) / sh.bn);
     for (long long s = 1; s <= 64; s *= 2) {
       const long long per = ((K + s - 1) / s + bk - 1) / bk * bk, splits = (K + per - 1) / per;
@@ -526,9 +510,6 @@ static TilePlan tile_plan(const VeexDense* d, long long I, long long J, long lon
       if (c < cost) { cost = c; best = {sh.code, sh.bm, sh.bn, (unsigned)splits, per}; }
     }
   }
-#ifdef DT_SAY
-  printf("I %lld J %lld K %lld: tile %d splits %u\n", I, J, K, best.tile, best.splits);
-#endif
   return best;
 }
 
@@ -555,7 +536,7 @@ static long long product_bytes(int kind, const VeexDense* d) {
   if (kind == kKindFwd && few_rows(d)) return few_bytes(d, g);
   if (!uses_tiles(d)) return general_bytes(g.I, g.J, g.K);
   const TilePlan t = tile_plan(d, g.I, g.J, g.K);
-  return t.splits > 1 ? align256((long long)t.splits * g.I * g.J * 4) : 0;
+  return t.splits > 1 ? align256(t.splits * g.I * slab_ld(g.J) * 4) : 0;
 }
 
 static int general_any(int kind, int dtype, const DenseGemm& g, void* ws, hipStream_t st) {

@@ -154,7 +154,18 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& ep, float (&v)[8]
   if (ep.res != nullptr) load8<T>(r, static_cast<const T*>(ep.res) + at, n, vec);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += b[e];
-  if (ep.pre != nullptr) store8<T>(static_cast<T*>(ep.pre) + at, v, n, vec);
+  if (ep.pre != nullptr) {
+    // z for the backward pass, rounded to the tensors' type like the activation that a user would keep.  A finite z that the type
+    // does not hold (fp16 ends at 65504) stays finite: the derivative there is its limit, and at an infinity it would be NaN.
+    if constexpr (TrunkType<T>::code == VEEX_T_F16) {
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = __builtin_isfinite(v[e]) ? fminf(fmaxf(v[e], -65504.f), 65504.f) : v[e];
+      store8<T>(static_cast<T*>(ep.pre) + at, z, n, vec);
+    } else {
+      store8<T>(static_cast<T*>(ep.pre) + at, v, n, vec);
+    }
+  }
   dense_act<T, 8>(v, ep.act);
   if (ep.drop.cut != 0u)
 #pragma unroll
@@ -173,6 +184,9 @@ inline bool dense_epi_vec(const DenseEpi& ep, int J) {
   return true;
 }
 
+// floats between the rows of a split product's slab: rows of whole 16-byte pieces (what is behind column J is never used)
+__host__ __device__ inline long long slab_ld(int J) { return (J + 3LL) / 4 * 4; }
+
 // One operand: element (row, k) at p + row * row_stride + k * k_stride; exactly one of the strides is 1.
 struct DenseOperand { const void* p; long long row_stride, k_stride; };
 
@@ -182,7 +196,7 @@ struct DenseGemm {
   int J;
   long long K;
   DenseEpi epi;
-  float* slab;           // [splits][I][J] when splits > 1
+  float* slab;           // [splits][I][slab_ld(J)] when splits > 1
   int splits;
   long long k_per_split;
   int vec_e;             // the epilogue's tensors move in 16-byte pieces of 8 columns

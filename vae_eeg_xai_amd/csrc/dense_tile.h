@@ -24,13 +24,14 @@ struct DtPack { const void* src; void* dst; long long ld, rows, plane_bytes; int
 int dense_pack_launch(int dtype, const DtPack* jobs, int n, hipStream_t st);
 
 // Eight fp32 values as their three bf16 terms: f = t1 + t2 + t3 to 2^-27 (each term rounds what the ones before left; the
-// differences are exact).  A value that is not finite, or that rounds to an infinity, is its first term alone.
+// differences are exact).  A value that is not finite is its first term alone; one that would round to an infinity takes the largest bf16
+// first.  Terms below 2^-126 may be lost: values under about 2^-110 keep fewer bits.
 __device__ __forceinline__ void dt_store_planes(char* dst, long long plane_bytes, const float (&f)[8]) {
   Piece<bf16_t, 8> t[3];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const bf16_t a = (bf16_t)f[e];
-    const bool fin = __builtin_isfinite((float)a);
+    const bool fin = __builtin_isfinite(f[e]);
+    const bf16_t a = (bf16_t)(fin ? fminf(fmaxf(f[e], -0x1.FEp127f), 0x1.FEp127f) : f[e]);
     const float r1 = fin ? f[e] - (float)a : 0.f;
     const bf16_t b = (bf16_t)r1;
     const float r2 = r1 - (float)b;

@@ -269,22 +269,17 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
           *reinterpret_cast<DT_LDS dt_f4*>(strip + ((mi - m0) * 32 + l31) * CW * 4 + (((nj * 8 + 2 * q + lh) ^ (l31 & 7)) * 16)) =
               dt_f4{acc[mi][nj][4 * q], acc[mi][nj][4 * q + 1], acc[mi][nj][4 * q + 2], acc[mi][nj][4 * q + 3]};
     dt_wave_sync();
-    long long i = i0 + (wi * MT + m0) * 32 + lane / OCT, at = i * g.J + j;
+    const long long ld = g.slab != nullptr ? slab_ld(g.J) : g.J;
+    long long i = i0 + (wi * MT + m0) * 32 + lane / OCT, at = i * ld + j;
 #pragma unroll 2
-    for (int r = lane / OCT; r < 32 * SM; r += RPP, i += RPP, at += (long long)RPP * g.J) {
+    for (int r = lane / OCT; r < 32 * SM; r += RPP, i += RPP, at += RPP * ld) {
       const dt_f4 lo = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o) ^ (r & 7)) * 16));
       const dt_f4 hi = *reinterpret_cast<DT_LDS dt_f4*>(strip + r * CW * 4 + (((2 * o + 1) ^ (r & 7)) * 16));
       if (i >= g.I || j >= g.J) continue;
       if (g.slab != nullptr) {
-        float* s = g.slab + z * g.I * g.J + at;
-        if (g.J % 4 == 0) {
-          *reinterpret_cast<dt_f4*>(s) = lo;
-          if (j + 4 < g.J) *reinterpret_cast<dt_f4*>(s + 4) = hi;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (j + e < g.J) s[e] = e < 4 ? lo[e & 3] : hi[e & 3];
-        }
+        float* s = g.slab + z * g.I * ld + at;
+        *reinterpret_cast<dt_f4*>(s) = lo;
+        if (j + 4 < g.J) *reinterpret_cast<dt_f4*>(s + 4) = hi;
       } else {
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         unsigned w[4] = {0u, 0u, 0u, 0u};

@@ -78,7 +78,7 @@ extern "C" int veex_dropout(const void* x, const void* residual, void* y, long l
   if (x == nullptr || y == nullptr || rows < 0 || cols < 1 || !trunk_dtype_ok(dtype)) {
     veex_set_error("dropout: x and y, rows >= 0, cols >= 1 and a dtype of VEEX_T_* are needed"); return VEEX_EINVAL;
   }
-  if (rows > (1ll << 40) || rows * cols > (1ll << 46)) { veex_set_error("dropout: more rows than a launch addresses"); return VEEX_EINVAL; }
+  if (cols > (1 << 30) || rows > (1ll << 46) / cols) { veex_set_error("dropout: at most 2^30 columns and 2^46 elements"); return VEEX_EINVAL; }
   if (!trunk_drop_args(rate, seed, first_row, counter, d)) {
     veex_set_error("dropout: rate %g is outside [0, 1 - 2^-17)", rate); return VEEX_EINVAL;
   }

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNo
     row = min(row, p.rows - 1);
     row_load<T, V, C, LANES>(r.x, p.x, row * p.cols, lane, p.cols);
     if (p.h != nullptr) row_load<T, V, C, LANES>(r.h, p.h, row * p.cols, lane, p.cols);
-    if (p.gate != nullptr) row_load<T, V, C, LANES>(r.g, p.gate, row / p.rows_per_group * p.cols, lane, p.cols);
+    if (p.gate != nullptr) row_load<T, V, C, LANES>(r.g, p.gate, (long long)((unsigned)row / (unsigned)p.rows_per_group) * p.cols, lane, p.cols);      // (rows <= 2^31)
     else row_fill<T, V, C, LANES>(r.g, 1.f);
   };
   const long long step = (long long)gridDim.x * RG;
@@ -409,7 +409,8 @@ static bool rnorm_vec(const RNormParams& p, int dtype) {
 template <typename T>
 static int rnorm_fwd_launch(const RNormParams& p, bool vec, hipStream_t st) {
   unsigned grid = 0;
-#define RNORM_FWD_GRID(RG) grid = (unsigned)std::min<long long>((p.rows + (RG) - 1) / (RG), 256 * 16)
+  // (as many blocks as the chip holds at a time: 8192x4096 64 us with 4096, 59 with 1024)
+#define RNORM_FWD_GRID(RG) grid = (unsigned)std::min<long long>((p.rows + (RG) - 1) / (RG), 1024)
   if (vec) RNORM_BY_WIDTH(rnorm_fwd_kernel, RNORM_FWD_GRID, T, true);
   else RNORM_BY_WIDTH(rnorm_fwd_kernel, RNORM_FWD_GRID, T, false);
   VEEX_CHECK_LAUNCH();

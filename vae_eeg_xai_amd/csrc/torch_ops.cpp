@@ -68,7 +68,18 @@ struct BelowUnlessRecording {
 };
 
 // ------------------------------------------------------------------------------------------------ dropout
+// (the low-level ops check what keeps their kernels inside the tensors; the public ones run the same checks before autograd)
+void check_dropout_args(const Tensor& x, const Tensor& residual, double rate, int64_t first_row, const Tensor& counter) {
+  check_type("dropout", x);
+  check_same("dropout", x, residual, "residual");
+  check_drop("dropout", x, rate, first_row, counter);
+  TORCH_CHECK_VALUE(x.dim() >= 1, "dropout: x has no columns");
+  TORCH_CHECK_VALUE(x.size(-1) <= 1 << 30, "dropout: x ", x.sizes(), " has more than 2^30 columns");
+  TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x.sizes(), "dropout: residual ", residual.sizes(), " is not of x's shape ", x.sizes());
+}
+
 Tensor dropout_fwd(const Tensor& x_in, double rate, int64_t seed, int64_t first_row, const OptTensor& residual_in, const OptTensor& counter) {
+  check_dropout_args(x_in, get(residual_in), rate, first_row, get(counter));
   const c10::DeviceGuard guard(x_in.device());
   const Tensor x = x_in.contiguous(), residual = contig(get(residual_in));
   Tensor y = at::empty_like(x);
@@ -109,11 +120,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, double rate, int64_t seed, int64_t first_row, const OptTensor& residual_in, const OptTensor& counter) {
   const Tensor residual = get(residual_in);
-  check_type("dropout", x);
-  check_same("dropout", x, residual, "residual");
-  check_drop("dropout", x, rate, first_row, get(counter));
-  TORCH_CHECK_VALUE(x.dim() >= 1, "dropout: x has no columns");
-  TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x.sizes(), "dropout: residual ", residual.sizes(), " is not of x's shape ", x.sizes());
+  check_dropout_args(x, residual, rate, first_row, get(counter));
   if (at::GradMode::is_enabled() && (learns(x) || learns(residual))) return Dropout::apply(x, rate, seed, first_row, residual_in, counter);
   return call_dropout_fwd(x, rate, seed, first_row, residual_in, counter);
 }
@@ -133,6 +140,26 @@ Tensor as_rows(const Tensor& x) {
   const Tensor r = x.dim() == 2 ? x : x.reshape({rows_of(x), x.size(-1)});
   if (r.size(0) <= 1) return r.contiguous();
   return (r.size(1) == 1 || r.stride(1) == 1) && r.stride(0) >= r.size(1) ? r : r.contiguous();
+}
+
+std::vector<int64_t> dense_shape(const Tensor& x, const Tensor& w) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = w.size(1);
+  return s;
+}
+
+void check_dense_args(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, double rate, int64_t first_row, const Tensor& counter) {
+  check_type("dense", x);
+  check_same("dense", x, w, "w");
+  check_same("dense", x, bias, "bias");
+  check_same("dense", x, residual, "residual");
+  check_drop("dense", x, rate, first_row, counter);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(0) && w.size(0) > 0 && w.size(1) > 0, "dense: x ", x.sizes(),
+                    " is not (..., K) for w ", w.sizes(), " = (K, N) with K, N >= 1");
+  TORCH_CHECK_VALUE(w.size(0) <= 1 << 30 && w.size(1) <= 1 << 30, "dense: w ", w.sizes(), " has more than 2^30 rows or columns");
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == w.size(1)), "dense: bias ", bias.sizes(), " is not (", w.size(1), ",)");
+  TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == at::IntArrayRef(dense_shape(x, w)), "dense: residual ", residual.sizes(),
+                    " is not of y's shape ", at::IntArrayRef(dense_shape(x, w)));
 }
 
 VeexDense dense_desc(const Tensor& x, const Tensor& w, int64_t activation, double rate, int64_t seed, int64_t first_row, const Tensor& counter) {
@@ -155,14 +182,9 @@ Tensor workspace(VeexDense& d, long long bytes, const Tensor& x, const char* wha
   return w;
 }
 
-std::vector<int64_t> dense_shape(const Tensor& x, const Tensor& w) {
-  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
-  s.back() = w.size(1);
-  return s;
-}
-
 std::tuple<Tensor, Tensor> dense_fwd(const Tensor& x_in, const Tensor& w_in, const OptTensor& bias_in, int64_t activation,
                                      const OptTensor& residual_in, double rate, int64_t seed, int64_t first_row, const OptTensor& counter, bool keep) {
+  check_dense_args(x_in, w_in, get(bias_in), get(residual_in), rate, first_row, get(counter));
   const c10::DeviceGuard guard(x_in.device());
   const Tensor x = as_rows(x_in), w = w_in.contiguous(), bias = contig(get(bias_in)), residual = contig(get(residual_in));
   Tensor y = at::empty(dense_shape(x_in, w), x.options());
@@ -179,6 +201,9 @@ std::tuple<Tensor, Tensor> dense_fwd(const Tensor& x_in, const Tensor& w_in, con
 std::tuple<Tensor, Tensor, Tensor> dense_bwd(const Tensor& dy_in, const Tensor& x_in, const Tensor& w_in, const OptTensor& pre_in,
                                              int64_t activation, double rate, int64_t seed, int64_t first_row, const OptTensor& counter,
                                              bool need_x, bool need_w, bool need_b) {
+  check_dense_args(x_in, w_in, Tensor(), dy_in, rate, first_row, get(counter));       // (dy is of the residual's shape)
+  check_same("dense", x_in, get(pre_in), "pre");
+  TORCH_CHECK_VALUE(activation == VEEX_ACT_NONE || (pre_in.has_value() && pre_in->sizes() == dy_in.sizes()), "dense backward: pre is not of dy's shape ", dy_in.sizes());
   const c10::DeviceGuard guard(x_in.device());
   const Tensor x = as_rows(x_in), w = w_in.contiguous(), dy = dy_in.contiguous(), pre = contig(get(pre_in));
   const bool rows = x.size(0) > 0;
@@ -244,24 +269,31 @@ struct Dense : torch::autograd::Function<Dense> {
 Tensor dense(const Tensor& x, const Tensor& w, const OptTensor& bias_in, std::optional<std::string> activation, const OptTensor& residual_in, double rate,
              int64_t seed, int64_t first_row, const OptTensor& counter) {
   const Tensor bias = get(bias_in), residual = get(residual_in);
-  check_type("dense", x);
-  check_same("dense", x, w, "w");
-  check_same("dense", x, bias, "bias");
-  check_same("dense", x, residual, "residual");
-  check_drop("dense", x, rate, first_row, get(counter));
+  check_dense_args(x, w, bias, residual, rate, first_row, get(counter));
   const int act = activation_code(activation);
-  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(0) && w.size(0) > 0 && w.size(1) > 0, "dense: x ", x.sizes(),
-                    " is not (..., K) for w ", w.sizes(), " = (K, N) with K, N >= 1");
-  TORCH_CHECK_VALUE(w.size(0) <= INT32_MAX && w.size(1) <= INT32_MAX, "dense: w ", w.sizes(), " is beyond 2^31 - 1 rows or columns");
-  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == w.size(1)), "dense: bias ", bias.sizes(), " is not (", w.size(1), ",)");
-  TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == at::IntArrayRef(dense_shape(x, w)), "dense: residual ", residual.sizes(),
-                    " is not of y's shape ", at::IntArrayRef(dense_shape(x, w)));
   if (at::GradMode::is_enabled() && (learns(x) || learns(w) || learns(bias) || learns(residual)))
     return Dense::apply(x, w, bias_in, (int64_t)act, residual_in, rate, seed, first_row, counter);
   return std::get<0>(call_dense_fwd(x, w, bias_in, act, residual_in, rate, seed, first_row, counter, false));
 }
 
 // ------------------------------------------------------------------------------------------------ residual_norm
+void check_norm_args(const Tensor (&t)[8], int64_t groups, double eps) {
+  static const char* const names[8] = {"x", "h", "gate", "scale", "post_weight", "post_bias", "pre_weight", "pre_bias"};
+  const Tensor& x = t[0];
+  check_type("residual_norm", x);
+  for (int i = 1; i < 8; ++i) check_same("residual_norm", x, t[i], names[i]);
+  TORCH_CHECK_VALUE(eps >= 0.0, "residual_norm: eps has to be >= 0");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= VEEX_NORM_MAX_COLS, "residual_norm: rows of 1 to ", VEEX_NORM_MAX_COLS,
+                    " columns, not x ", x.sizes());
+  TORCH_CHECK_VALUE(t[1].defined() || !(t[2].defined() || t[3].defined() || t[4].defined() || t[5].defined()),
+                    "residual_norm: gate, scale and the post norm's parameters go with h");
+  TORCH_CHECK_VALUE(!t[1].defined() || t[1].sizes() == x.sizes(), "residual_norm: h (", t[1].sizes(), ") is not of x's shape ", x.sizes());
+  for (int i = 3; i < 8; ++i)
+    TORCH_CHECK_VALUE(!t[i].defined() || (t[i].dim() == 1 && t[i].size(0) == x.size(-1)), "residual_norm: ", names[i], " ", t[i].sizes(), " is not (", x.size(-1), ",)");
+  TORCH_CHECK_VALUE(groups >= 1 && (!t[2].defined() || t[2].numel() == 0 || (t[2].numel() == groups * x.size(-1) && rows_of(x) % groups == 0)),
+                    "residual_norm: gate ", t[2].sizes(), " does not go with x ", x.sizes());
+}
+
 VeexResidualNorm norm_desc(const Tensor (&t)[8], int64_t groups, int64_t kind, double eps) {
   VeexResidualNorm d = {};
   d.struct_size = sizeof(d);
@@ -277,6 +309,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_fwd(const Tensor& x, const OptTensor& h,
                                             double eps, bool keep) {
   const c10::DeviceGuard guard(x.device());
   const Tensor t[8] = {x.contiguous(), contig(get(h)), contig(get(gate)), contig(get(scale)), contig(get(post_w)), contig(get(post_b)), contig(get(pre_w)), contig(get(pre_b))};
+  check_norm_args(t, groups, eps);
   Tensor out = h.has_value() ? at::empty_like(t[0]) : at::empty({0}, x.options());
   Tensor u = at::empty_like(t[0]);
   Tensor stats = at::empty({keep ? rows_of(x) : 0, 4}, x.options().dtype(at::kFloat));
@@ -296,6 +329,12 @@ std::vector<Tensor> norm_bwd(const Tensor& x, const OptTensor& h, const OptTenso
   const c10::DeviceGuard guard(x.device());
   const Tensor t[8] = {x.contiguous(), contig(get(h)), contig(get(gate)), contig(get(scale)), contig(get(post_w)), contig(get(post_b)), contig(get(pre_w)), contig(get(pre_b))};
   const Tensor dx_out = contig(get(dx_out_in)), du = contig(get(du_in));
+  check_norm_args(t, groups, eps);
+  check_same("residual_norm", x, dx_out, "dx_out");
+  check_same("residual_norm", x, du, "du");
+  TORCH_CHECK_VALUE((!dx_out.defined() || dx_out.sizes() == x.sizes()) && (!du.defined() || du.sizes() == x.sizes()) && stats.is_contiguous() &&
+                        stats.scalar_type() == at::kFloat && stats.device() == x.device() && stats.numel() == rows_of(x) * 4,
+                    "residual_norm backward: dx_out, du or stats do not go with x ", x.sizes());
   const bool rows = rows_of(x) > 0;
   std::vector<Tensor> g(8);
   void* out[8];
@@ -373,26 +412,15 @@ int64_t gate_groups(const Tensor& gate, const Tensor& x) {
 
 std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& h_in, const OptTensor& gate_in, const OptTensor& scale, const OptTensor& post_w,
                                          const OptTensor& post_b, const OptTensor& pre_w, const OptTensor& pre_b, std::string kind, double eps) {
-  const Tensor h = get(h_in), gate = get(gate_in);
-  const std::pair<const char*, Tensor> vectors[5] = {{"scale", get(scale)}, {"post_weight", get(post_w)}, {"post_bias", get(post_b)}, {"pre_weight", get(pre_w)}, {"pre_bias", get(pre_b)}};
-  check_type("residual_norm", x);
-  check_same("residual_norm", x, h, "h");
-  check_same("residual_norm", x, gate, "gate");
-  for (const auto& v : vectors) check_same("residual_norm", x, v.second, v.first);
+  const Tensor t[8] = {x, get(h_in), get(gate_in), get(scale), get(post_w), get(post_b), get(pre_w), get(pre_b)};
+  const Tensor &h = t[1], &gate = t[2];
   TORCH_CHECK_VALUE(kind == "layer" || kind == "rms", "residual_norm: kind '", kind, "' is neither 'layer' nor 'rms'");
-  TORCH_CHECK_VALUE(eps >= 0.0, "residual_norm: eps has to be >= 0");
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= VEEX_NORM_MAX_COLS, "residual_norm: rows of 1 to ", VEEX_NORM_MAX_COLS,
-                    " columns, not x ", x.sizes());
-  TORCH_CHECK_VALUE(h.defined() || !(gate.defined() || scale.has_value() || post_w.has_value() || post_b.has_value()),
-                    "residual_norm: gate, scale and the post norm's parameters go with h");
-  TORCH_CHECK_VALUE(!h.defined() || h.sizes() == x.sizes(), "residual_norm: h (", h.sizes(), ") is not of x's shape ", x.sizes());
-  bool grad = learns(x) || learns(h) || learns(gate);
-  for (const auto& v : vectors) {
-    TORCH_CHECK_VALUE(!v.second.defined() || (v.second.dim() == 1 && v.second.size(0) == x.size(-1)), "residual_norm: ", v.first, " ", v.second.sizes(),
-                      " is not (", x.size(-1), ",)");
-    grad = grad || learns(v.second);
-  }
+  check_type("residual_norm", x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "residual_norm: rows of 1 to ", VEEX_NORM_MAX_COLS, " columns, not x ", x.sizes());
   const int64_t groups = gate.defined() ? gate_groups(gate, x) : 1, code = kind == "layer" ? VEEX_NORM_LAYER : VEEX_NORM_RMS;
+  check_norm_args(t, groups, eps);
+  bool grad = false;
+  for (const Tensor& v : t) grad = grad || learns(v);
   if (grad && at::GradMode::is_enabled()) {
     const auto r = ResidualNorm::apply(x, h_in, gate_in, scale, post_w, post_b, pre_w, pre_b, groups, code, eps);
     return {h.defined() ? r[0] : x, r.back()};
