@@ -70,16 +70,20 @@ struct DgOperand {
   }
 };
 
-template <typename T, bool AKC, bool BKC, bool SPLIT, bool VEC>
-__global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
-  __shared__ float As[2][32 * DG_LD], Bs[2][32 * DG_LD];
+struct DgLds { float a[2][32 * DG_LD], b[2][32 * DG_LD]; };
+
+// One tile of one split: part of C.  GRAD: a gradient, which has no epilogue.
+template <typename T, bool AKC, bool BKC, bool GRAD, bool VEC>
+__device__ __forceinline__ void dg_tile(const DenseGemm& g, unsigned tile, unsigned split, DgLds& lds) {
+  float (&As)[2][32 * DG_LD] = lds.a;
+  float (&Bs)[2][32 * DG_LD] = lds.b;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l31 = lane & 31, lh = lane >> 5, wi = wave & 1, wj = wave >> 1;
   const int tiles_j = (g.J + 63) / 64;
-  const long long ti = blockIdx.x / tiles_j;
-  const long long i0 = ti * 64;
-  const int j0 = (int)(blockIdx.x - ti * tiles_j) * 64;
-  const long long k_begin = (long long)blockIdx.y * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
+  const unsigned ti = tile / (unsigned)tiles_j;
+  const long long i0 = ti * 64ll;
+  const int j0 = (int)(tile - ti * tiles_j) * 64;
+  const long long k_begin = (long long)split * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
 
   f32x16 acc;
 #pragma unroll
@@ -112,20 +116,22 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
   for (int q = 0; q < 4; ++q)
     *reinterpret_cast<float4*>(strip + l31 * 36 + 8 * q + 4 * lh) = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
   __syncthreads();
-  const unsigned long long base = drop_base(g.epi.drop);
+  const unsigned long long base = GRAD ? 0ull : drop_base(g.epi.drop);
   const int j = j0 + wj * 32 + 8 * (lane & 3);
   float bias[8];
-  if (!SPLIT) dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
+  if (!GRAD && g.splits == 1) dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
 #pragma unroll 1
   for (int r = lane >> 2; r < 32; r += 16) {
     const long long i = i0 + wi * 32 + r;
     if (i >= g.I || j >= g.J) continue;
     const float4 lo = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3)), hi = *reinterpret_cast<const float4*>(strip + r * 36 + 8 * (lane & 3) + 4);
     float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    if (SPLIT) {
-      float* s = g.slab + ((long long)blockIdx.y * g.I + i) * slab_ld(g.J) + j;
+    if (g.splits > 1) {
+      float* s = g.slab + ((long long)split * g.I + i) * slab_ld(g.J) + j;
       *reinterpret_cast<float4*>(s) = lo;
       if (j + 4 < g.J) *reinterpret_cast<float4*>(s + 4) = hi;
+    } else if (GRAD) {
+      store8<T>(static_cast<T*>(g.epi.y) + i * g.J + j, v, g.J - j, g.vec_e);
     } else {
       unsigned w[4] = {0u, 0u, 0u, 0u};
       if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
@@ -134,27 +140,42 @@ __global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
   }
 }
 
-// Sum of the slabs, then the epilogue: 8 columns of one row a thread.  Where the output alone is too small to fill the chip, SL
-// threads share an output block, each adding every SL'th slab up; the SL sums are added in a fixed order.
-template <typename T, int SL>
-__global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dense_general_kernel(DenseGemm g) {
+  __shared__ DgLds lds;
+  dg_tile<T, true, false, false, VEC>(g, blockIdx.x, blockIdx.y, lds);
+}
+
+// Both gradients in one launch (either may have no blocks): a small layer's products leave most of the chip idle one after the other,
+// and a launch costs the host as much as such a product costs the GPU.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dense_general_grads_kernel(DenseGemm dx, DenseGemm dw, unsigned dx_tiles, unsigned dx_blocks, unsigned dw_tiles) {
+  __shared__ DgLds lds;
+  const unsigned b = blockIdx.x;
+  if (b < dx_blocks) dg_tile<T, true, true, true, VEC>(dx, b % dx_tiles, b / dx_tiles, lds);
+  else dg_tile<T, false, false, true, VEC>(dw, (b - dx_blocks) % dw_tiles, (b - dx_blocks) / dw_tiles, lds);
+}
+
+// Sum of the slabs [splits][I][slab_ld(J)], 8 columns of one row a thread.  Where the output alone is too small to fill the chip, SL
+// threads share an output block, each adding every SL'th slab up; the SL sums are added in a fixed order.  out(v, i, j) gets the sums.
+template <int SL, typename OUT>
+__device__ __forceinline__ void dense_sum_slabs(const float* slab, long long I, int J, int splits, unsigned block, unsigned blocks, float* part, OUT out) {
   constexpr int OB = 256 / SL;                    // output blocks of a workgroup; a wave holds all of them (SL > 1), 64 / OB times
   static_assert(SL == 1 || OB <= 64, "");
-  __shared__ float part[SL > 1 ? 4 * OB * 9 : 1];
-  const int bpr = (g.J + 7) / 8;
-  const long long nb = g.I * bpr, stride = g.I * slab_ld(g.J);
+  const int bpr = (J + 7) / 8;
+  const long long nb = I * bpr, stride = I * slab_ld(J);
   const int ob = threadIdx.x % OB, sl = threadIdx.x / OB;
-  for (long long b0 = (long long)blockIdx.x * OB; b0 < nb; b0 += (long long)gridDim.x * OB) {
+  for (long long b0 = (long long)block * OB; b0 < nb; b0 += (long long)blocks * OB) {
     const long long b = min(b0 + ob, nb - 1);     // (every thread meets the barriers)
     const long long i = nb <= 0xFFFFFFFFll ? (long long)((unsigned)b / (unsigned)bpr) : b / bpr;
     const int j = 8 * (int)(b - i * bpr);
-    const float* s = g.slab + i * slab_ld(g.J) + j;
+    const float* s = slab + i * slab_ld(J) + j;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    const int second = j + 4 < g.J ? 4 : 0;
+    const int second = j + 4 < J ? 4 : 0;
 #pragma unroll 8
-    for (int z = sl; z < g.splits; z += SL) {
+    for (int z = sl; z < splits; z += SL) {
       const float4 x = *reinterpret_cast<const float4*>(s + z * stride);
       const float4 t = *reinterpret_cast<const float4*>(s + z * stride + second);
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
@@ -174,13 +195,67 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = part[ob * 9 + e] + part[(OB + ob) * 9 + e] + (part[(2 * OB + ob) * 9 + e] + part[(3 * OB + ob) * 9 + e]);
     }
-    if (sl == 0 && b0 + ob < nb) {
-      unsigned w[4] = {0u, 0u, 0u, 0u};
-      if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
-      float bias[8];
-      dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
-      dense_epilogue<T>(g.epi, v, bias, i * g.J + j, g.J - j, g.vec_e, w);
-    }
+    if (sl == 0 && b0 + ob < nb) out(v, i, j);
+  }
+}
+#define DJ_PART (4 * 32 * 9)     // floats of `part` at SL = 8 (SL = 32 needs fewer)
+
+// threads an output block: shared while there are fewer than two workgroups a CU (100 slabs of 100 columns: 34 us with 1, 5 with 32)
+static int join_lanes(long long I, int J, int splits) {
+  const long long nb = I * ((J + 7) / 8);
+  return nb >= 512 * 256 || splits < 8 ? 1 : nb >= 512 * 32 || splits < 32 ? 8 : 32;
+}
+static unsigned join_blocks(long long I, int J, int lanes) {
+  return (unsigned)std::min<long long>((I * ((J + 7) / 8) + 256 / lanes - 1) / (256 / lanes), 1 << 16);
+}
+
+// the forward product's join, with the epilogue
+template <typename T, int SL>
+__global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
+  __shared__ float part[SL > 1 ? DJ_PART : 1];
+  dense_sum_slabs<SL>(g.slab, g.I, g.J, g.splits, blockIdx.x, gridDim.x, part, [&](float (&v)[8], long long i, int j) {
+    unsigned w[4] = {0u, 0u, 0u, 0u};
+    if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)i, (unsigned)j >> 3, w);
+    float bias[8];
+    dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
+    dense_epilogue<T>(g.epi, v, bias, i * g.J + j, g.J - j, g.vec_e, w);
+  });
+}
+
+// What a backward pass has left to add up, in one launch: the slabs of dx and of dw, and db's partial rows (32 columns and 8 row lanes a
+// block).  Jobs without blocks are skipped.
+struct DenseFinish {
+  struct Sum { const float* slab; void* out; long long I; int J, splits, lanes, vec; } sum[2];
+  const float* part; void* db; int chunks, n;
+  unsigned first[4];             // a job's first block; the end
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void dense_finish_kernel(DenseFinish f) {
+  __shared__ float part[DJ_PART];
+  const unsigned b = blockIdx.x;
+  if (b < f.first[2]) {
+    const int q = b < f.first[1] ? 0 : 1;
+    const DenseFinish::Sum& s = f.sum[q];
+    const unsigned block = b - f.first[q], blocks = f.first[q + 1] - f.first[q];
+    auto out = [&](float (&v)[8], long long i, int j) { store8<T>(static_cast<T*>(s.out) + i * s.J + j, v, s.J - j, s.vec); };
+    if (s.lanes == 1) dense_sum_slabs<1>(s.slab, s.I, s.J, s.splits, block, blocks, part, out);
+    else if (s.lanes == 8) dense_sum_slabs<8>(s.slab, s.I, s.J, s.splits, block, blocks, part, out);
+    else dense_sum_slabs<32>(s.slab, s.I, s.J, s.splits, block, blocks, part, out);
+    return;
+  }
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = (b - f.first[2]) * 32 + tx;
+  const float* p = f.part + min(col, f.n - 1);
+  float a = 0.f;
+#pragma unroll 8
+  for (int c = ty; c < f.chunks; c += 8) a += p[(long long)c * f.n];
+  part[ty * 33 + tx] = a;
+  __syncthreads();
+  if (ty == 0 && col < f.n) {
+    a = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) a += part[q * 33 + tx];
+    static_cast<T*>(f.db)[col] = (T)a;
   }
 }
 
@@ -319,25 +394,6 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
   }
 }
 
-// db = the partial rows' sum, 32 columns and 32 row lanes a block
-template <typename T>
-__global__ __launch_bounds__(1024) void dense_db_kernel(const float* part, int chunks, int n, void* db) {
-  __shared__ float s[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
-  const float* p = part + min(col, n - 1);
-  float a = 0.f;
-#pragma unroll 8
-  for (int c = ty; c < chunks; c += 32) a += p[(long long)c * n];
-  s[ty][tx] = a;
-  __syncthreads();
-  if (ty == 0 && col < n) {
-    a = 0.f;
-#pragma unroll
-    for (int q = 0; q < 32; ++q) a += s[q][tx];
-    static_cast<T*>(db)[col] = (T)a;
-  }
-}
-
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
@@ -369,13 +425,11 @@ static long long general_bytes(long long I, int J, long long K) {
 
 template <typename T>
 static int join_launch(const DenseGemm& g, hipStream_t st) {
-  const long long nb = g.I * ((g.J + 7) / 8);
-#define DJ_GO(SL) hipLaunchKernelGGL((dense_join_kernel<T, SL>), dim3((unsigned)std::min<long long>((nb + 256 / SL - 1) / (256 / SL), 1 << 16)), dim3(256), 0, st, g)
-  // shared output blocks while there are fewer than two workgroups a CU: 100 slabs of 100 columns 34 -> 5 us
-  if (nb >= 512 * 256 || g.splits < 8) DJ_GO(1);
-  else if (nb >= 512 * 32 || g.splits < 32) DJ_GO(8);
-  else DJ_GO(32);
-#undef DJ_GO
+  const int lanes = join_lanes(g.I, g.J, g.splits);
+  const dim3 grid(join_blocks(g.I, g.J, lanes));
+  if (lanes == 1) hipLaunchKernelGGL((dense_join_kernel<T, 1>), grid, dim3(256), 0, st, g);
+  else if (lanes == 8) hipLaunchKernelGGL((dense_join_kernel<T, 8>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((dense_join_kernel<T, 32>), grid, dim3(256), 0, st, g);
   VEEX_CHECK_LAUNCH();
   return 0;
 }
@@ -385,26 +439,35 @@ static int join_any(int dtype, const DenseGemm& g, hipStream_t st) {
   return join_launch<f16_t>(g, st);
 }
 
+static bool general_vec(int kind, const DenseGemm& g, int elem) {
+  return operand_vec(g.a, kind == kKindDw ? g.I : g.K, elem) && operand_vec(g.b, kind == kKindDx ? g.K : g.J, elem);
+}
+static long long general_tiles(const DenseGemm& g) { return (g.I + 63) / 64 * ((g.J + 63) / 64); }
+static int too_many_tiles() { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
+
 template <typename T>
-static int general_launch(int kind, DenseGemm g, void* ws, hipStream_t st) {
+static int general_launch(DenseGemm g, void* ws, hipStream_t st) {
   general_split(g.I, g.J, g.K, g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
-  const bool vec = operand_vec(g.a, kind == kKindDw ? g.I : g.K, sizeof(T)) && operand_vec(g.b, kind == kKindDx ? g.K : g.J, sizeof(T));
   g.vec_e = dense_epi_vec(g.epi, g.J);
-  const long long tiles = (g.I + 63) / 64 * ((g.J + 63) / 64);
-  if (tiles > 0x7FFFFFFFll) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
-  const dim3 grid((unsigned)tiles, (unsigned)g.splits);
-#define DG_GO(AK, BK)                                                                                                             \
-  if (g.splits > 1 && vec) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, true, true>), grid, dim3(256), 0, st, g);           \
-  else if (g.splits > 1) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, true, false>), grid, dim3(256), 0, st, g);            \
-  else if (vec) hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, false, true>), grid, dim3(256), 0, st, g);                     \
-  else hipLaunchKernelGGL((dense_general_kernel<T, AK, BK, false, false>), grid, dim3(256), 0, st, g);
-  if (kind == kKindFwd) { DG_GO(true, false) }
-  else if (kind == kKindDx) { DG_GO(true, true) }
-  else { DG_GO(false, false) }
-#undef DG_GO
+  if (general_tiles(g) > 0x7FFFFFFFll) return too_many_tiles();
+  const dim3 grid((unsigned)general_tiles(g), (unsigned)g.splits);
+  if (general_vec(kKindFwd, g, sizeof(T))) hipLaunchKernelGGL((dense_general_kernel<T, true>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((dense_general_kernel<T, false>), grid, dim3(256), 0, st, g);
   VEEX_CHECK_LAUNCH();
-  if (g.splits > 1) return join_launch<T>(g, st);
+  return g.splits > 1 ? join_launch<T>(g, st) : 0;
+}
+
+// g[0]: dx, g[1]: dw, as dense_product gives them with split and slab set; I = 0: not wanted
+template <typename T>
+static int general_grads_launch(const DenseGemm (&g)[2], hipStream_t st) {
+  const long long t0 = general_tiles(g[0]), t1 = general_tiles(g[1]), n0 = t0 * g[0].splits, n1 = t1 * g[1].splits;
+  if (n0 + n1 > 0x7FFFFFFFll) return too_many_tiles();
+  const bool vec = (n0 == 0 || general_vec(kKindDx, g[0], sizeof(T))) && (n1 == 0 || general_vec(kKindDw, g[1], sizeof(T)));
+  const dim3 grid((unsigned)(n0 + n1));
+  if (vec) hipLaunchKernelGGL((dense_general_grads_kernel<T, true>), grid, dim3(256), 0, st, g[0], g[1], (unsigned)t0, (unsigned)n0, (unsigned)t1);
+  else hipLaunchKernelGGL((dense_general_grads_kernel<T, false>), grid, dim3(256), 0, st, g[0], g[1], (unsigned)t0, (unsigned)n0, (unsigned)t1);
+  VEEX_CHECK_LAUNCH();
   return 0;
 }
 
@@ -539,27 +602,20 @@ static long long product_bytes(int kind, const VeexDense* d) {
   return t.splits > 1 ? align256(t.splits * g.I * slab_ld(g.J) * 4) : 0;
 }
 
-static int general_any(int kind, int dtype, const DenseGemm& g, void* ws, hipStream_t st) {
-  if (dtype == VEEX_T_F32) return general_launch<float>(kind, g, ws, st);
-  if (dtype == VEEX_T_BF16) return general_launch<bf16_t>(kind, g, ws, st);
-  return general_launch<f16_t>(kind, g, ws, st);
+static int general_any(int dtype, const DenseGemm& g, void* ws, hipStream_t st) {
+  if (dtype == VEEX_T_F32) return general_launch<float>(g, ws, st);
+  if (dtype == VEEX_T_BF16) return general_launch<bf16_t>(g, ws, st);
+  return general_launch<f16_t>(g, ws, st);
 }
 
-static int tiles_any(int kind, const VeexDense* d, const DenseGemm& g, const DtTensor& a, const DtTensor& b, void* ws, hipStream_t st) {
-  const TilePlan t = tile_plan(d, g.I, g.J, g.K);
-  DtGemm q = {};
+// a product on tiles, up to the launch; false: more tiles than one takes
+static bool tile_gemm(const TilePlan& t, const DenseGemm& g, const DtTensor& a, const DtTensor& b, void* slab, DtGemm& q) {
+  q = {};
   q.a = a; q.b = b; q.I = g.I; q.J = g.J; q.K = g.K; q.k_per_split = t.per; q.splits = t.splits;
   q.epi = g.epi;
-  q.slab = t.splits > 1 ? static_cast<float*>(ws) : nullptr;
+  q.slab = t.splits > 1 ? static_cast<float*>(slab) : nullptr;
   q.vec_e = dense_epi_vec(g.epi, g.J);
-  if ((double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits > 2147483647.0) { veex_set_error("dense: more tiles than a launch takes"); return VEEX_EINVAL; }
-  if (int rc = dense_tile_launch(d->dtype, kind != kKindDw, kind == kKindDx, t.tile, q, st)) return rc;
-  if (t.splits > 1) {
-    DenseGemm j = g;
-    j.slab = q.slab; j.splits = (int)t.splits; j.vec_e = q.vec_e;
-    return join_any(d->dtype, j, st);
-  }
-  return 0;
+  return (double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits < 1073741824.0;
 }
 
 // x, w or dy as the tiles load it: where it lies, or packed into *at, which moves on (the job is added to the list)
@@ -580,9 +636,13 @@ static long long fwd_bytes(const VeexDense* d) {
   return b;
 }
 
-// the backward workspace: [dz: made here, or dy packed] [partial column sums] [x, w packed] [one product's slabs, used by dx and
-// then by dw on the same stream]
-struct BwdLayout { bool dz_own, tiles; long long dz, part, packed, prod; int chunks; long long rows_per_chunk; long long total() const { return dz + part + packed + prod; } };
+// the backward workspace: [dz: made here, or dy packed] [partial column sums] [x, w packed] [dx's slabs] [dw's slabs]
+struct BwdLayout {
+  bool dz_own, tiles;
+  long long dz, part, packed, slab[2], rows_per_chunk;
+  int chunks;
+  long long total() const { return dz + part + packed + slab[0] + slab[1]; }
+};
 
 static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
   BwdLayout l = {};
@@ -600,7 +660,8 @@ static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
     l.dz = l.dz_own ? align256(d->rows * d->n * trunk_elem_bytes(d->dtype)) : 0;
   }
   l.part = align256((long long)l.chunks * d->n * 4);
-  l.prod = std::max(d->dx != nullptr ? product_bytes(kKindDx, d) : 0, d->dw != nullptr ? product_bytes(kKindDw, d) : 0);
+  l.slab[0] = d->dx != nullptr ? product_bytes(kKindDx, d) : 0;
+  l.slab[1] = d->dw != nullptr ? product_bytes(kKindDw, d) : 0;
   return l;
 }
 
@@ -628,7 +689,7 @@ int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
     if (d->dtype == VEEX_T_BF16) return few_launch<bf16_t>(g, d->workspace, st);
     return few_launch<f16_t>(g, d->workspace, st);
   }
-  if (!uses_tiles(d)) return general_any(kKindFwd, d->dtype, g, d->workspace, st);
+  if (!uses_tiles(d)) return general_any(d->dtype, g, d->workspace, st);
   char* at = static_cast<char*>(d->workspace);
   DtTensor x = {}, w = {};
   DtPack jobs[2];
@@ -636,7 +697,13 @@ int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
   tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, jobs, n);
   tile_operand(d, d->w, d->n, d->k, d->n, at, w, jobs, n);
   if (int rc = dense_pack_launch(d->dtype, jobs, n, st)) return rc;
-  return tiles_any(kKindFwd, d, g, x, w, at, st);
+  const TilePlan t = tile_plan(d, g.I, g.J, g.K);
+  DtGemm q;
+  if (!tile_gemm(t, g, x, w, at, q)) return too_many_tiles();
+  if (int rc = dense_tile_launch(d->dtype, true, false, t.tile, q, st)) return rc;
+  if (t.splits == 1) return 0;
+  g.slab = q.slab; g.splits = (int)t.splits; g.vec_e = q.vec_e;
+  return join_any(d->dtype, g, st);
 }
 
 long long veex_dense_bwd_workspace_bytes(const VeexDense* d) {
@@ -681,38 +748,68 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
 #undef DZ_GO
       VEEX_CHECK_LAUNCH();
     }
-    if (p.part != nullptr) {
-      const dim3 grid((d->n + 31) / 32);
-      if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_db_kernel<float>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
-      else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_db_kernel<bf16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
-      else hipLaunchKernelGGL((dense_db_kernel<f16_t>), grid, dim3(1024), 0, st, p.part, l.chunks, d->n, d->db);
-      VEEX_CHECK_LAUNCH();
+  }
+  float* const part = d->db != nullptr && l.chunks > 1 ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
+  if (!products && part == nullptr) return 0;
+
+  char* at = ws + l.dz + l.part;
+  float* const slabs[2] = {reinterpret_cast<float*>(at + l.packed), reinterpret_cast<float*>(at + l.packed + l.slab[0])};
+  DenseGemm g[2] = {};
+  if (d->dx != nullptr) g[0] = dense_product(kKindDx, d, dz);
+  if (d->dw != nullptr) g[1] = dense_product(kKindDw, d, dz);
+  for (int q = 0; q < 2; ++q) { g[q].splits = 1; g[q].slab = slabs[q]; g[q].vec_e = dense_epi_vec(g[q].epi, g[q].J); }
+  if (products && !l.tiles) {
+    for (DenseGemm& q : g)
+      if (q.I > 0) general_split(q.I, q.J, q.K, q.splits, q.k_per_split);
+    const int rc = d->dtype == VEEX_T_F32 ? general_grads_launch<float>(g, st) : d->dtype == VEEX_T_BF16 ? general_grads_launch<bf16_t>(g, st) : general_grads_launch<f16_t>(g, st);
+    if (rc != 0) return rc;
+  } else if (products) {
+    DtTensor x = {}, w = {};
+    DtPack jobs[3];
+    int n = 0;
+    if (!l.dz_own) {
+      char* p = ws;
+      tile_operand(d, d->dy, d->n, d->rows, d->n, p, dzt, jobs, n);
+    }
+    if (d->dx != nullptr) tile_operand(d, d->w, d->n, d->k, d->n, at, w, jobs, n);
+    if (d->dw != nullptr) tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, jobs, n);
+    if (int rc = dense_pack_launch(d->dtype, jobs, n, st)) return rc;
+    TilePlan t[2] = {};
+    DtGemm q[2] = {};
+    for (int k = 0; k < 2; ++k)
+      if (g[k].I > 0) {
+        t[k] = tile_plan(d, g[k].I, g[k].J, g[k].K);
+        if (!tile_gemm(t[k], g[k], k == 0 ? dzt : x, k == 0 ? w : dzt, slabs[k], q[k])) return too_many_tiles();
+        g[k].splits = (int)t[k].splits;
+      }
+    if (g[0].I > 0 && g[1].I > 0 && t[0].tile == 2 && t[1].tile == 2) {
+      if (int rc = dense_tile_grads_launch(d->dtype, q[0], q[1], st)) return rc;
+    } else {
+      for (int k = 0; k < 2; ++k)
+        if (g[k].I > 0)
+          if (int rc = dense_tile_launch(d->dtype, k == 0, k == 0, t[k].tile, q[k], st)) return rc;
     }
   }
-  if (!products) return 0;
-  char* at = ws + l.dz + l.part;
-  char* slabs = at + l.packed;
-  if (!l.tiles) {
-    if (d->dx != nullptr)
-      if (int rc = general_any(kKindDx, d->dtype, dense_product(kKindDx, d, dz), slabs, st)) return rc;
-    if (d->dw != nullptr)
-      if (int rc = general_any(kKindDw, d->dtype, dense_product(kKindDw, d, dz), slabs, st)) return rc;
-    return 0;
+
+  DenseFinish f = {};
+  for (int q = 0; q < 2; ++q) {
+    f.first[q + 1] = f.first[q];
+    if (g[q].splits == 1) continue;
+    const int lanes = join_lanes(g[q].I, g[q].J, g[q].splits);
+    f.sum[q] = {slabs[q], g[q].epi.y, g[q].I, g[q].J, g[q].splits, lanes, g[q].vec_e};
+    f.first[q + 1] += join_blocks(g[q].I, g[q].J, lanes);
   }
-  DtTensor x = {}, w = {};
-  DtPack jobs[3];
-  int n = 0;
-  if (!l.dz_own) {
-    char* p = ws;
-    tile_operand(d, d->dy, d->n, d->rows, d->n, p, dzt, jobs, n);
+  f.first[3] = f.first[2];
+  if (part != nullptr) {
+    f.part = part; f.db = d->db; f.chunks = l.chunks; f.n = d->n;
+    f.first[3] += (unsigned)((d->n + 31) / 32);
   }
-  if (d->dx != nullptr) tile_operand(d, d->w, d->n, d->k, d->n, at, w, jobs, n);
-  if (d->dw != nullptr) tile_operand(d, d->x, d->ldx, d->rows, d->k, at, x, jobs, n);
-  if (int rc = dense_pack_launch(d->dtype, jobs, n, st)) return rc;
-  if (d->dx != nullptr)
-    if (int rc = tiles_any(kKindDx, d, dense_product(kKindDx, d, nullptr), dzt, w, slabs, st)) return rc;
-  if (d->dw != nullptr)
-    if (int rc = tiles_any(kKindDw, d, dense_product(kKindDw, d, nullptr), x, dzt, slabs, st)) return rc;
+  if (f.first[3] == 0) return 0;
+  const dim3 grid(f.first[3]);
+  if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_finish_kernel<float>), grid, dim3(256), 0, st, f);
+  else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_finish_kernel<bf16_t>), grid, dim3(256), 0, st, f);
+  else hipLaunchKernelGGL((dense_finish_kernel<f16_t>), grid, dim3(256), 0, st, f);
+  VEEX_CHECK_LAUNCH();
   return 0;
 }
 

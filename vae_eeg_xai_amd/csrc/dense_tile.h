@@ -17,8 +17,10 @@ struct DtGemm {
   int vec_e;             // the epilogue's tensors move in 16-byte pieces of 8 columns
 };
 
-// akc / bkc: that operand's k index is its contiguous one.  tile: 256 or 128 (16-bit types)
+// akc / bkc: that operand's k index is its contiguous one.  tile: 0 256x256 (16-bit types), 1 256x128, 2 128x128
 int dense_tile_launch(int dtype, bool akc, bool bkc, int tile, const DtGemm& g, hipStream_t st);
+// dx and dw together, both in tiles of 128x128
+int dense_tile_grads_launch(int dtype, const DtGemm& dx, const DtGemm& dw, hipStream_t st);
 // up to three packings in one launch
 struct DtPack { const void* src; void* dst; long long ld, rows, plane_bytes; int cols; };
 int dense_pack_launch(int dtype, const DtPack* jobs, int n, hipStream_t st);

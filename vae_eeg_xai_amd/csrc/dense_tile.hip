@@ -151,19 +151,19 @@ __device__ __forceinline__ void dt_mend(const DtGemm& g, f32x16 (&acc)[MT][NT], 
     }
 }
 
-template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int ST, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
+// One tile (or one split of it): block number -> its part of C.  GRAD: a gradient, which has no epilogue.
+template <typename T, typename M, int PL, bool AKC, bool BKC, bool GRAD, int BM, int BN, int BK, int ST, int WM, int WN>
+__device__ __forceinline__ void dt_tile(const DtGemm& g, unsigned block, char* smem_raw) {
   constexpr int WAVES = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
   typedef DtOperand<BM, BK, AKC, PL, WAVES> OpA;
   typedef DtOperand<BN, BK, BKC, PL, WAVES> OpB;
   typedef typename DtVec<M>::x8 V8;
   constexpr int STAGE = PL * (OpA::BYTES + OpB::BYTES);
-  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   DT_LDS char* smem = (DT_LDS char*)smem_raw;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WN, wj = wave % WN;
   unsigned ti, tj, z;
-  dt_tile_of(blockIdx.x, g.tiles_i, g.tiles_j, g.splits, ti, tj, z);
+  dt_tile_of(block, g.tiles_i, g.tiles_j, g.splits, ti, tj, z);
   const long long i0 = (long long)ti * BM;
   const int j0 = tj * BN;
   const long long k_begin = z * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
@@ -254,10 +254,10 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
   DT_LDS char* strip = smem + wave * SM * 32 * CW * 4;
   const int l31 = lane & 31, lh = lane >> 5;
-  const unsigned long long base = drop_base(g.epi.drop);
+  const unsigned long long base = GRAD ? 0ull : drop_base(g.epi.drop);
   const int o = lane % OCT, j = j0 + wj * CW + 8 * o;
   float bias[8];
-  if (g.slab == nullptr) dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
+  if (!GRAD && g.slab == nullptr) dense_bias<T>(g.epi, bias, j, g.J, g.vec_e);
 #pragma unroll
   for (int m0 = 0; m0 < MT; m0 += SM) {
 #pragma unroll
@@ -282,13 +282,32 @@ __global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
         if (j + 4 < g.J) *reinterpret_cast<dt_f4*>(s + 4) = hi;
       } else {
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        unsigned w[4] = {0u, 0u, 0u, 0u};
-        if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
-        dense_epilogue<T>(g.epi, v, bias, at, g.J - j, g.vec_e, w);
+        if (GRAD) {
+          store8<T>(static_cast<T*>(g.epi.y) + at, v, g.J - j, g.vec_e);
+        } else {
+          unsigned w[4] = {0u, 0u, 0u, 0u};
+          if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, base + (unsigned long long)i, (unsigned)j >> 3, w);
+          dense_epilogue<T>(g.epi, v, bias, at, g.J - j, g.vec_e, w);
+        }
       }
     }
     dt_wave_sync();
   }
+}
+
+template <typename T, typename M, int PL, bool AKC, bool BKC, int BM, int BN, int BK, int ST, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void dense_tile_kernel(DtGemm g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  dt_tile<T, M, PL, AKC, BKC, !(AKC && !BKC), BM, BN, BK, ST, WM, WN>(g, blockIdx.x, smem);
+}
+
+// Both gradients in one launch: dx = dz w^T (k contiguous in both), dw = x^T dz (in neither).  A small layer's products leave most of
+// the chip idle one after the other.
+template <typename T, typename M, int PL, int BM, int BN, int BK, int ST, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void dense_tile_grads_kernel(DtGemm dx, DtGemm dw, unsigned dx_blocks) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  if (blockIdx.x < dx_blocks) dt_tile<T, M, PL, true, true, true, BM, BN, BK, ST, WM, WN>(dx, blockIdx.x, smem);
+  else dt_tile<T, M, PL, false, false, true, BM, BN, BK, ST, WM, WN>(dw, blockIdx.x - dx_blocks, smem);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -386,6 +405,27 @@ static int dt_pick(int tile, const DtGemm& g, hipStream_t st) {
     if (tile == 1) return dt_go<T, M, 1, AKC, BKC, 256, 128, 64, 3, 4, 2>(g, st);
     return dt_go<T, M, 1, AKC, BKC, 128, 128, 64, 4, 2, 4>(g, st);
   }
+}
+
+template <typename T, typename M, int PL, int BM, int BN, int BK, int ST, int WM, int WN>
+static int dt_grads_go(const DtGemm& dx_in, const DtGemm& dw_in, hipStream_t st) {
+  DtGemm g[2] = {dx_in, dw_in};
+  for (DtGemm& q : g) { q.tiles_i = (unsigned)((q.I + BM - 1) / BM); q.tiles_j = (unsigned)((q.J + BN - 1) / BN); }
+  constexpr int lds = ST * PL * (BM + BN) * BK * 2;
+  const void* fn = reinterpret_cast<const void*>(dense_tile_grads_kernel<T, M, PL, BM, BN, BK, ST, WM, WN>);
+  if (lds > 64 * 1024 && hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    veex_set_error("dense: cannot raise the dynamic LDS limit"); return VEEX_ELAUNCH;
+  }
+  const unsigned n0 = g[0].tiles_i * g[0].tiles_j * g[0].splits, n1 = g[1].tiles_i * g[1].tiles_j * g[1].splits;
+  hipLaunchKernelGGL((dense_tile_grads_kernel<T, M, PL, BM, BN, BK, ST, WM, WN>), dim3(n0 + n1), dim3(64 * WM * WN), lds, st, g[0], g[1], n0);
+  VEEX_CHECK_LAUNCH();
+  return 0;
+}
+
+int dense_tile_grads_launch(int dtype, const DtGemm& dx, const DtGemm& dw, hipStream_t st) {
+  if (dtype == VEEX_T_F32) return dt_grads_go<float, bf16_t, 3, 128, 128, 32, 3, 2, 4>(dx, dw, st);
+  if (dtype == VEEX_T_BF16) return dt_grads_go<bf16_t, bf16_t, 1, 128, 128, 64, 4, 2, 4>(dx, dw, st);
+  return dt_grads_go<f16_t, f16_t, 1, 128, 128, 64, 4, 2, 4>(dx, dw, st);
 }
 
 template <typename T, typename M>
