@@ -66,7 +66,7 @@ def _check_dense(ops, m, k, n, dt, act, residual, rate, train, first_row=0):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (2, 7, 3), (1, 6400, 100), (3, 28, 4096), (63, 33, 65), (64, 64, 64), (65, 100, 56),
-                                   (129, 32, 8), (130, 257, 333), (257, 1001, 127), (512, 96, 320), (520, 264, 264)])
+                                   (129, 32, 8), (70, 12, 20), (200, 36, 100), (130, 257, 333), (257, 1001, 127), (512, 96, 320), (520, 264, 264)])
 def test_dense_sizes(ops, m, k, n, dt):
     _check_dense(ops, m, k, n, dt, "gelu", True, 0.0, True)
 
@@ -79,7 +79,7 @@ def test_dense_large(ops, m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,k,n", [(1, 65536, 1), (1, 257, 1000), (2, 700, 264), (3, 1001, 77), (5, 640, 4096), (8, 4096, 136)])
+@pytest.mark.parametrize("m,k,n", [(1, 65536, 1), (1, 257, 1000), (1, 700, 100), (2, 700, 264), (3, 1001, 77), (5, 640, 4096), (8, 4096, 136)])
 def test_dense_few_rows(ops, m, k, n, dt):
     _check_dense(ops, m, k, n, dt, "gelu", True, 0.2, False)
     _check_dense(ops, m, k, n, dt, "sigmoid", False, 0.0, True)

@@ -33,11 +33,10 @@ struct DgOperand {
   __device__ __forceinline__ void load(float (&r)[8]) {
     if (vec) {
       constexpr int V = 16 / sizeof(T);
-      const bool in = rows_left > 0 && k_left > 0;
-      const T* q = in ? at : safe;
 #pragma unroll
       for (int c = 0; c < 8 / V; ++c) {
-        const Piece<T, V> x = piece_load<T, V>(q + c * V);
+        const bool in = (KC ? rows_left > 0 && k_left > c * V : rows_left > c * V && k_left > 0);
+        const Piece<T, V> x = piece_load<T, V>(in ? at + c * V : safe);
 #pragma unroll
         for (int e = 0; e < V; ++e) r[c * V + e] = in ? (float)x.v[e] : 0.f;
       }
@@ -399,10 +398,10 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
 // ---------------------------------------------------------------------------------------------------------------
 static const int kKindFwd = 0, kKindDx = 1, kKindDw = 2;     // which of A, B have k contiguous: A only; both; neither
 
-// a tensor's pieces of 8 elements along its contiguous index (length `len`) are whole and 16-byte aligned
+// a tensor's 16-byte pieces along its contiguous index (length `len`) are whole and aligned
 static bool operand_vec(const DenseOperand& o, long long len, int elem) {
   const long long other = o.k_stride == 1 ? o.row_stride : o.k_stride;
-  return trunk_aligned16(o.p) && other * elem % 16 == 0 && len % 8 == 0;
+  return trunk_aligned16(o.p) && other * elem % 16 == 0 && len * elem % 16 == 0;
 }
 
 // The reduction is split where the tiles are fewer than two a CU: up to 512 blocks, at least 64 k each (1001x1003x1005 fp32 52 us
@@ -449,7 +448,7 @@ template <typename T>
 static int general_launch(DenseGemm g, void* ws, hipStream_t st) {
   general_split(g.I, g.J, g.K, g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
-  g.vec_e = dense_epi_vec(g.epi, g.J);
+  g.vec_e = dense_epi_vec(g.epi, g.J, sizeof(T));
   if (general_tiles(g) > 0x7FFFFFFFll) return too_many_tiles();
   const dim3 grid((unsigned)general_tiles(g), (unsigned)g.splits);
   if (general_vec(kKindFwd, g, sizeof(T))) hipLaunchKernelGGL((dense_general_kernel<T, true>), grid, dim3(256), 0, st, g);
@@ -500,7 +499,7 @@ static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
   const bool vec = few_vec<T>(g);
   few_split(g, vec, sizeof(T), g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
-  g.vec_e = dense_epi_vec(g.epi, g.J);
+  g.vec_e = dense_epi_vec(g.epi, g.J, sizeof(T));
   const dim3 grid((unsigned)(vec ? ((long long)g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64), (unsigned)g.splits);
 #define DF_GO(R)                                                                                              \
   if (vec) hipLaunchKernelGGL((dense_few_rows_kernel<T, R, true>), grid, dim3(256), 0, st, g);                 \
@@ -609,12 +608,12 @@ static int general_any(int dtype, const DenseGemm& g, void* ws, hipStream_t st) 
 }
 
 // a product on tiles, up to the launch; false: more tiles than one takes
-static bool tile_gemm(const TilePlan& t, const DenseGemm& g, const DtTensor& a, const DtTensor& b, void* slab, DtGemm& q) {
+static bool tile_gemm(int elem, const TilePlan& t, const DenseGemm& g, const DtTensor& a, const DtTensor& b, void* slab, DtGemm& q) {
   q = {};
   q.a = a; q.b = b; q.I = g.I; q.J = g.J; q.K = g.K; q.k_per_split = t.per; q.splits = t.splits;
   q.epi = g.epi;
   q.slab = t.splits > 1 ? static_cast<float*>(slab) : nullptr;
-  q.vec_e = dense_epi_vec(g.epi, g.J);
+  q.vec_e = dense_epi_vec(g.epi, g.J, elem);
   return (double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits < 1073741824.0;
 }
 
@@ -699,7 +698,7 @@ int veex_dense_fwd(const VeexDense* d, hipStream_t st) {
   if (int rc = dense_pack_launch(d->dtype, jobs, n, st)) return rc;
   const TilePlan t = tile_plan(d, g.I, g.J, g.K);
   DtGemm q;
-  if (!tile_gemm(t, g, x, w, at, q)) return too_many_tiles();
+  if (!tile_gemm(trunk_elem_bytes(d->dtype), t, g, x, w, at, q)) return too_many_tiles();
   if (int rc = dense_tile_launch(d->dtype, true, false, t.tile, q, st)) return rc;
   if (t.splits == 1) return 0;
   g.slab = q.slab; g.splits = (int)t.splits; g.vec_e = q.vec_e;
@@ -736,7 +735,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
     p.db = l.chunks == 1 ? d->db : nullptr;
     p.part = d->db != nullptr && l.chunks > 1 ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
     p.rows = d->rows; p.rows_per_chunk = l.rows_per_chunk; p.n = d->n; p.act = d->activation; p.drop = drop;
-    p.vec = d->n % 8 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
+    p.vec = (long long)d->n * trunk_elem_bytes(d->dtype) % 16 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
     if (p.dz != nullptr || d->db != nullptr) {
       const dim3 grid((d->n + 255) / 256, l.chunks);
 #define DZ_GO(T)                                                                                              \
@@ -757,7 +756,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
   DenseGemm g[2] = {};
   if (d->dx != nullptr) g[0] = dense_product(kKindDx, d, dz);
   if (d->dw != nullptr) g[1] = dense_product(kKindDw, d, dz);
-  for (int q = 0; q < 2; ++q) { g[q].splits = 1; g[q].slab = slabs[q]; g[q].vec_e = dense_epi_vec(g[q].epi, g[q].J); }
+  for (int q = 0; q < 2; ++q) { g[q].splits = 1; g[q].slab = slabs[q]; g[q].vec_e = dense_epi_vec(g[q].epi, g[q].J, trunk_elem_bytes(d->dtype)); }
   if (products && !l.tiles) {
     for (DenseGemm& q : g)
       if (q.I > 0) general_split(q.I, q.J, q.K, q.splits, q.k_per_split);
@@ -779,7 +778,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
     for (int k = 0; k < 2; ++k)
       if (g[k].I > 0) {
         t[k] = tile_plan(d, g[k].I, g[k].J, g[k].K);
-        if (!tile_gemm(t[k], g[k], k == 0 ? dzt : x, k == 0 ? w : dzt, slabs[k], q[k])) return too_many_tiles();
+        if (!tile_gemm(trunk_elem_bytes(d->dtype), t[k], g[k], k == 0 ? dzt : x, k == 0 ? w : dzt, slabs[k], q[k])) return too_many_tiles();
         g[k].splits = (int)t[k].splits;
       }
     if (g[0].I > 0 && g[1].I > 0 && t[0].tile == 2 && t[1].tile == 2) {

@@ -96,7 +96,8 @@ __device__ __forceinline__ void dense_act_grad(float (&d)[W], const float (&s)[W
   }
 }
 
-// Eight elements at p (n of them inside the row), as they lie; vec: as 16-byte pieces.  Kept apart from their conversion, so that
+// Eight elements at p (n of them inside the row), as they lie; vec: as 16-byte pieces (a row then ends with a piece: of fp32, which has
+// two, the second may be missing and reads as zeros).  Kept apart from their conversion, so that
 // several loads are on their way before the first is waited for.
 template <typename T> struct Raw8 { T v[8]; };
 template <typename T>
@@ -105,9 +106,10 @@ __device__ __forceinline__ void load_raw(Raw8<T>& r, const T* p, int n, bool vec
   if (vec) {
 #pragma unroll
     for (int q = 0; q < 8 / V; ++q) {
-      const Piece<T, V> b = piece_load<T, V>(p + q * V);
+      const bool in = q * V < n;
+      const Piece<T, V> b = piece_load<T, V>(in ? p + q * V : p);
 #pragma unroll
-      for (int e = 0; e < V; ++e) r.v[q * V + e] = b.v[e];
+      for (int e = 0; e < V; ++e) r.v[q * V + e] = in ? b.v[e] : (T)0.f;
     }
   } else {
 #pragma unroll
@@ -130,7 +132,7 @@ __device__ __forceinline__ void store8(T* p, const float (&s)[8], int n, bool ve
       Piece<T, V> b;
 #pragma unroll
       for (int e = 0; e < V; ++e) b.v[e] = (T)s[q * V + e];
-      piece_store<T, V>(p + q * V, b);
+      if (q * V < n) piece_store<T, V>(p + q * V, b);
     }
   } else {
 #pragma unroll
@@ -176,9 +178,9 @@ __device__ __forceinline__ void dense_epilogue(const DenseEpi& ep, float (&v)[8]
   store8<T>(static_cast<T*>(ep.y) + at, v, n, vec);
 }
 
-// every tensor of the epilogue can be moved in 16-byte pieces of blocks of 8 columns
-inline bool dense_epi_vec(const DenseEpi& ep, int J) {
-  if (J % 8 != 0) return false;
+// every tensor of the epilogue can be moved in 16-byte pieces
+inline bool dense_epi_vec(const DenseEpi& ep, int J, int elem) {
+  if ((long long)J * elem % 16 != 0) return false;
   for (const void* q : {ep.bias, ep.res, (const void*)ep.y, (const void*)ep.pre})
     if (!trunk_aligned16(q)) return false;
   return true;
@@ -199,7 +201,7 @@ struct DenseGemm {
   float* slab;           // [splits][I][slab_ld(J)] when splits > 1
   int splits;
   long long k_per_split;
-  int vec_e;             // the epilogue's tensors move in 16-byte pieces of 8 columns
+  int vec_e;             // the epilogue's tensors move in 16-byte pieces
 };
 
 #endif

@@ -14,7 +14,7 @@ struct DtGemm {
   unsigned splits, tiles_i, tiles_j;
   DenseEpi epi;
   float* slab;           // null: the epilogue runs here
-  int vec_e;             // the epilogue's tensors move in 16-byte pieces of 8 columns
+  int vec_e;             // the epilogue's tensors move in 16-byte pieces
 };
 
 // akc / bkc: that operand's k index is its contiguous one.  tile: 0 256x256 (16-bit types), 1 256x128, 2 128x128
