@@ -8,9 +8,10 @@
 //   dgate = sum over the group of D scale n;  dscale = sum D gate n;  dpost_w = sum dn xhat;  dpost_b = sum dn;
 //   dpre_w = sum du rhat;  dpre_b = sum du          (RMSNorm: without the means of t and e)
 //
-// Bound: HBM.  A row lives in the registers of 1 to 16 waves (8 or 16 elements a lane), so the forward pass reads x, h and
+// Bound: HBM.  A row lives in the registers of 8 lanes to 16 waves (8 or 16 elements a lane), so the forward pass reads x, h and
 // gate once and writes x_out and u once; the backward pass recomputes x_out from x and h in fp32 instead of reading the
-// rounded one (the same bytes, and the gradient is that of the unrounded chain).  All statistics and sums are fp32; the
+// rounded one (the same bytes, and the gradient is that of the unrounded chain).  8192x4096 bf16: forward 50 us (5.4 TB/s),
+// backward 91 us with its column sums (4.4 TB/s); fp32 99 and 131 us (5.4 and 6.2 TB/s; a copy of 1 GB runs at 4.9).  All statistics and sums are fp32; the
 // variance is the mean of squared deviations (two passes over registers), not a difference of moments.
 // Column sums: each block adds up its own run of rows in registers, writes one partial row per sum, and a second kernel adds
 // the partial rows in a fixed order: no atomics, the same bits every time.
@@ -31,37 +32,44 @@ struct RNormParams {
   long long groups, rows_per_group, rows_per_chunk, chunks_per_group;
 };
 
-// Sum over a wave's 64 lanes, in every lane: neighbours, pairs, quads and eights through DPP, the four rows of 16 through lane swaps.
+// Sum over groups of G = 8 to 64 neighbouring lanes, in every lane: neighbours, pairs, quads and eights through DPP, rows of 16 through
+// lane swaps.
 // (A shuffle goes through LDS, some hundred cycles a step; six steps twice or more a row were a third of these kernels' time.)
-__device__ __forceinline__ float rn_wave_sum(float x) {
+template <int G> __device__ __forceinline__ float rn_lanes_sum(float x) {
 #define RN_DPP(CTRL) x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xF, 0xF, true))
   RN_DPP(0xB1);       // quad_perm [1,0,3,2]
   RN_DPP(0x4E);       // quad_perm [2,3,0,1]
   RN_DPP(0x141);      // row_half_mirror
-  RN_DPP(0x140);      // row_mirror
+  if (G >= 16) RN_DPP(0x140);      // row_mirror
 #undef RN_DPP
-  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(h[0]) + __uint_as_float(h[1]);
-  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+  if (G >= 32) {
+    const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  }
+  if (G >= 64) {
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+  }
+  return x;
 }
 
-// sum of a (and b) over the 64 * WPR lanes of a row; red: two buffers of 2 * 16 floats, taken in turn, so that one barrier a
-// sum is enough (a wave can write a buffer again only after the barrier of the sum in between)
-template <int WPR>
+// sum of a and b over the LANES lanes of a row; red: two buffers of 2 * 16 floats, taken in turn, so that one barrier a sum is enough
+// (a wave can write a buffer again only after the barrier of the sum in between)
+template <int LANES>
 struct RowSum {
-  float* red; int rg, wave, turn;
-  __device__ __forceinline__ RowSum(float* r, int rg_, int wave_) : red(r), rg(rg_), wave(wave_), turn(0) {}
+  static constexpr int WPR = LANES > 64 ? LANES / 64 : 1;        // waves a row
+  float* red; int first, wave, turn;                             // first: the row's first wave
+  __device__ __forceinline__ RowSum(float* r) : red(r), first(threadIdx.x / LANES * WPR), wave(threadIdx.x >> 6), turn(0) {}
   __device__ __forceinline__ float2 operator()(float a, float b) {
-    a = rn_wave_sum(a); b = rn_wave_sum(b);
+    a = rn_lanes_sum<LANES < 64 ? LANES : 64>(a); b = rn_lanes_sum<LANES < 64 ? LANES : 64>(b);
     if (WPR == 1) return make_float2(a, b);
     float* r = red + turn * 32;
     turn ^= 1;
-    if ((threadIdx.x & 63) == 0) { r[(rg * WPR + wave) * 2] = a; r[(rg * WPR + wave) * 2 + 1] = b; }
+    if ((threadIdx.x & 63) == 0) { r[wave * 2] = a; r[wave * 2 + 1] = b; }
     __syncthreads();
     a = 0.f; b = 0.f;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) { a += r[(rg * WPR + w) * 2]; b += r[(rg * WPR + w) * 2 + 1]; }
+    for (int w = 0; w < WPR; ++w) { a += r[(first + w) * 2]; b += r[(first + w) * 2 + 1]; }
     return make_float2(a, b);
   }
 };
@@ -74,10 +82,15 @@ __device__ __forceinline__ void row_load(RowRaw<T, V, C>& r, const void* base, l
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int col = (c * LANES + lane) * V;
-    if (col < cols) r.p[c] = piece_load<T, V>(p + col);
-    else
+    if (V == 1) {      // (whole pieces: a load of some piece and a choice; a branch around the load put fp32 rows into scratch memory,
+                       // 16384x1024 65 us for 42)
+      if (col < cols) r.p[c] = piece_load<T, V>(p + col);
+      else r.p[c].v[0] = (T)0.f;
+    } else {
+      const Piece<T, V> q = piece_load<T, V>(p + (col < cols ? col : 0));
 #pragma unroll
-      for (int e = 0; e < V; ++e) r.p[c].v[e] = (T)0.f;
+      for (int e = 0; e < V; ++e) r.p[c].v[e] = col < cols ? q.v[e] : (T)0.f;
+    }
   }
 }
 template <typename T, int V, int C>
@@ -114,22 +127,29 @@ __device__ __forceinline__ void row_param(RowRaw<T, V, C>& r, const void* p, flo
   else row_fill<T, V, C, LANES>(r, otherwise);
 }
 
-// WPR waves a row, EPL elements a lane; VEC: rows are whole 16-byte pieces
-template <typename T, int WPR, int EPL, bool VEC>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNormParams p) {
-  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V, LANES = 64 * WPR;
-  constexpr int RG = WPR > 4 ? 1 : 4 / WPR;
+// LANES lanes a row (8 of a wave, 32 rows a block, up to 16 waves), EPL elements a lane; VEC: rows are whole 16-byte pieces
+template <typename T, int LANES, int EPL, bool VEC>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_fwd_kernel(RNormParams p) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V;
+  constexpr int RG = LANES > 256 ? 1 : 256 / LANES;        // rows a block works on
   __shared__ float red[64];
   const int lane = threadIdx.x % LANES, rg = threadIdx.x / LANES;
-  RowSum<WPR> row_sum(red, rg, (threadIdx.x >> 6) % WPR);
+  RowSum<LANES> row_sum(red);
   const float inv = 1.f / (float)p.cols;
 
+  // (16 elements a lane of 16 waves, 128 registers each: the next row is not fetched ahead, and the vectors are read again each row)
+  constexpr bool AHEAD = EPL == 8;
   RowRaw<T, V, C> scale, ow, ob, pw, pb;
-  row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
-  row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
-  row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
-  row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols);
-  row_param<T, V, C, LANES>(pb, p.pre_b, 0.f, lane, p.cols);
+  auto vectors_post = [&] {
+    row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
+    row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
+    row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
+  };
+  auto vectors_pre = [&] {
+    row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols);
+    row_param<T, V, C, LANES>(pb, p.pre_b, 0.f, lane, p.cols);
+  };
+  if (AHEAD) { vectors_post(); vectors_pre(); }
 
   bool in[C];
 #pragma unroll
@@ -162,16 +182,18 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNo
   };
   const long long step = (long long)gridDim.x * RG;
   In in_now, in_next;
-  fetch(in_now, (long long)blockIdx.x * RG + rg);
+  if (AHEAD) fetch(in_now, (long long)blockIdx.x * RG + rg);
   for (long long r0 = (long long)blockIdx.x * RG; r0 < p.rows; r0 += step) {
     const bool live = r0 + rg < p.rows;
     const long long row = live ? r0 + rg : p.rows - 1, at = row * p.cols;
-    if (r0 + step < p.rows) fetch(in_next, r0 + step + rg);
+    if (!AHEAD) fetch(in_now, row);
+    else if (r0 + step < p.rows) fetch(in_next, r0 + step + rg);
     float v[EPL], mean1 = 0.f, rstd1 = 0.f, mean2, rstd2;
     if (p.h != nullptr) {
 #pragma unroll
       for (int e = 0; e < EPL; ++e) v[e] = (float)in_now.h.p[e / V].v[e % V];
       moments(v, mean1, rstd1);
+      if (!AHEAD) vectors_post();
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         const int c = e / V, k = e % V;
@@ -184,33 +206,40 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_fwd_kernel(RNo
       for (int e = 0; e < EPL; ++e) v[e] = (float)in_now.x.p[e / V].v[e % V];
     }
     moments(v, mean2, rstd2);
+    if (!AHEAD) vectors_pre();
 #pragma unroll
     for (int e = 0; e < EPL; ++e) v[e] = fmaf((v[e] - mean2) * rstd2, (float)pw.p[e / V].v[e % V], (float)pb.p[e / V].v[e % V]);
     if (live) {
       row_store<T, V, C, LANES>(p.u, at, v, lane, p.cols);
       if (p.stats != nullptr && lane == 0) *reinterpret_cast<float4*>(p.stats + row * 4) = make_float4(mean1, rstd1, mean2, rstd2);
     }
-    row_copy(in_now.x, in_next.x); row_copy(in_now.h, in_next.h); row_copy(in_now.g, in_next.g);
+    if (AHEAD) { row_copy(in_now.x, in_next.x); row_copy(in_now.h, in_next.h); row_copy(in_now.g, in_next.g); }
   }
 }
 
 // One block a chunk: rows_per_chunk consecutive rows of one gate group.  BIAS: a bias learns too (two more sums a column).
-template <typename T, int WPR, int EPL, bool VEC, bool BIAS>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNormParams p) {
-  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V, LANES = 64 * WPR;
-  constexpr int RG = WPR > 4 ? 1 : 4 / WPR;
+template <typename T, int LANES, int EPL, bool VEC, bool BIAS>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RNormParams p) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V;
+  constexpr int RG = LANES > 256 ? 1 : 256 / LANES;        // rows a block works on
   __shared__ float red[64];
   __shared__ float comb[RG > 1 ? RG * LANES * EPL : 1];
   const int lane = threadIdx.x % LANES, rg = threadIdx.x / LANES;
-  RowSum<WPR> row_sum(red, rg, (threadIdx.x >> 6) % WPR);
+  RowSum<LANES> row_sum(red);
   const float inv = 1.f / (float)p.cols;
   const bool post = p.h != nullptr;
 
+  // A block of 16 waves has 128 registers a lane: there the vectors are read again for each row (from the L2), the next row is not
+  // fetched ahead and the column sums stay in LDS, or registers would be spilled (8192 columns, 4096 rows, bf16: 411 us, so 101).
+  constexpr bool AHEAD = LANES < 1024;
   RowRaw<T, V, C> scale, ow, ob, pw, gr;
-  row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
-  row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
-  row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
-  row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols);
+  auto vectors_post = [&] {
+    row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
+    row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
+    row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
+  };
+  auto vectors_pre = [&] { row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols); };
+  if (AHEAD) { vectors_post(); vectors_pre(); }
   bool in[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) in[c] = (c * LANES + lane) * V < p.cols;
@@ -219,15 +248,28 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
   const long long first = group * p.rows_per_group + piece * p.rows_per_chunk;
   const long long last = min(first + p.rows_per_chunk, (group + 1) * p.rows_per_group);     // one past
   const bool full_gate = p.gate != nullptr && p.rows_per_group == 1;
-  if (p.gate != nullptr) row_load<T, V, C, LANES>(gr, p.gate, group * p.cols, lane, p.cols);
-  else row_fill<T, V, C, LANES>(gr, 1.f);
+  auto gate_row = [&](RowRaw<T, V, C>& g) {
+    if (p.gate != nullptr) row_load<T, V, C, LANES>(g, p.gate, group * p.cols, lane, p.cols);
+    else row_fill<T, V, C, LANES>(g, 1.f);
+  };
+  if (AHEAD) gate_row(gr);
 
-  float a_gate[EPL], a_ow[EPL], a_pw[EPL], a_ob[BIAS ? EPL : 1], a_pb[BIAS ? EPL : 1];
+  // the column sums of the block's rows; a lane's own, the first HELD of them in LDS
+  enum { GATE, POST_W, PRE_W, POST_B, PRE_B };
+  constexpr int SUMS = BIAS ? 5 : 3, HELD = AHEAD ? 0 : EPL > 8 ? 2 : BIAS ? 4 : 3;
+  __shared__ float held[HELD > 0 ? HELD * EPL * LANES : 1];
+  float acc[SUMS][EPL];
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    a_gate[e] = a_ow[e] = a_pw[e] = 0.f;
-    if (BIAS) a_ob[e] = a_pb[e] = 0.f;
-  }
+  for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      if (k < HELD) held[(k * EPL + e) * LANES + lane] = 0.f;
+      else acc[k][e] = 0.f;
+    }
+  auto add = [&](int k, int e, float x, float y) {
+    float& a = k < HELD ? held[(k * EPL + e) * LANES + lane] : acc[k][e];
+    a = fmaf(x, y, a);
+  };
 
   // (a gate per element: the chunks of one row each would leave as many partial rows as there are rows, so there the host
   // hands out chunks of several "groups" and the gate is read with its row)
@@ -244,15 +286,17 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
     if (p.du != nullptr) row_load<T, V, C, LANES>(r.du, p.du, at, lane, p.cols);
     else row_fill<T, V, C, LANES>(r.du, 0.f);
     if (full_gate) row_load<T, V, C, LANES>(r.g, p.gate, at, lane, p.cols);
-    else row_copy(r.g, gr);
+    else if (AHEAD) row_copy(r.g, gr);
+    else gate_row(r.g);
     r.st = *reinterpret_cast<const float4*>(p.stats + row * 4);
   };
   In in_now, in_next;
-  if (c_first < c_last) fetch(in_now, c_first + rg);
+  if (AHEAD && c_first < c_last) fetch(in_now, c_first + rg);
   for (long long r0 = c_first; r0 < c_last; r0 += RG) {
     const bool live = r0 + rg < c_last;
     const long long row = live ? r0 + rg : c_last - 1, at = row * p.cols;
-    if (r0 + RG < c_last) fetch(in_next, r0 + RG + rg);          // (as in the forward kernel)
+    if (!AHEAD) { fetch(in_now, r0 + rg); vectors_post(); vectors_pre(); }
+    else if (r0 + RG < c_last) fetch(in_next, r0 + RG + rg);          // (as in the forward kernel)
     const RowRaw<T, V, C>&xr = in_now.x, &hr = in_now.h, &dor = in_now.dout, &dur = in_now.du, &gr = in_now.g;
     const float4 st = in_now.st;
     float xh[EPL], rh[EPL], d[EPL];
@@ -269,8 +313,8 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
       rh[e] = in[c] ? (out - st.z) * st.w : 0.f;
       const float du = (float)dur.p[c].v[k];
       if (live) {
-        a_pw[e] = fmaf(du, rh[e], a_pw[e]);
-        if (BIAS) a_pb[e] += du;
+        add(PRE_W, e, du, rh[e]);
+        if (BIAS) add(PRE_B, e, du, 1.f);
       }
       d[e] = du * (float)pw.p[c].v[k];
       s1 += d[e]; s2 = fmaf(d[e], rh[e], s2);
@@ -285,6 +329,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
     }
     if (live && p.dx != nullptr) row_store<T, V, C, LANES>(p.dx, at, d, lane, p.cols);
     if (post) {
+      if (!AHEAD) vectors_post();
       if (live && full_gate && p.dgate != nullptr) {
         float dg[EPL];
 #pragma unroll
@@ -299,9 +344,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
         if (!in[c]) d[e] = 0.f;
         const float dn = d[e] * (s * g);
         if (live) {
-          a_gate[e] = fmaf(d[e] * n, full_gate ? g : 1.f, a_gate[e]);
-          a_ow[e] = fmaf(dn, xh[e], a_ow[e]);
-          if (BIAS) a_ob[e] += dn;
+          add(GATE, e, d[e] * n, full_gate ? g : 1.f);
+          add(POST_W, e, dn, xh[e]);
+          if (BIAS) add(POST_B, e, dn, 1.f);
         }
         d[e] = dn * (float)ow.p[c].v[k];
         s1 += d[e]; s2 = fmaf(d[e], in[c] ? xh[e] : 0.f, s2);
@@ -312,13 +357,18 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
       for (int e = 0; e < EPL; ++e) d[e] = st.y * (d[e] - fmaf(xh[e], m.y, m.x));
       if (live && p.dh != nullptr) row_store<T, V, C, LANES>(p.dh, at, d, lane, p.cols);
     }
-    row_copy(in_now.x, in_next.x); row_copy(in_now.h, in_next.h); row_copy(in_now.dout, in_next.dout);
-    row_copy(in_now.du, in_next.du); row_copy(in_now.g, in_next.g);
-    in_now.st = in_next.st;
+    if (AHEAD) {
+      row_copy(in_now.x, in_next.x); row_copy(in_now.h, in_next.h); row_copy(in_now.dout, in_next.dout);
+      row_copy(in_now.du, in_next.du); row_copy(in_now.g, in_next.g);
+      in_now.st = in_next.st;
+    }
   }
 
   float* part = p.part + (long long)blockIdx.x * 5 * p.cols;
-  auto flush = [&](float (&a)[EPL], int k) {
+  auto flush = [&](int sum, int k) {
+    float a[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) a[e] = sum < HELD ? held[(sum * EPL + e) * LANES + lane] : acc[sum][e];
     if (RG > 1) {                      // the block's row groups, added in order
       __syncthreads();
 #pragma unroll
@@ -339,11 +389,11 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void rnorm_bwd_kernel(RNo
         for (int e = 0; e < V; ++e) part[(long long)k * p.cols + col + e] = a[c * V + e];
     }
   };
-  if (p.dscale != nullptr || (p.dgate != nullptr && !full_gate)) flush(a_gate, 0);
-  if (p.dpost_w != nullptr) flush(a_ow, 1);
-  if constexpr (BIAS) if (p.dpost_b != nullptr) flush(a_ob, 2);
-  if (p.dpre_w != nullptr) flush(a_pw, 3);
-  if constexpr (BIAS) if (p.dpre_b != nullptr) flush(a_pb, 4);
+  if (p.dscale != nullptr || (p.dgate != nullptr && !full_gate)) flush(GATE, 0);
+  if (p.dpost_w != nullptr) flush(POST_W, 1);
+  if constexpr (BIAS) if (p.dpost_b != nullptr) flush(POST_B, 2);
+  if (p.dpre_w != nullptr) flush(PRE_W, 3);
+  if constexpr (BIAS) if (p.dpre_b != nullptr) flush(PRE_B, 4);
 }
 
 // Column sums of the partial rows, 64 columns and 16 row lanes a block.  blockIdx.y 0: dscale (each chunk's sum times its group's
@@ -387,16 +437,16 @@ __global__ __launch_bounds__(1024) void rnorm_sums_kernel(RNormParams p, long lo
   if (ty == 0 && col < p.cols) out[col] = (T)a;
 }
 
-// waves a row / elements a lane: the fewest lanes that hold the row at 8 elements each, up to 16 waves; wider rows take 16
-#define RNORM_BY_WIDTH(KERNEL, GRID, T, ...)                                                                      \
-  do {                                                                                                                       \
-    if (p.cols <= 512) { GRID(4); hipLaunchKernelGGL((KERNEL<T, 1, 8, __VA_ARGS__>), dim3(grid), dim3(256), 0, st, p); }              \
-    else if (p.cols <= 1024) { GRID(2); hipLaunchKernelGGL((KERNEL<T, 2, 8, __VA_ARGS__>), dim3(grid), dim3(256), 0, st, p); }        \
-    else if (p.cols <= 2048) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 4, 8, __VA_ARGS__>), dim3(grid), dim3(256), 0, st, p); }        \
-    else if (p.cols <= 4096) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 8, 8, __VA_ARGS__>), dim3(grid), dim3(512), 0, st, p); }        \
-    else if (p.cols <= 8192) { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 8, __VA_ARGS__>), dim3(grid), dim3(1024), 0, st, p); }      \
-    else { GRID(1); hipLaunchKernelGGL((KERNEL<T, 16, 16, __VA_ARGS__>), dim3(grid), dim3(1024), 0, st, p); }                         \
+// lanes a row: the fewest that hold it at 8 elements each, from 8 to 16 waves (65536 rows of 64 columns, fp32: 64 lanes a row 34 us
+// forward and 63 backward, 8 lanes 12 and 37; of 128: 35 and 63, 16 lanes 21 and 38); wider rows take 16 elements a lane, and some
+// spilled registers (16384 columns, 2048 rows, bf16: 110 and 344 us, 2.4 and 1.2 TB/s).  GO(lanes, elements)
+#define RNORM_BY_WIDTH(GO)                                                                              \
+  do {                                                                                                  \
+    if (p.cols <= 64) { GO(8, 8); } else if (p.cols <= 128) { GO(16, 8); } else if (p.cols <= 256) { GO(32, 8); }     \
+    else if (p.cols <= 512) { GO(64, 8); } else if (p.cols <= 1024) { GO(128, 8); } else if (p.cols <= 2048) { GO(256, 8); } \
+    else if (p.cols <= 4096) { GO(512, 8); } else if (p.cols <= 8192) { GO(1024, 8); } else { GO(1024, 16); }           \
   } while (0)
+static int rnorm_rows_per_block(int cols) { return cols <= 64 ? 32 : cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 512 ? 4 : cols <= 1024 ? 2 : 1; }
 
 static bool rnorm_vec(const RNormParams& p, int dtype) {
   if (p.cols % (16 / trunk_elem_bytes(dtype)) != 0) return false;
@@ -408,24 +458,27 @@ static bool rnorm_vec(const RNormParams& p, int dtype) {
 
 template <typename T>
 static int rnorm_fwd_launch(const RNormParams& p, bool vec, hipStream_t st) {
-  unsigned grid = 0;
   // (as many blocks as the chip holds at a time: 8192x4096 64 us with 4096, 59 with 1024)
-#define RNORM_FWD_GRID(RG) grid = (unsigned)std::min<long long>((p.rows + (RG) - 1) / (RG), 1024)
-  if (vec) RNORM_BY_WIDTH(rnorm_fwd_kernel, RNORM_FWD_GRID, T, true);
-  else RNORM_BY_WIDTH(rnorm_fwd_kernel, RNORM_FWD_GRID, T, false);
+  const int rg = rnorm_rows_per_block(p.cols);
+  const unsigned grid = (unsigned)std::min<long long>((p.rows + rg - 1) / rg, 1024);
+#define RNORM_FWD_GO(L, E)                                                                                                        \
+  if (vec) hipLaunchKernelGGL((rnorm_fwd_kernel<T, L, E, true>), dim3(grid), dim3((L) > 256 ? (L) : 256), 0, st, p);               \
+  else hipLaunchKernelGGL((rnorm_fwd_kernel<T, L, E, false>), dim3(grid), dim3((L) > 256 ? (L) : 256), 0, st, p)
+  RNORM_BY_WIDTH(RNORM_FWD_GO);
   VEEX_CHECK_LAUNCH();
   return 0;
 }
 
 template <typename T>
 static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hipStream_t st) {
-  const unsigned grid = (unsigned)chunks;
-#define RNORM_BWD_GRID(RG) (void)0
+  const dim3 grid((unsigned)chunks);
   const bool bias = p.dpost_b != nullptr || p.dpre_b != nullptr;
-  if (vec && bias) RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, true, true);
-  else if (vec) RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, true, false);
-  else if (bias) RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, false, true);
-  else RNORM_BY_WIDTH(rnorm_bwd_kernel, RNORM_BWD_GRID, T, false, false);
+#define RNORM_BWD_GO(L, E)                                                                                                        \
+  if (vec && bias) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, true>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);       \
+  else if (vec) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);         \
+  else if (bias) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, true>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);        \
+  else hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p)
+  RNORM_BY_WIDTH(RNORM_BWD_GO);
   VEEX_CHECK_LAUNCH();
   if (p.dgate != nullptr || p.dscale != nullptr || p.dpost_w != nullptr || p.dpost_b != nullptr || p.dpre_w != nullptr || p.dpre_b != nullptr) {
     const long long gate_rows = p.dgate != nullptr && p.rows_per_group > 1 ? std::min<long long>(p.groups, 1024) : 0;
@@ -438,7 +491,7 @@ static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hi
 // rows of a chunk and chunks of a launch: about as many blocks as the chip holds, none across a group's end
 static long long rnorm_chunks(long long rows, int cols, long long groups, long long& per_chunk, long long& per_group) {
   const long long t = rows / groups, blocks = cols > 2048 ? 256 : 512;       // (resident at once: 8 waves a CU)
-  const long long want = std::max<long long>((rows + blocks - 1) / blocks, 4);
+  const long long want = std::max<long long>((rows + blocks - 1) / blocks, std::max(4, rnorm_rows_per_block(cols)));
   if (groups == rows) { per_chunk = want; per_group = 1; return (rows + want - 1) / want; }   // (a gate per element, or one row)
   per_group = (t + want - 1) / want;
   per_chunk = (t + per_group - 1) / per_group;
