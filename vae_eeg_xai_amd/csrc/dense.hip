@@ -87,26 +87,35 @@ __device__ __forceinline__ void dg_tile(const DenseGemm& g, unsigned tile, unsig
   f32x16 acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-  float ra[8], rb[8];
+  // Tiles two turns ahead are on their way in the forward product (64x4096x14336 fp32: one ahead 104 us, two 94; the gradients' shorter
+  // reductions lose by it, 512x6400x100 27 us, 29).
+  constexpr int AHEAD = GRAD ? 1 : 2;
+  float ra[AHEAD][8], rb[AHEAD][8];
   DgOperand<T, AKC, VEC> a;
   DgOperand<T, BKC, VEC> b;
   a.init(g.a, i0, g.I, k_begin, k_end);
   b.init(g.b, j0, g.J, k_begin, k_end);
-  a.load(ra);
-  b.load(rb);
-  int cur = 0;
-  for (long long k0 = k_begin; k0 < k_end; k0 += 32, cur ^= 1) {
-    a.store(As[cur], ra);
-    b.store(Bs[cur], rb);
+  const int turns = (int)((k_end - k_begin + 31) / 32);
+#pragma unroll
+  for (int q = 0; q < AHEAD; ++q)
+    if (q < turns) { a.load(ra[q]); b.load(rb[q]); }
+  auto turn = [&](int t, int cur, int q) {
+    a.store(As[cur], ra[q]);
+    b.store(Bs[cur], rb[q]);
     __syncthreads();      // (the other buffer's readers passed the barrier of the turn before)
-    if (k0 + 32 < k_end) {
-      a.load(ra);
-      b.load(rb);
-    }
+    if (t + AHEAD < turns) { a.load(ra[q]); b.load(rb[q]); }
 #pragma unroll
     for (int s = 0; s < 16; ++s)
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Bs[cur][(2 * s + lh) * DG_LD + wj * 32 + l31],
                                                  As[cur][(2 * s + lh) * DG_LD + wi * 32 + l31], acc, 0, 0, 0);
+  };
+  if (AHEAD == 1) {
+    for (int t = 0; t < turns; ++t) turn(t, t & 1, 0);
+  } else {
+    for (int t = 0; t < turns; t += 2) {
+      turn(t, 0, 0);
+      if (t + 1 < turns) turn(t + 1, 1, AHEAD - 1);
+    }
   }
   // The way out, as in dense_tile.hip: each wave turns its 32 x 32 block round in LDS, so that a lane holds 8 columns of a row
   __syncthreads();
@@ -480,9 +489,9 @@ static int dense_check(const VeexDense* d, const char* who, DropArgs& drop) {
   return 0;
 }
 
-// ---- few rows -------------------------------------------------------------------------------------------------------
-static const int kFewRows = 8;
+static bool lies_well(const VeexDense* d, const void* p, long long ld, long long cols);
 
+// ---- few rows -------------------------------------------------------------------------------------------------------
 template <typename T>
 static bool few_vec(const DenseGemm& g) { return operand_vec(g.b, g.J, sizeof(T)); }
 
@@ -513,8 +522,13 @@ static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
   return join_launch<T>(g, st);
 }
 
-// the weights are worth a second launch to join: from 2^16 of them on (below, one tile of the general product is as quick)
-static bool few_rows(const VeexDense* d) { return d->rows <= kFewRows && (long long)d->k * d->n >= (1 << 16); }
+// Up to 8 rows; 2 where the tiles take the operands as they lie (4096x14336 bf16: 22.9 us for one row, 24.2 for two, 26.3 for three and
+// 46 for eight, where the tiles take 25 for any of them; fp32 4096x14336: 38.4 to 49.6, the general product 90).  And the weights
+// are worth a second launch to join: from 2^16 of them on (below, one tile of the general product is as quick).
+static bool few_rows(const VeexDense* d) {
+  const bool tiles = lies_well(d, d->x, d->ldx, d->k) && lies_well(d, d->w, d->n, d->n);
+  return d->rows <= (tiles ? 2 : 8) && (long long)d->k * d->n >= (1 << 16);
+}
 
 static long long few_bytes(const VeexDense* d, const DenseGemm& g) {
   const int elem = trunk_elem_bytes(d->dtype);
@@ -526,16 +540,15 @@ static long long few_bytes(const VeexDense* d, const DenseGemm& g) {
 // ---- large products -------------------------------------------------------------------------------------------------
 // Which products go to dense_tile.hip.  16-bit types: all that need no packing (16x1024x1024 9.0 us on the general product, 8.5 on
 // the tiles; 512^3 15.3, 8.4), packed ones from 2^26 multiplications on (257x255x259 10, 12.5; 385x383x387 13, 13.7).
-// fp32, which is packed and multiplied six times: from 1.5e9 on (1000^3 34, 32; 2048x1024x1024 53, 43; 4096x1024x1024 90, 60) and 128
-// rows (64x4096x4096 34, 55).
-static bool lies_well(const VeexDense* d, const void* p, long long ld, long long cols);
-
+// fp32, which is packed and multiplied six times: from 1.5e9 on (1000^3 34, 32; 2048x1024x1024 53, 43; 4096x1024x1024 90, 60), with 160
+// rows and columns, or the packed copies are used too little (forward and training call of 128x4096x4096 52 and 154, 66 and 191;
+// 176x4096x4096 92 and 232, 76 and 208; 4096x4096x128 52 and 169, 70 and 195; 8192x100x6400 196 and 614, 184 and 529).
 static bool uses_tiles(const VeexDense* d) {
   // a tile addresses its operand by 32 bits from its first row on: 256 rows of up to 4 MB, 64 k's of up to 16 MB
   const long long widest = std::max<long long>(std::max<long long>(d->k, d->n), d->ldx);
   if (widest >= (1 << 21)) return false;
   const double work = (double)d->rows * d->k * d->n;
-  if (d->dtype == VEEX_T_F32) return work >= 1.5e9 && d->rows >= 128;
+  if (d->dtype == VEEX_T_F32) return work >= 1.5e9 && d->rows >= 160 && d->n >= 160;
   return work >= (1 << 26) || (lies_well(d, d->x, d->ldx, d->k) && lies_well(d, d->w, d->n, d->n) && lies_well(d, d->dy, d->n, d->n));
 }
 
