@@ -282,7 +282,7 @@ int veex_dropout(const void* x, const void* residual, void* y, long long rows, i
  * Backward: dz = D'(dy) act'(z), dx = dz w^T, dw = x^T dz, db = column sums of dz; each of dx, dw, db may be NULL.  pre is what
  * the forward wrote there; for VEEX_ACT_RELU without residual it may be the forward's y instead (y > 0 exactly where an element
  * was kept and z > 0), for VEEX_ACT_NONE it is not read.  d(residual) is dy.
- * rows <= 2^31, k and n <= 2^30.  Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned,
+ * rows <= 2^31, k and n <= 2^30, and a launch takes 2^24 tiles of 64 x 64 (VEEX_EINVAL beyond).  Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned,
  * of at least the bytes that the _workspace function of the direction returns for the same struct (host only; -1: bad). */
 typedef struct VeexDense {
   const void* x; const void* w; const void* bias; const void* residual;
@@ -308,9 +308,10 @@ int veex_dense_bwd(const VeexDense* d, veexStream_t s);
 /* x_out = x + scale gate Norm(h; post_w, post_b), u = Norm(x_out; pre_w, pre_b); with h NULL: u = Norm(x; pre_w, pre_b).
  * Norm: (v - mean) / sqrt(var + eps) * w + b over the row (LAYER), v / sqrt(mean(v^2) + eps) * w + b (RMS); NULL weights
  * and biases are 1 and 0.  gate [groups][cols], row g for rows/groups consecutive rows of x; scale [cols]; both may be NULL (1).
- * stats [rows][4] fp32: written by the forward when not NULL, read by the backward.
+ * stats [rows][4] fp32, 16-byte aligned: written by the forward when not NULL, read by the backward.
  * Backward: gradients of whatever output pointer is not NULL, from dx_out and du (NULL: zero); workspace of
- * veex_residual_norm_bwd_workspace_floats(rows, cols, groups) floats (groups = 1 without gate or h); rows >= 1. */
+ * veex_residual_norm_bwd_workspace_floats(rows, cols, groups) floats (groups = 1 without gate or h); rows >= 1; up to 2^22
+ * groups, or one a row. */
 typedef struct VeexResidualNorm {
   const void* x; const void* h; const void* gate; const void* scale;
   const void* post_w; const void* post_b; const void* pre_w; const void* pre_b;

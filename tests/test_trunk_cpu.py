@@ -158,3 +158,28 @@ def test_host_side_refuses_before_any_launch():
     q.stats = q.workspace = some
     q.workspace_floats = floats - 1
     assert lib.veex_residual_norm_bwd(C.byref(q), None) == -2 and "workspace" in err()
+
+
+def test_more_blocks_than_a_launch_takes_are_refused():
+    from vae_eeg_xai_amd import _lib
+    lib = _lib.lib
+    some = 1 << 20                       # never dereferenced
+    for dtype, rows, k, n in ((0, 1 << 31, 1, 64), (0, 1, 1, 1 << 30), (1, 1 << 31, 512, 256)):
+        d = _lib.DenseDesc()
+        d.struct_size = C.sizeof(d)
+        d.rows, d.k, d.n, d.ldx, d.dtype = rows, k, n, k, dtype
+        d.x = d.w = d.y = d.workspace = some
+        d.workspace_bytes = 1 << 62
+        assert lib.veex_dense_fwd(C.byref(d), None) == -1 and "tiles" in lib.veex_last_error().decode()
+    q = _lib.ResidualNormDesc()
+    q.struct_size = C.sizeof(q)
+    q.rows, q.cols, q.groups, q.eps = 1 << 24, 8, 1 << 23, 1e-3
+    q.x = q.h = q.gate = q.dgate = q.du = q.dx = q.workspace = some
+    q.stats = some + 4
+    q.workspace_floats = 1 << 60
+    assert lib.veex_residual_norm_bwd(C.byref(q), None) == -1 and "aligned" in lib.veex_last_error().decode()
+    q.stats = some
+    assert lib.veex_residual_norm_bwd(C.byref(q), None) == -1 and "groups" in lib.veex_last_error().decode()
+    q.u = q.x_out = some
+    q.stats = some + 8
+    assert lib.veex_residual_norm_fwd(C.byref(q), None) == -1 and "aligned" in lib.veex_last_error().decode()

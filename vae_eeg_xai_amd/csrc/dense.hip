@@ -458,7 +458,7 @@ static int general_launch(DenseGemm g, void* ws, hipStream_t st) {
   general_split(g.I, g.J, g.K, g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
   g.vec_e = dense_epi_vec(g.epi, g.J, sizeof(T));
-  if (general_tiles(g) > 0x7FFFFFFFll) return too_many_tiles();
+  if (!trunk_grid_ok(general_tiles(g), 256)) return too_many_tiles();
   const dim3 grid((unsigned)general_tiles(g), (unsigned)g.splits);
   if (general_vec(kKindFwd, g, sizeof(T))) hipLaunchKernelGGL((dense_general_kernel<T, true>), grid, dim3(256), 0, st, g);
   else hipLaunchKernelGGL((dense_general_kernel<T, false>), grid, dim3(256), 0, st, g);
@@ -470,7 +470,7 @@ static int general_launch(DenseGemm g, void* ws, hipStream_t st) {
 template <typename T>
 static int general_grads_launch(const DenseGemm (&g)[2], hipStream_t st) {
   const long long t0 = general_tiles(g[0]), t1 = general_tiles(g[1]), n0 = t0 * g[0].splits, n1 = t1 * g[1].splits;
-  if (n0 + n1 > 0x7FFFFFFFll) return too_many_tiles();
+  if (!trunk_grid_ok(n0 + n1, 256)) return too_many_tiles();
   const bool vec = (n0 == 0 || general_vec(kKindDx, g[0], sizeof(T))) && (n1 == 0 || general_vec(kKindDw, g[1], sizeof(T)));
   const dim3 grid((unsigned)(n0 + n1));
   if (vec) hipLaunchKernelGGL((dense_general_grads_kernel<T, true>), grid, dim3(256), 0, st, g[0], g[1], (unsigned)t0, (unsigned)n0, (unsigned)t1);
@@ -509,7 +509,9 @@ static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
   few_split(g, vec, sizeof(T), g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
   g.vec_e = dense_epi_vec(g.epi, g.J, sizeof(T));
-  const dim3 grid((unsigned)(vec ? ((long long)g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64), (unsigned)g.splits);
+  const long long strips = vec ? ((long long)g.J * (int)sizeof(T) + 255) / 256 : (g.J + 63) / 64;
+  if (!trunk_grid_ok(strips, 256)) return too_many_tiles();
+  const dim3 grid((unsigned)strips, (unsigned)g.splits);
 #define DF_GO(R)                                                                                              \
   if (vec) hipLaunchKernelGGL((dense_few_rows_kernel<T, R, true>), grid, dim3(256), 0, st, g);                 \
   else hipLaunchKernelGGL((dense_few_rows_kernel<T, R, false>), grid, dim3(256), 0, st, g);
@@ -627,7 +629,7 @@ static bool tile_gemm(int elem, const TilePlan& t, const DenseGemm& g, const DtT
   q.epi = g.epi;
   q.slab = t.splits > 1 ? static_cast<float*>(slab) : nullptr;
   q.vec_e = dense_epi_vec(g.epi, g.J, elem);
-  return (double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits < 1073741824.0;
+  return (double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits < (1 << 22);      // (512 threads each, two products a launch)
 }
 
 // x, w or dy as the tiles load it: where it lies, or packed into *at, which moves on (the job is added to the list)
@@ -817,6 +819,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
     f.first[3] += (unsigned)((d->n + 31) / 32);
   }
   if (f.first[3] == 0) return 0;
+  if (!trunk_grid_ok(f.first[3], 256)) return too_many_tiles();
   const dim3 grid(f.first[3]);
   if (d->dtype == VEEX_T_F32) hipLaunchKernelGGL((dense_finish_kernel<float>), grid, dim3(256), 0, st, f);
   else if (d->dtype == VEEX_T_BF16) hipLaunchKernelGGL((dense_finish_kernel<bf16_t>), grid, dim3(256), 0, st, f);

@@ -536,6 +536,7 @@ int veex_residual_norm_fwd(const VeexResidualNorm* d, hipStream_t st) {
   if (d->x == nullptr || d->u == nullptr || (d->h != nullptr && d->x_out == nullptr)) {
     veex_set_error("residual_norm: x and u (with h also x_out) are needed"); return VEEX_EINVAL;
   }
+  if (!trunk_aligned16(d->stats)) { veex_set_error("residual_norm: stats has to be 16-byte aligned"); return VEEX_EINVAL; }
   if (int rc = rnorm_check("residual_norm", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps)) return rc;
   if (d->rows == 0) return 0;
   RNormParams p;
@@ -556,8 +557,8 @@ long long veex_residual_norm_bwd_workspace_floats(long long rows, int cols, long
 
 int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
   if (!rnorm_struct_ok(d)) return VEEX_EINVAL;
-  if (d->x == nullptr || d->stats == nullptr || d->workspace == nullptr) {
-    veex_set_error("residual_norm backward: x, stats and workspace are needed"); return VEEX_EINVAL;
+  if (d->x == nullptr || d->stats == nullptr || !trunk_aligned16(d->stats) || d->workspace == nullptr) {
+    veex_set_error("residual_norm backward: x, 16-byte aligned stats and workspace are needed"); return VEEX_EINVAL;
   }
   if (int rc = rnorm_check("residual_norm backward", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps)) return rc;
   if (d->rows == 0) { veex_set_error("residual_norm backward: no rows"); return VEEX_EINVAL; }
@@ -566,6 +567,7 @@ int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
   p.x_out = p.u = nullptr;
   const long long chunks = rnorm_chunks(p.rows, p.cols, p.groups, p.rows_per_chunk, p.chunks_per_group);
   if (d->workspace_floats < chunks * 5 * p.cols) { veex_set_error("residual_norm backward: workspace of %lld floats is needed", chunks * 5 * p.cols); return VEEX_ENOMEM; }
+  if (!trunk_grid_ok(chunks, 1024)) { veex_set_error("residual_norm backward: more gate groups than a launch takes"); return VEEX_EINVAL; }
   const bool vec = rnorm_vec(p, d->dtype);
   if (d->dtype == VEEX_T_F32) return rnorm_bwd_launch<float>(p, vec, chunks, st);
   if (d->dtype == VEEX_T_BF16) return rnorm_bwd_launch<bf16_t>(p, vec, chunks, st);

@@ -62,4 +62,7 @@ inline bool trunk_drop_args(double rate, unsigned long long seed, unsigned long 
   return true;
 }
 
+// host: a launch counts its threads along x in 32 bits
+inline bool trunk_grid_ok(long long blocks, int threads) { return blocks > 0 && blocks <= 0xFFFFFFFFll / threads; }
+
 #endif
