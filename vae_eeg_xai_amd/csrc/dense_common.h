@@ -31,21 +31,24 @@ template <typename T> __device__ __forceinline__ float act_rcp(float x) {
   if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(x);
   else return 1.f / x;
 }
-// Phi(z), and e = exp(-z^2 / 2)
+// Phi(z), and e = exp(-z^2 / 2); 16-bit types with every constant folded (8192x1024x4096 bf16: gelu was 16 us of 94)
 template <typename T> __device__ __forceinline__ float act_phi(float z, float& e) {
-  const float x = fabsf(z) * 0.70710678f, t = act_rcp<T>(fmaf(0.37f, x, 1.f));
   float q;
   if constexpr (sizeof(T) == 2) {
-    q = -0.142551705f;
-    q = fmaf(q, t, 0.435660362f); q = fmaf(q, t, -0.186432138f); q = fmaf(q, t, 0.31740576f);
-    q = fmaf(q, t, 0.152655855f); q = fmaf(q, t, 0.214882717f); q = fmaf(q, t, 0.20837988f);
+    const float t = act_rcp<T>(fmaf(0.261629509f, fabsf(z), 1.f));      // 0.37 / sqrt 2
+    q = -0.0712758525f;                                                 // P / 2
+    q = fmaf(q, t, 0.217830181f); q = fmaf(q, t, -0.093216069f); q = fmaf(q, t, 0.15870288f);
+    q = fmaf(q, t, 0.0763279275f); q = fmaf(q, t, 0.107441359f); q = fmaf(q, t, 0.10418994f);
+    e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+    q *= t * e;
   } else {
+    const float x = fabsf(z) * 0.70710678f, t = act_rcp<T>(fmaf(0.37f, x, 1.f));
     q = 0.0619231425f;
     q = fmaf(q, t, -0.303273201f); q = fmaf(q, t, 0.486842126f); q = fmaf(q, t, -0.285312116f); q = fmaf(q, t, 0.310802102f);
     q = fmaf(q, t, 0.106520303f); q = fmaf(q, t, 0.206254035f); q = fmaf(q, t, 0.207429841f); q = fmaf(q, t, 0.208813742f);
+    e = act_exp<T>(-0.5f * z * z);
+    q *= 0.5f * t * e;
   }
-  e = act_exp<T>(-0.5f * z * z);
-  q *= 0.5f * t * e;
   return z > 0.f ? 1.f - q : q;
 }
 
