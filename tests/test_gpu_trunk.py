@@ -79,7 +79,7 @@ def test_dense_large(ops, m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,k,n", [(1, 65536, 1), (1, 257, 1000), (1, 700, 100), (2, 700, 264), (3, 1001, 77), (5, 640, 4096), (8, 4096, 136), (2, 640, 4096), (1, 4096, 136), (7, 700, 264)])
+@pytest.mark.parametrize("m,k,n", [(1, 65536, 1), (1, 257, 1000), (1, 700, 100), (2, 700, 264), (3, 1001, 77), (5, 640, 4096), (8, 4096, 136), (2, 640, 4096), (1, 4096, 136), (7, 700, 264), (1, 1024, 1000), (2, 100, 6400), (4, 1023, 68), (8, 64, 1032), (1, 7, 9368), (3, 1025, 200)])
 def test_dense_few_rows(ops, m, k, n, dt):
     _check_dense(ops, m, k, n, dt, "gelu", True, 0.2, False)
     _check_dense(ops, m, k, n, dt, "sigmoid", False, 0.0, True)

@@ -325,6 +325,79 @@ __global__ __launch_bounds__(256) void dense_few_rows_kernel(DenseGemm g) {
   }
 }
 
+// The same for short columns (k up to 1024) of aligned weights: a block of 1024 threads owns 128 bytes of a row over all of k, each thread
+// every 128th k, all its loads in flight at once; the threads of a column meet through lane rotations and LDS, and the epilogue runs
+// here.  No second launch: one row of 1024x1024 bf16 6.0 us for 7.9, 100x6400 fp32 4.5 for 8.1; with longer columns the strips
+// are too few (4096x1024 bf16 15 us, split 8.5).
+#define DF_SHORT_K 1024
+// sum over a wave's lanes of the same lane % 8
+__device__ __forceinline__ float df_lanes_sum(float x) {
+  x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xF, 0xF, true));      // row_ror:8, of 16 lanes
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+template <typename T, int R>
+__global__ __launch_bounds__(1024) void dense_few_short_kernel(DenseGemm g, unsigned strips) {
+  constexpr int V = 16 / (int)sizeof(T), CL = 8, W = CL * V, KL = 1024 / CL, U = DF_SHORT_K / KL;
+  __shared__ float xs[R][DF_SHORT_K];
+  __shared__ float part[16][R][W + 4];
+  const int cl = threadIdx.x % CL, kl = threadIdx.x / CL, K = (int)g.K;
+  // (blocks go round the 8 XCDs in turn: neighbouring strips, which share lines where rows are not whole ones, to one of them)
+  const unsigned per = strips / 8, extra = strips % 8, xcd = blockIdx.x % 8;
+  const int j0 = (int)(xcd * per + min(xcd, extra) + blockIdx.x / 8) * W, j = j0 + cl * V;
+  const T* x = static_cast<const T*>(g.a.p);
+  const T* w = static_cast<const T*>(g.b.p) + (j < g.J ? j : 0);        // (J is a multiple of V)
+  Piece<T, V> p[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) p[u] = piece_load<T, V>(w + min(kl + u * KL, K - 1) * g.b.k_stride);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (threadIdx.x < K) xs[r][threadIdx.x] = r < g.I ? (float)x[r * g.a.row_stride + threadIdx.x] : 0.f;
+  __syncthreads();
+  float acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[r][e] = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (kl + u * KL < K)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float a = xs[r][kl + u * KL];
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[r][e] = fmaf(a, (float)p[u].v[e], acc[r][e]);
+      }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float a = df_lanes_sum(acc[r][e]);
+      if (lane < CL) part[wave][r][lane * V + e] = a;
+    }
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t < R * W) {
+    float a = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) a += part[q][t / W][t % W];
+    part[0][t / W][t % W] = a;
+  }
+  __syncthreads();
+  const int r = t / (W / 8), c = 8 * (t % (W / 8));
+  if (r >= R || r >= g.I || j0 + c >= g.J) return;
+  float v[8], bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = part[0][r][c + e];
+  unsigned words[4] = {0u, 0u, 0u, 0u};
+  if (g.epi.drop.cut != 0u) drop_words(g.epi.drop, drop_base(g.epi.drop) + (unsigned long long)r, (unsigned)(j0 + c) >> 3, words);
+  dense_bias<T>(g.epi, bias, j0 + c, g.J, g.vec_e);
+  dense_epilogue<T>(g.epi, v, bias, (long long)r * g.J + j0 + c, g.J - (j0 + c), g.vec_e, words);
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // dz = D'(dy) act'(z) and the partial column sums of it (fp32, before dz is rounded): 256 columns a block as 32 threads of 8
 // columns, 8 rows at a time; each block adds a run of rows up and writes one partial row.
@@ -492,9 +565,6 @@ static int dense_check(const VeexDense* d, const char* who, DropArgs& drop) {
 static bool lies_well(const VeexDense* d, const void* p, long long ld, long long cols);
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-template <typename T>
-static bool few_vec(const DenseGemm& g) { return operand_vec(g.b, g.J, sizeof(T)); }
-
 // about 1024 blocks, at least 64 k's each
 static void few_split(const DenseGemm& g, bool vec, int elem, int& splits, long long& per) {
   const long long strips = vec ? ((long long)g.J * elem + 255) / 256 : (g.J + 63) / 64;
@@ -503,9 +573,22 @@ static void few_split(const DenseGemm& g, bool vec, int elem, int& splits, long 
   splits = (int)((g.K + per - 1) / per);
 }
 
+static bool few_short(const DenseGemm& g, int elem) { return g.K <= DF_SHORT_K && operand_vec(g.b, g.J, elem); }
+
 template <typename T>
 static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
-  const bool vec = few_vec<T>(g);
+  if (few_short(g, sizeof(T))) {
+    g.splits = 1;
+    g.vec_e = dense_epi_vec(g.epi, g.J, sizeof(T));
+    const unsigned strips = (unsigned)(((long long)g.J * (int)sizeof(T) + 127) / 128);
+    if (g.I == 1) hipLaunchKernelGGL((dense_few_short_kernel<T, 1>), dim3(strips), dim3(1024), 0, st, g, strips);
+    else if (g.I == 2) hipLaunchKernelGGL((dense_few_short_kernel<T, 2>), dim3(strips), dim3(1024), 0, st, g, strips);
+    else if (g.I <= 4) hipLaunchKernelGGL((dense_few_short_kernel<T, 4>), dim3(strips), dim3(1024), 0, st, g, strips);
+    else hipLaunchKernelGGL((dense_few_short_kernel<T, 8>), dim3(strips), dim3(1024), 0, st, g, strips);
+    VEEX_CHECK_LAUNCH();
+    return 0;
+  }
+  const bool vec = operand_vec(g.b, g.J, sizeof(T));
   few_split(g, vec, sizeof(T), g.splits, g.k_per_split);
   g.slab = static_cast<float*>(ws);
   g.vec_e = dense_epi_vec(g.epi, g.J, sizeof(T));
@@ -529,11 +612,12 @@ static int few_launch(DenseGemm g, void* ws, hipStream_t st) {
 // are worth a second launch to join: from 2^16 of them on (below, one tile of the general product is as quick).
 static bool few_rows(const VeexDense* d) {
   const bool tiles = lies_well(d, d->x, d->ldx, d->k) && lies_well(d, d->w, d->n, d->n);
-  return d->rows <= (tiles ? 2 : 8) && (long long)d->k * d->n >= (1 << 16);
+  return d->rows <= (tiles ? 2 : 8) && (long long)d->k * d->n >= (1 << 16) && d->n <= (1 << 24);
 }
 
 static long long few_bytes(const VeexDense* d, const DenseGemm& g) {
   const int elem = trunk_elem_bytes(d->dtype);
+  if (few_short(g, elem)) return 0;
   int s; long long per;
   few_split(g, operand_vec(g.b, g.J, elem), elem, s, per);
   return align256(s * g.I * slab_ld(g.J) * 4);
