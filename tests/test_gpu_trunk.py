@@ -72,7 +72,7 @@ def test_dense_sizes(ops, m, k, n, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,k,n", [(300, 1000, 520), (1030, 264, 1001), (129, 4104, 260), (260, 5000, 136), (1500, 72, 2056), (2051, 513, 259), (1500, 1032, 1104), (1303, 1001, 1207)])
+@pytest.mark.parametrize("m,k,n", [(300, 1000, 520), (1030, 264, 1001), (129, 4104, 260), (260, 5000, 136), (8000, 2000, 60), (1500, 72, 2056), (2051, 513, 259), (1500, 1032, 1104), (1303, 1001, 1207)])
 def test_dense_large(ops, m, k, n, dt):
     """On the 16-bit matrix cores: tiles that end inside the tensors, odd sizes that are packed, split reductions."""
     _check_dense(ops, m, k, n, dt, "silu", True, 0.1, True)
