@@ -229,17 +229,18 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
   const float inv = 1.f / (float)p.cols;
   const bool post = p.h != nullptr;
 
-  // A block of 16 waves has 128 registers a lane: there the vectors are read again for each row (from the L2), the next row is not
-  // fetched ahead and the column sums stay in LDS, or registers would be spilled (8192 columns, 4096 rows, bf16: 411 us, so 101).
+  // The vectors are kept as fp32 and scale times a grouped gate as one (unpacked for every row they were a fifth of the arithmetic, and
+  // with two waves a SIMD that counts: 16384x1024 fp32 73 us, so 66; bf16 49, 47.5).  A block of 16 waves has 128 registers a lane: there they are read
+  // again for each row (from the L2), the next row is not fetched ahead and the column sums stay in LDS, or registers would be
+  // spilled (8192 columns, 4096 rows, bf16: 411 us, so 101).
   constexpr bool AHEAD = LANES < 1024;
-  RowRaw<T, V, C> scale, ow, ob, pw, gr;
-  auto vectors_post = [&] {
-    row_param<T, V, C, LANES>(scale, p.scale, 1.f, lane, p.cols);
-    row_param<T, V, C, LANES>(ow, p.post_w, 1.f, lane, p.cols);
-    row_param<T, V, C, LANES>(ob, p.post_b, 0.f, lane, p.cols);
+  float sg[EPL], ow[EPL], ob[EPL], pw[EPL];
+  auto vector = [&](float (&v)[EPL], const void* q, float otherwise) {
+    RowRaw<T, V, C> r;
+    row_param<T, V, C, LANES>(r, q, otherwise, lane, p.cols);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) v[e] = (float)r.p[e / V].v[e % V];
   };
-  auto vectors_pre = [&] { row_param<T, V, C, LANES>(pw, p.pre_w, 1.f, lane, p.cols); };
-  if (AHEAD) { vectors_post(); vectors_pre(); }
   bool in[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) in[c] = (c * LANES + lane) * V < p.cols;
@@ -248,11 +249,16 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
   const long long first = group * p.rows_per_group + piece * p.rows_per_chunk;
   const long long last = min(first + p.rows_per_chunk, (group + 1) * p.rows_per_group);     // one past
   const bool full_gate = p.gate != nullptr && p.rows_per_group == 1;
-  auto gate_row = [&](RowRaw<T, V, C>& g) {
-    if (p.gate != nullptr) row_load<T, V, C, LANES>(g, p.gate, group * p.cols, lane, p.cols);
-    else row_fill<T, V, C, LANES>(g, 1.f);
+  auto vectors_post = [&] {
+    vector(sg, p.scale, 1.f); vector(ow, p.post_w, 1.f); vector(ob, p.post_b, 0.f);
+    if (p.gate != nullptr && !full_gate) {
+      float g[EPL];
+      vector(g, static_cast<const T*>(p.gate) + group * p.cols, 1.f);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) sg[e] *= g[e];
+    }
   };
-  if (AHEAD) gate_row(gr);
+  if (AHEAD) { vectors_post(); vector(pw, p.pre_w, 1.f); }
 
   // the column sums of the block's rows; a lane's own, the first HELD of them in LDS
   enum { GATE, POST_W, PRE_W, POST_B, PRE_B };
@@ -286,8 +292,6 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
     if (p.du != nullptr) row_load<T, V, C, LANES>(r.du, p.du, at, lane, p.cols);
     else row_fill<T, V, C, LANES>(r.du, 0.f);
     if (full_gate) row_load<T, V, C, LANES>(r.g, p.gate, at, lane, p.cols);
-    else if (AHEAD) row_copy(r.g, gr);
-    else gate_row(r.g);
     r.st = *reinterpret_cast<const float4*>(p.stats + row * 4);
   };
   In in_now, in_next;
@@ -295,10 +299,16 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
   for (long long r0 = c_first; r0 < c_last; r0 += RG) {
     const bool live = r0 + rg < c_last;
     const long long row = live ? r0 + rg : c_last - 1, at = row * p.cols;
-    if (!AHEAD) { fetch(in_now, r0 + rg); vectors_post(); vectors_pre(); }
+    if (!AHEAD) { fetch(in_now, r0 + rg); vectors_post(); vector(pw, p.pre_w, 1.f); }
     else if (r0 + RG < c_last) fetch(in_next, r0 + RG + rg);          // (as in the forward kernel)
     const RowRaw<T, V, C>&xr = in_now.x, &hr = in_now.h, &dor = in_now.dout, &dur = in_now.du, &gr = in_now.g;
     const float4 st = in_now.st;
+    // (behind the row's end x, h and the gradients are zeros: with a zero for 1 / deviation there, so is all that follows)
+    float rstd1[C], rstd2[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) { rstd1[c] = in[c] ? st.y : 0.f; rstd2[c] = in[c] ? st.w : 0.f; }
+    // scale times the gate of this row
+    auto weight = [&](int e) { return full_gate ? sg[e] * (float)gr.p[e / V].v[e % V] : sg[e]; };
     float xh[EPL], rh[EPL], d[EPL];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -307,49 +317,43 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
       float out = (float)xr.p[c].v[k];
       xh[e] = 0.f;
       if (post) {
-        xh[e] = ((float)hr.p[c].v[k] - st.x) * st.y;
-        out = fmaf((float)scale.p[c].v[k] * (float)gr.p[c].v[k], fmaf(xh[e], (float)ow.p[c].v[k], (float)ob.p[c].v[k]), out);
+        xh[e] = ((float)hr.p[c].v[k] - st.x) * rstd1[c];
+        out = fmaf(weight(e), fmaf(xh[e], ow[e], ob[e]), out);
       }
-      rh[e] = in[c] ? (out - st.z) * st.w : 0.f;
+      rh[e] = (out - st.z) * rstd2[c];
       const float du = (float)dur.p[c].v[k];
       if (live) {
         add(PRE_W, e, du, rh[e]);
         if (BIAS) add(PRE_B, e, du, 1.f);
       }
-      d[e] = du * (float)pw.p[c].v[k];
+      d[e] = du * pw[e];
       s1 += d[e]; s2 = fmaf(d[e], rh[e], s2);
     }
     float2 m = row_sum(s1, s2);
     m.x = p.layer ? m.x * inv : 0.f; m.y *= inv;
     s1 = s2 = 0.f;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      const int c = e / V, k = e % V;
-      d[e] = fmaf(st.w, d[e] - fmaf(rh[e], m.y, m.x), (float)dor.p[c].v[k]);      // D
-    }
+    for (int e = 0; e < EPL; ++e) d[e] = fmaf(rstd2[e / V], d[e] - fmaf(rh[e], m.y, m.x), (float)dor.p[e / V].v[e % V]);      // D
     if (live && p.dx != nullptr) row_store<T, V, C, LANES>(p.dx, at, d, lane, p.cols);
     if (post) {
       if (!AHEAD) vectors_post();
       if (live && full_gate && p.dgate != nullptr) {
         float dg[EPL];
 #pragma unroll
-        for (int e = 0; e < EPL; ++e)
-          dg[e] = d[e] * (float)scale.p[e / V].v[e % V] * fmaf(xh[e], (float)ow.p[e / V].v[e % V], (float)ob.p[e / V].v[e % V]);
+        for (int e = 0; e < EPL; ++e) dg[e] = d[e] * sg[e] * fmaf(xh[e], ow[e], ob[e]);
         row_store<T, V, C, LANES>(p.dgate, at, dg, lane, p.cols);
       }
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
-        const int c = e / V, k = e % V;
-        const float s = (float)scale.p[c].v[k], g = (float)gr.p[c].v[k], n = fmaf(xh[e], (float)ow.p[c].v[k], (float)ob.p[c].v[k]);
-        if (!in[c]) d[e] = 0.f;
-        const float dn = d[e] * (s * g);
+        const float n = fmaf(xh[e], ow[e], ob[e]), dn = d[e] * weight(e);
         if (live) {
-          add(GATE, e, d[e] * n, full_gate ? g : 1.f);
+          if (full_gate) add(GATE, e, d[e] * n, (float)gr.p[e / V].v[e % V]);
+          else add(GATE, e, d[e], n);
           add(POST_W, e, dn, xh[e]);
           if (BIAS) add(POST_B, e, dn, 1.f);
         }
-        d[e] = dn * (float)ow.p[c].v[k];
-        s1 += d[e]; s2 = fmaf(d[e], in[c] ? xh[e] : 0.f, s2);
+        d[e] = dn * ow[e];
+        s1 += d[e]; s2 = fmaf(d[e], xh[e], s2);
       }
       m = row_sum(s1, s2);
       m.x = p.layer ? m.x * inv : 0.f; m.y *= inv;
