@@ -12,6 +12,12 @@
 //   [row][64]: s = (row >> 1) & 7;  [row][32]: s = (row >> 2) & 3;  [k][128]: s = (k & 3) << 2
 // (16 lanes read at a time, 256 bytes: 16 consecutive rows of one piece have to fall on 16 different ones)
 //
+// Bound: matrix cores and the chip's power: 4096^3 bf16 runs at 1 120 TFLOP/s, 8192x4096x4096 at 1 190, with the matrix cores busy 55 %
+// of the cycles and the clock down to 1.9 GHz (library: 1 116 at 8192^3, 1 340 at 8192x4096x4096); fp32 at 190 to 200 (library 153).
+// Short reductions pay for the epilogue, which nothing overlaps (one tile a CU): 8192x1024x4096 bf16 77 us, with gelu 92, with z
+// kept as well 96 to 105; 8192x4096x1024 70.  Two tiles a CU of half the size overlap it but gather twice the operands: 88 to 130 us.
+// 256x256 by 4 waves of 128x128, with a third fewer LDS reads: 107 us for 92, one wave a SIMD hides nothing.
+//
 // Needs: 16-byte aligned operands and rows; a k-contiguous operand's K a multiple of 8.  Pieces past a tensor's end
 // are sent out of the buffer's range and arrive as zeros.
 #include "dense_tile.h"

@@ -3,7 +3,9 @@
 // dy: nothing is kept between the two.
 //
 // Bound: HBM (2 or 3 elements moved per element).  A thread owns blocks of 8 columns of one row -- one Philox call each, and
-// 16 bytes per tensor of a 16-bit type.
+// 16 bytes per tensor of a 16-bit type.  16384x4096 bf16: 49 us (5.5 TB/s), with a residual 70 us (5.8 TB/s; a copy of 1 GB: 4.9).
+// Stores that pass by the caches would take 4 % less, but the kernel that reads y next then waits for it: fp32 of 64 MB, a
+// chain of dropouts, 20 us each as it is and 26 with them.
 #include "trunk_common.h"
 #include "../../include/veex.h"
 #include <algorithm>
