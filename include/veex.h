@@ -257,6 +257,7 @@ int veex_band_outside_counts(const float* z, int N, int L, int nb, const double*
  * composes a dense residual network from beside the convolution layers above.  Data of all tensors of a call has one
  * type (VEEX_T_*); all sums and statistics are fp32.  Rows are row-major and unpadded except where a stride is given.
  * No reference call site beyond keras.layers.Dense (models.py:238-241,264).
+ * Outputs may not overlap inputs.
  * ---------------------------------------------------------------------------------------- */
 #define VEEX_T_F32 0
 #define VEEX_T_BF16 1

@@ -20,6 +20,11 @@ and backward draw the same one, and shards of a batch that pass their first glob
 ``counter`` is an int64 word on the device that is read when the kernel runs: a captured step that advances it draws anew at
 every replay.  The backward pass uses the word's value at the forward call.
 
+dense takes an x whose rows lie any distance apart as it is; other tensors that are not contiguous, a transposed w among them, are
+copied first, on every call.  All ops can be captured into graphs, training steps too.  As with every torch op, no eager
+graph of the same leaves may be alive while a backward pass is captured: torch keeps a leaf's gradient node on the stream where
+it was made, and the capture fails there.
+
 The ops, their checks and their autograd are C++ (csrc/torch_ops.cpp, libveex_torch.so); this module loads them and adds the fake
 implementations of the low-level ops ``veex::dense_fwd`` etc., whose kernels are registered for the ``cuda`` device type only.
 """
