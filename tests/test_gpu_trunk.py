@@ -534,3 +534,85 @@ def test_two_captured_graphs_share_nothing(ops, dt, m, k, n):
                 graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_offsets_past_32_bits(ops, dt):
+    """Tensors of more than 2^31 elements: their last rows come out as those of a call that holds only them.  The products pick single
+    elements: exact, but for fp32 ones as three bf16 terms (2^-25 left out, and up to six roundings of 2^-24: 2^-21 covers them)."""
+    t = ref.TYPES[dt]
+    same = torch.equal if dt == "bf16" else lambda a, b: bool(((a - b).abs() <= b.abs() * 2.0 ** -21).all())  # noqa: E731
+    rows, cols, last = (1 << 21) + 5, 1032, 7
+    x = torch.empty(rows, cols, device="cuda", dtype=t).normal_()
+    tail = x[-last:].clone()
+    y = ops.dropout(x, 0.25, 3)
+    assert torch.equal(y[-last:], ops.dropout(tail, 0.25, 3, rows - last))
+    out, u = ops.residual_norm(x, y, kind="rms")
+    alone = ops.residual_norm(tail, y[-last:].clone(), kind="rms")
+    assert torch.equal(out[-last:], alone[0]) and torch.equal(u[-last:], alone[1])
+    st = torch.ones(rows, 4, device="cuda")
+    st[:, 0] = st[:, 2] = 0.0
+    need = [True, True] + [False] * 6
+    whole = ops.residual_norm_bwd(x, y, None, None, None, None, None, None, 1, 1, 1e-3, st, x, None, need)
+    part = ops.residual_norm_bwd(tail, y[-last:].clone(), None, None, None, None, None, None, 1, 1, 1e-3, st[-last:].clone(), tail, None, need)
+    assert torch.equal(whole[0][-last:], part[0]) and torch.equal(whole[1][-last:], part[1])
+    del out, u, alone, whole, part, y, st
+    # dx of a product whose dy is the large tensor, y of one whose y is, dw of one whose x is
+    w = torch.zeros(8, cols, device="cuda", dtype=t)
+    w[torch.arange(8), torch.arange(8) * 129] = 1.0
+    small = torch.ones(rows, 8, device="cuda", dtype=t)
+    dx = ops.dense_bwd(x, small, w, None, 0, 0.0, 0, 0, None, True, False, False)[0]
+    assert same(dx[-last:], x[-last:, ::129][:, :8])
+    y = ops.dense(dx, w)
+    assert same(y[-last:, ::129][:, :8], dx[-last:]) and int((y[-last:] != 0).sum()) <= 8 * last
+    del y, dx
+    small.zero_()
+    small[-1] = 1.0
+    dw = ops.dense_bwd(small, x, torch.zeros(cols, 8, device="cuda", dtype=t), None, 0, 0.0, 0, 0, None, False, True, False)[1]
+    assert torch.equal(dw, x[-1][:, None].expand(cols, 8))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("k,n", [(65544, 32776), (1024, 2100008), (65543, 32777)])
+def test_weights_of_more_than_2_to_the_31_elements(ops, k, n, dt):
+    """Rows of x with a single one pick rows of w, the last among them, on every path a forward call takes."""
+    t = ref.TYPES[dt]
+    w = torch.empty(k, n, device="cuda", dtype=t).normal_()
+    for m in (1, 2, 5, 20):
+        x = torch.zeros(m, k, device="cuda", dtype=t)
+        at = k - 1 - torch.arange(m) * 3
+        x[torch.arange(m), at] = 1.0
+        assert torch.equal(ops.dense(x, w), w[at.cuda()])
+
+
+def test_calls_from_several_threads_at_once(ops):
+    """Each thread on a stream of its own: nothing is shared between calls, so each gets what it gets alone."""
+    import threading
+
+    def work(i):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        m, k, n = [(1, 700, 264), (300, 264, 520), (129, 100, 77), (64, 1001, 333)][i % 4]
+        t = [torch.float32, torch.bfloat16, torch.float16][i % 3]
+        x, w, r = (torch.randn(*s, device="cuda", generator=g).to(t).requires_grad_() for s in ((m, k), (k, n), (m, n)))
+        y = ops.dense(x, w, None, "gelu", r, 0.1, i)
+        out, u = ops.residual_norm(r, y, kind="rms")
+        return [y.detach(), u.detach()] + list(torch.autograd.grad((u * u).sum() + out.sum(), (x, w, r)))
+
+    alone = [work(i) for i in range(8)]
+    torch.cuda.synchronize()
+    together = [None] * 8
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                together[i] = work(i)
+        s.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, together):
+        assert b is not None and all(torch.equal(p, q) for p, q in zip(a, b))
