@@ -59,6 +59,13 @@ void check_drop(const char* what, const Tensor& x, double rate, int64_t first_ro
                     what, ": counter has to be one int64 word on x's device");
 }
 
+// Forward-mode derivatives: no tangents are computed.  A dual tensor need not have requires_grad, and the ops under the public ones are
+// called below autograd, where its tangent would go unnoticed and count as zero; so it is refused here, and in the backward passes.
+void refuse_tangents(const char* what, at::ArrayRef<Tensor> tensors) {
+  for (const Tensor& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not implemented");
+}
+
 // the counter's word as a forward call saw it, for the backward pass: the caller may advance it in between
 Tensor word_now(const Tensor& counter, bool used) { return counter.defined() && used ? counter.detach().add(0) : Tensor(); }
 
@@ -122,6 +129,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 Tensor dropout(const Tensor& x, double rate, int64_t seed, int64_t first_row, const OptTensor& residual_in, const OptTensor& counter) {
   const Tensor residual = get(residual_in);
   check_dropout_args(x, residual, rate, first_row, get(counter));
+  refuse_tangents("dropout", {x, residual});
   if (at::GradMode::is_enabled() && (learns(x) || learns(residual))) return Dropout::apply(x, rate, seed, first_row, residual_in, counter);
   return call_dropout_fwd(x, rate, seed, first_row, residual_in, counter);
 }
@@ -255,6 +263,7 @@ struct Dense : torch::autograd::Function<Dense> {
     if (need_x || need_w || need_b) {
       static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("veex::dense_bwd", "").typed<decltype(dense_bwd)>();
       const auto saved = ctx->get_saved_variables();
+      refuse_tangents("dense backward", {grads[0], saved[0], saved[1]});
       const BelowUnlessRecording below;
       auto [dx, dw, db] = op.call(grads[0], saved[0], saved[1], opt(saved[2]), ctx->saved_data["activation"].toInt(), ctx->saved_data["rate"].toDouble(),
                                   ctx->saved_data["seed"].toInt(), ctx->saved_data["first_row"].toInt(), opt(saved[3]), need_x, need_w, need_b);
@@ -272,6 +281,7 @@ Tensor dense(const Tensor& x, const Tensor& w, const OptTensor& bias_in, std::op
   const Tensor bias = get(bias_in), residual = get(residual_in);
   check_dense_args(x, w, bias, residual, rate, first_row, get(counter));
   const int act = activation_code(activation);
+  refuse_tangents("dense", {x, w, bias, residual});
   if (at::GradMode::is_enabled() && (learns(x) || learns(w) || learns(bias) || learns(residual)))
     return Dense::apply(x, w, bias_in, (int64_t)act, residual_in, rate, seed, first_row, counter);
   return std::get<0>(call_dense_fwd(x, w, bias_in, act, residual_in, rate, seed, first_row, counter, false));
@@ -386,6 +396,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     if (!dx_out.defined() && !du.defined()) return out;
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("veex::residual_norm_bwd", "").typed<decltype(norm_bwd)>();
     const auto s = ctx->get_saved_variables();
+    refuse_tangents("residual_norm backward", {dx_out, du});
+    refuse_tangents("residual_norm backward", s);
     std::array<bool, 8> need;
     for (int i = 0, given = 0; i < 8; ++i) need[i] = s[i].defined() && ctx->needs_input_grad(given++);   // (counts the tensors given)
     const BelowUnlessRecording below;
@@ -420,6 +432,7 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& h_in,
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "residual_norm: rows of 1 to ", VEEX_NORM_MAX_COLS, " columns, not x ", x.sizes());
   const int64_t groups = gate.defined() ? gate_groups(gate, x) : 1, code = kind == "layer" ? VEEX_NORM_LAYER : VEEX_NORM_RMS;
   check_norm_args(t, groups, eps);
+  refuse_tangents("residual_norm", t);
   bool grad = false;
   for (const Tensor& v : t) grad = grad || learns(v);
   if (grad && at::GradMode::is_enabled()) {

@@ -13,7 +13,8 @@
         x (B, T, N)), or x's shape; for a two-dimensional x also (G, N) with G dividing the rows, row r taking gate[r // (rows / G)].
 
 float32, bfloat16 and float16, one type for all tensors of a call; sums and statistics are fp32 inside.  All are differentiable
-once (dropout any number of times) in every tensor but ``counter``.
+once (dropout any number of times) in every tensor but ``counter``, in reverse mode: a tensor with a forward-mode tangent
+(torch.func.jvp, forward_ad.make_dual) is refused with NotImplementedError.
 
 Dropout keeps no mask: the decision for an element is a function of (seed, first_row + counter + its row, its column), so forward
 and backward draw the same one, and shards of a batch that pass their first global row draw what one process would.
