@@ -141,6 +141,7 @@ __device__ __forceinline__ void dg_tile(const DenseGemm& g, unsigned tile, unsig
       *reinterpret_cast<float4*>(s) = lo;
       if (j + 4 < g.J) *reinterpret_cast<float4*>(s + 4) = hi;
     } else if (GRAD) {
+      grad_scale<T>(v, g.alpha);
       store8<T>(static_cast<T*>(g.epi.y) + i * g.J + j, v, g.J - j, g.vec_e);
     } else {
       unsigned w[4] = {0u, 0u, 0u, 0u};
@@ -236,6 +237,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseGemm g) {
 // block).  Jobs without blocks are skipped.
 struct DenseFinish {
   struct Sum { const float* slab; void* out; long long I; int J, splits, lanes, vec; } sum[2];
+  float alpha;
   const float* part; void* db; int chunks, n;
   unsigned first[4];             // a job's first block; the end
 };
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(256) void dense_finish_kernel(DenseFinish f) {
     const int q = b < f.first[1] ? 0 : 1;
     const DenseFinish::Sum& s = f.sum[q];
     const unsigned block = b - f.first[q], blocks = f.first[q + 1] - f.first[q];
-    auto out = [&](float (&v)[8], long long i, int j) { store8<T>(static_cast<T*>(s.out) + i * s.J + j, v, s.J - j, s.vec); };
+    auto out = [&](float (&v)[8], long long i, int j) { grad_scale<T>(v, f.alpha); store8<T>(static_cast<T*>(s.out) + i * s.J + j, v, s.J - j, s.vec); };
     if (s.lanes == 1) dense_sum_slabs<1>(s.slab, s.I, s.J, s.splits, block, blocks, part, out);
     else if (s.lanes == 8) dense_sum_slabs<8>(s.slab, s.I, s.J, s.splits, block, blocks, part, out);
     else dense_sum_slabs<32>(s.slab, s.I, s.J, s.splits, block, blocks, part, out);
@@ -407,6 +409,9 @@ __global__ __launch_bounds__(1024) void dense_few_short_kernel(DenseGemm g, unsi
 // dz is rounded to the tensors' type, as the matrix cores take it and as a gradient handed on between layers would be: dx and dw of 16-bit
 // types carry that half step beside their own (8192x1024x4096 bf16: 1.4 times the error of sums over an unrounded dz); db does not,
 // and fp32 goes on as three planes.
+// fp16's dz is stored without the dropout's scale and times 7/8 behind an activation whose slope passes 1 (gelu 1.129, silu 1.100): then
+// it is no larger than dy, and a finite dy (of up to 65504) never becomes an infinity, which the products would spread over whole rows and columns;
+// grad_scale undoes the factor on the fp32 sums.  At the low end dz keeps steps of 2^-24, those that dy itself came in.
 // Bound: HBM.  8192x4096 bf16 gelu: 41 us with dy and z in the cache behind the L2, 54 without (201 MB, 4.9 and 3.7 TB/s).
 // ---------------------------------------------------------------------------------------------------------------
 struct DenseDz {
@@ -417,6 +422,7 @@ struct DenseDz {
   void* db;              // with one chunk: the sums themselves, instead of part
   long long rows, rows_per_chunk;
   int n, act, vec;
+  float dz_scale;        // fp16: the factor that dz is stored with
   DropArgs drop;
 };
 
@@ -463,6 +469,10 @@ __global__ __launch_bounds__(256) void dense_dz_kernel(DenseDz p) {
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += g[e];
+        if constexpr (TrunkType<T>::code == VEEX_T_F16) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] *= p.dz_scale;
+        }
         if (p.dz != nullptr && p.plane_bytes != 0) dt_store_planes(static_cast<char*>(p.dz) + (i * p.ld + j) * 2, p.plane_bytes, g);
         else if (p.dz != nullptr) store8<T>(static_cast<T*>(p.dz) + i * p.ld + j, g, (int)(p.ld - j), VEC);
       }
@@ -726,6 +736,7 @@ static bool tile_gemm(int elem, const TilePlan& t, const DenseGemm& g, const DtT
   q.epi = g.epi;
   q.slab = t.splits > 1 ? static_cast<float*>(slab) : nullptr;
   q.vec_e = dense_epi_vec(g.epi, g.J, elem);
+  q.alpha = g.alpha;
   return (double)((g.I + t.bm - 1) / t.bm) * ((g.J + t.bn - 1) / t.bn) * t.splits < (1 << 22);      // (512 threads each, two products a launch)
 }
 
@@ -754,6 +765,13 @@ struct BwdLayout {
   int chunks;
   long long total() const { return dz + part + packed + slab[0] + slab[1]; }
 };
+
+// what dz is stored with (dense_dz_kernel)
+static float dz_factor(const VeexDense* d, const DropArgs& drop) {
+  if (d->dtype != VEEX_T_F16) return 1.f;
+  const bool steep = d->activation == VEEX_ACT_GELU || d->activation == VEEX_ACT_SILU;
+  return (steep ? 0.875f : 1.f) * (drop.cut != 0u ? (float)(65536u - drop.cut) / 65536.f : 1.f);
+}
 
 static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
   BwdLayout l = {};
@@ -838,6 +856,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
   char* ws = static_cast<char*>(d->workspace);
   const bool products = d->dx != nullptr || d->dw != nullptr;
   const void* dz = l.dz_own ? ws : d->dy;                  // the general product's
+  const float factor = l.dz_own ? dz_factor(d, drop) : 1.f;
   DtTensor dzt = {ws, round8(d->n) * 2, packed_plane(d->rows, d->n)};    // the tiles'
   if (l.dz_own || d->db != nullptr) {
     DenseDz p = {};
@@ -846,7 +865,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
     p.plane_bytes = l.tiles && d->dtype == VEEX_T_F32 ? dzt.plane_bytes : 0;
     p.db = l.chunks == 1 ? d->db : nullptr;
     p.part = d->db != nullptr && l.chunks > 1 ? reinterpret_cast<float*>(ws + l.dz) : nullptr;
-    p.rows = d->rows; p.rows_per_chunk = l.rows_per_chunk; p.n = d->n; p.act = d->activation; p.drop = drop;
+    p.rows = d->rows; p.rows_per_chunk = l.rows_per_chunk; p.n = d->n; p.act = d->activation; p.drop = drop; p.dz_scale = factor;
     p.vec = (long long)d->n * trunk_elem_bytes(d->dtype) % 16 == 0 && trunk_aligned16(d->dy) && (d->activation == VEEX_ACT_NONE || trunk_aligned16(d->pre));
     if (p.dz != nullptr || d->db != nullptr) {
       const dim3 grid((d->n + 255) / 256, l.chunks);
@@ -868,7 +887,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
   DenseGemm g[2] = {};
   if (d->dx != nullptr) g[0] = dense_product(kKindDx, d, dz);
   if (d->dw != nullptr) g[1] = dense_product(kKindDw, d, dz);
-  for (int q = 0; q < 2; ++q) { g[q].splits = 1; g[q].slab = slabs[q]; g[q].vec_e = dense_epi_vec(g[q].epi, g[q].J, trunk_elem_bytes(d->dtype)); }
+  for (int q = 0; q < 2; ++q) { g[q].splits = 1; g[q].alpha = 1.f / factor; g[q].slab = slabs[q]; g[q].vec_e = dense_epi_vec(g[q].epi, g[q].J, trunk_elem_bytes(d->dtype)); }
   if (products && !l.tiles) {
     for (DenseGemm& q : g)
       if (q.I > 0) general_split(q.I, q.J, q.K, q.splits, q.k_per_split);
@@ -903,6 +922,7 @@ int veex_dense_bwd(const VeexDense* d, hipStream_t st) {
   }
 
   DenseFinish f = {};
+  f.alpha = 1.f / factor;
   for (int q = 0; q < 2; ++q) {
     f.first[q + 1] = f.first[q];
     if (g[q].splits == 1) continue;

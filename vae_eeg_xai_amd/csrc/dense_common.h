@@ -144,6 +144,15 @@ __device__ __forceinline__ void store8(T* p, const float (&s)[8], int n, bool ve
   }
 }
 
+// A gradient on its way out: times alpha, which undoes the factor that fp16's dz was stored with (dense.hip; 1 for the other types)
+template <typename T>
+__device__ __forceinline__ void grad_scale(float (&v)[8], float alpha) {
+  if constexpr (TrunkType<T>::code == VEEX_T_F16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= alpha;
+  }
+}
+
 // Columns j .. j + 7 (j a multiple of 8, n of them inside the row) of row i, `at` = i * J + j: v = acc, b = the bias there (zeros
 // without one), words = the row's dropout words of that block.  A thread that walks down rows loads b once.
 template <typename T>
@@ -205,6 +214,7 @@ struct DenseGemm {
   int splits;
   long long k_per_split;
   int vec_e;             // the epilogue's tensors move in 16-byte pieces
+  float alpha;           // a gradient: grad_scale
 };
 
 #endif

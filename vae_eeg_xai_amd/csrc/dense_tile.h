@@ -15,6 +15,7 @@ struct DtGemm {
   DenseEpi epi;
   float* slab;           // null: the epilogue runs here
   int vec_e;             // the epilogue's tensors move in 16-byte pieces
+  float alpha;           // a gradient: grad_scale
 };
 
 // akc / bkc: that operand's k index is its contiguous one.  tile: 0 256x256 (16-bit types), 1 256x128, 2 128x128

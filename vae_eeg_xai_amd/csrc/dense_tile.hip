@@ -289,6 +289,7 @@ __device__ __forceinline__ void dt_tile(const DtGemm& g, unsigned block, char* s
       } else {
         float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         if (GRAD) {
+          grad_scale<T>(v, g.alpha);
           store8<T>(static_cast<T*>(g.epi.y) + at, v, g.J - j, g.vec_e);
         } else {
           unsigned w[4] = {0u, 0u, 0u, 0u};
