@@ -56,3 +56,21 @@ def test_fp16_gradients_of_large_and_small_dy(ops, m, k, n, act, rate, size):
     got = torch.autograd.grad(y, dev[:2], dy.cuda())
     ref.within(got[0], want[0], ex, "dx")
     ref.within(got[1], want[1], ew, "dw")
+
+
+@pytest.mark.parametrize("m,k,n", [(16, 64, 16), (40, 33, 21), (300, 264, 520)])
+@pytest.mark.parametrize("act", ["gelu", "silu", "relu"])
+def test_bf16_sums_between_its_range_and_fp32s(ops, m, k, n, act):
+    """A z that fp32 holds and bf16 rounds to an infinity: the gradient is the activation's limit, not NaN, as for fp16."""
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        x[:, 0], x[:, 1] = 255 * 2.0 ** 120, 2.0 ** 119
+    w = torch.zeros(k, n, dtype=torch.bfloat16, device="cuda")
+    w[:2, ::2], w[:2, 1::2] = 1.0, -1.0
+    assert float((x.detach().float() @ w.float())[0, 0]) == 511 * 2.0 ** 119
+    r = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    for residual in (None, r):
+        y = ops.dense(x, w, None, act, residual)
+        assert bool((y[:, ::2] == float("inf")).all()) and not y[:, 1::2].any()
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert bool((dx[:, :2] == (n + 1) // 2).all()) and not dx[:, 2:].any()
