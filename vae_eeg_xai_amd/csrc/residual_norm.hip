@@ -25,11 +25,12 @@ struct RNormParams {
   float* stats;              // [rows][4]: mean1, rstd1, mean2, rstd2
   const void *dx_out, *du;   // backward; either may be null (a zero gradient)
   void *dx, *dh, *dgate, *dscale, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
-  float* part;               // [chunks][5][cols]
+  float* part;               // [chunks][5][cols]; walk: then [chunks][rows a block works on][cols], dscale's running sums
   long long rows;
   int cols, layer;
   float eps;
   long long groups, rows_per_group, rows_per_chunk, chunks_per_group;
+  int walk;                  // a chunk is rows_per_chunk rows of whole groups (rnorm_plan)
 };
 
 // Sum over groups of G = 8 to 64 neighbouring lanes, in every lane: neighbours, pairs, quads and eights through DPP, rows of 16 through
@@ -217,8 +218,9 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_fwd_kernel(RN
   }
 }
 
-// One block a chunk: rows_per_chunk consecutive rows of one gate group.  BIAS: a bias learns too (two more sums a column).
-template <typename T, int LANES, int EPL, bool VEC, bool BIAS>
+// One block a chunk: rows_per_chunk consecutive rows of one gate group, or (WALK) of many whole groups.  BIAS: a bias learns too (two
+// more sums a column).
+template <typename T, int LANES, int EPL, bool VEC, bool BIAS, bool WALK>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RNormParams p) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1, C = EPL / V;
   constexpr int RG = LANES > 256 ? 1 : 256 / LANES;        // rows a block works on
@@ -249,9 +251,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
   const long long first = group * p.rows_per_group + piece * p.rows_per_chunk;
   const long long last = min(first + p.rows_per_chunk, (group + 1) * p.rows_per_group);     // one past
   const bool full_gate = p.gate != nullptr && p.rows_per_group == 1;
+  const bool row_gate = full_gate || WALK;       // the gate is read with its row
   auto vectors_post = [&] {
     vector(sg, p.scale, 1.f); vector(ow, p.post_w, 1.f); vector(ob, p.post_b, 0.f);
-    if (p.gate != nullptr && !full_gate) {
+    if (p.gate != nullptr && !row_gate) {
       float g[EPL];
       vector(g, static_cast<const T*>(p.gate) + group * p.cols, 1.f);
 #pragma unroll
@@ -278,9 +281,23 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
   };
 
   // (a gate per element: the chunks of one row each would leave as many partial rows as there are rows, so there the host
-  // hands out chunks of several "groups" and the gate is read with its row)
-  const long long c_first = full_gate ? blockIdx.x * p.rows_per_chunk : first;
-  const long long c_last = full_gate ? min(c_first + p.rows_per_chunk, p.rows) : last;
+  // hands out chunks of several "groups" and the gate is read with its row; where groups of few rows are many (walk), so too, and
+  // each of the block's row lanes takes every RG'th group from its first row to its last: the group's gate gradient is then whole in its
+  // registers, and is written there and then)
+  const long long c_first = row_gate ? blockIdx.x * p.rows_per_chunk : first;
+  const long long c_last = row_gate ? min(c_first + p.rows_per_chunk, p.rows) : last;
+  const int t = (int)p.rows_per_group;             // (WALK: at most rows_per_chunk)
+  // WALK: this lane's columns of dscale's sum over the groups behind it (its own words: no one else reads or writes them)
+  float* const dscale_at = p.part + (long long)gridDim.x * 5 * p.cols + ((long long)blockIdx.x * RG + rg) * p.cols;
+  const bool dscale_sum = WALK && p.dscale != nullptr;
+  auto each_column = [&](auto f) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (in[c]) f(c * V + e, (c * LANES + lane) * V + e);
+  };
+  if (dscale_sum) each_column([&](int, int col) { dscale_at[col] = 0.f; });
   struct In { RowRaw<T, V, C> x, h, dout, du, g; float4 st; };
   auto fetch = [&](In& r, long long row) {
     row = min(row, c_last - 1);
@@ -291,16 +308,24 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
     else row_fill<T, V, C, LANES>(r.dout, 0.f);
     if (p.du != nullptr) row_load<T, V, C, LANES>(r.du, p.du, at, lane, p.cols);
     else row_fill<T, V, C, LANES>(r.du, 0.f);
-    if (full_gate) row_load<T, V, C, LANES>(r.g, p.gate, at, lane, p.cols);
+    if (row_gate) row_load<T, V, C, LANES>(r.g, p.gate, full_gate ? at : (long long)((unsigned)row / (unsigned)t) * p.cols, lane, p.cols);      // (rows <= 2^31)
     r.st = *reinterpret_cast<const float4*>(p.stats + row * 4);
   };
   In in_now, in_next;
-  if (AHEAD && c_first < c_last) fetch(in_now, c_first + rg);
-  for (long long r0 = c_first; r0 < c_last; r0 += RG) {
-    const bool live = r0 + rg < c_last;
-    const long long row = live ? r0 + rg : c_last - 1, at = row * p.cols;
-    if (!AHEAD) { fetch(in_now, r0 + rg); vectors_post(); vector(pw, p.pre_w, 1.f); }
-    else if (r0 + RG < c_last) fetch(in_next, r0 + RG + rg);          // (as in the forward kernel)
+  // WALK: a turn's row of this row lane, and its place in its group.  Every row lane takes as many turns as the first, which has the most
+  // rows: the sums hold barriers.
+  constexpr int STEP = WALK ? 1 : RG;
+  const long long from = WALK ? 0 : c_first, to = WALK ? ((c_last - c_first) / t + RG - 1) / RG * t : c_last;
+  long long walk_row = c_first + (long long)rg * t;
+  int in_group = 0;
+  if (AHEAD && c_first < c_last) fetch(in_now, WALK ? walk_row : c_first + rg);
+  for (long long r0 = from; r0 < to; r0 += STEP) {
+    const long long own = WALK ? walk_row : r0 + rg;
+    const bool live = own < c_last, group_ends = WALK && in_group == t - 1;
+    const long long row = live ? own : c_last - 1, at = row * p.cols;
+    if (WALK) { walk_row += group_ends ? 1 + (RG - 1ll) * t : 1; in_group = group_ends ? 0 : in_group + 1; }
+    if (!AHEAD) { fetch(in_now, own); vectors_post(); vector(pw, p.pre_w, 1.f); }
+    else if (r0 + STEP < to) fetch(in_next, WALK ? walk_row : r0 + RG + rg);          // (as in the forward kernel)
     const RowRaw<T, V, C>&xr = in_now.x, &hr = in_now.h, &dor = in_now.dout, &dur = in_now.du, &gr = in_now.g;
     const float4 st = in_now.st;
     // (behind the row's end x, h and the gradients are zeros: with a zero for 1 / deviation there, so is all that follows)
@@ -308,7 +333,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
 #pragma unroll
     for (int c = 0; c < C; ++c) { rstd1[c] = in[c] ? st.y : 0.f; rstd2[c] = in[c] ? st.w : 0.f; }
     // scale times the gate of this row
-    auto weight = [&](int e) { return full_gate ? sg[e] * (float)gr.p[e / V].v[e % V] : sg[e]; };
+    auto weight = [&](int e) { return row_gate ? sg[e] * (float)gr.p[e / V].v[e % V] : sg[e]; };
     float xh[EPL], rh[EPL], d[EPL];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -355,6 +380,17 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
         d[e] = dn * ow[e];
         s1 += d[e]; s2 = fmaf(d[e], xh[e], s2);
       }
+      if (live && group_ends) {       // the group is done: its dgate, and its part of dscale
+        float sum[EPL], dg[EPL];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          float& a = GATE < HELD ? held[(GATE * EPL + e) * LANES + lane] : acc[GATE][e];
+          sum[e] = a; a = 0.f;
+          dg[e] = sum[e] * sg[e];
+        }
+        if (p.dgate != nullptr) row_store<T, V, C, LANES>(p.dgate, (long long)((unsigned)row / (unsigned)t) * p.cols, dg, lane, p.cols);
+        if (dscale_sum) each_column([&](int e, int col) { dscale_at[col] = fmaf(sum[e], (float)gr.p[e / V].v[e % V], dscale_at[col]); });
+      }
       m = row_sum(s1, s2);
       m.x = p.layer ? m.x * inv : 0.f; m.y *= inv;
 #pragma unroll
@@ -373,6 +409,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
     float a[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) a[e] = sum < HELD ? held[(sum * EPL + e) * LANES + lane] : acc[sum][e];
+    if (WALK && sum == GATE) each_column([&](int e, int col) { a[e] = dscale_at[col]; });
     if (RG > 1) {                      // the block's row groups, added in order
       __syncthreads();
 #pragma unroll
@@ -393,7 +430,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rnorm_bwd_kernel(RN
         for (int e = 0; e < V; ++e) part[(long long)k * p.cols + col + e] = a[c * V + e];
     }
   };
-  if (p.dscale != nullptr || (p.dgate != nullptr && !full_gate)) flush(GATE, 0);
+  if (p.dscale != nullptr || (p.dgate != nullptr && !row_gate)) flush(GATE, 0);
   if (p.dpost_w != nullptr) flush(POST_W, 1);
   if constexpr (BIAS) if (p.dpost_b != nullptr) flush(POST_B, 2);
   if (p.dpre_w != nullptr) flush(PRE_W, 3);
@@ -407,7 +444,7 @@ __global__ __launch_bounds__(1024) void rnorm_sums_kernel(RNormParams p, long lo
   __shared__ float s[16][64];
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   const int col = blockIdx.x * 64 + tx, lc = min(col, p.cols - 1);
-  const bool grouped = p.gate != nullptr && p.rows_per_group > 1;
+  const bool grouped = p.gate != nullptr && p.rows_per_group > 1 && !p.walk;
   const T* gate = static_cast<const T*>(p.gate);
   auto column = [&](int k, long long from, long long to, bool weigh) -> float {       // valid in row lane 0
     float a = 0.f;
@@ -478,30 +515,43 @@ static int rnorm_bwd_launch(const RNormParams& p, bool vec, long long chunks, hi
   const dim3 grid((unsigned)chunks);
   const bool bias = p.dpost_b != nullptr || p.dpre_b != nullptr;
 #define RNORM_BWD_GO(L, E)                                                                                                        \
-  if (vec && bias) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, true>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);       \
-  else if (vec) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);         \
-  else if (bias) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, true>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);        \
-  else hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p)
+  if (p.walk && vec) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, true, true>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);  \
+  else if (p.walk) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, true, true>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);   \
+  else if (vec && bias) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, true, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);       \
+  else if (vec) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, true, false, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);         \
+  else if (bias) hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, true, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p);        \
+  else hipLaunchKernelGGL((rnorm_bwd_kernel<T, L, E, false, false, false>), grid, dim3((L) > 256 ? (L) : 256), 0, st, p)
   RNORM_BY_WIDTH(RNORM_BWD_GO);
   VEEX_CHECK_LAUNCH();
   if (p.dgate != nullptr || p.dscale != nullptr || p.dpost_w != nullptr || p.dpost_b != nullptr || p.dpre_w != nullptr || p.dpre_b != nullptr) {
-    const long long gate_rows = p.dgate != nullptr && p.rows_per_group > 1 ? std::min<long long>(p.groups, 1024) : 0;
+    const long long gate_rows = p.dgate != nullptr && p.rows_per_group > 1 && !p.walk ? std::min<long long>(p.groups, 1024) : 0;
     hipLaunchKernelGGL((rnorm_sums_kernel<T>), dim3((p.cols + 63) / 64, (unsigned)(5 + gate_rows)), dim3(1024), 0, st, p, chunks);
     VEEX_CHECK_LAUNCH();
   }
   return 0;
 }
 
-// rows of a chunk and chunks of a launch: about as many blocks as the chip holds, none across a group's end
-static long long rnorm_chunks(long long rows, int cols, long long groups, long long& per_chunk, long long& per_group) {
+// How the backward pass hands its rows out: about as many chunks as the chip holds blocks, none across a group's end.  Groups that are
+// many and small would leave a chunk each, and with it five partial rows to keep and to add (131072 rows of 1024 in 65536 groups: 1.3 GB
+// and 3.2 ms): there (walk) a chunk is a run of whole groups, RG of them at a time, one for each of the block's row lanes.  That takes
+// RG t rows a chunk, so it serves while they are not far more than a block's share (bf16 us, a chunk a group and walking: 131072x1024 in 65536
+// groups 3181 and 422, in 8192 664 and 333, 2080x1024 in 1040 57 and 21, 16384x8192 in 4096 1538 and 535; at twice the share, 65536x128 in 4096,
+// 142 and 40; at four times 65536x64 in 4096 146 and 36, 524288x64 in 4096 209 and 246, fp32 352 and 283; at eight times 524288x64 in 2048 152 and
+// 465).  So there are at most 512 (RG / 4 + 1) partial rows, whatever the groups.
+struct RNormPlan { long long chunks, rows_per_chunk, chunks_per_group; int walk; };
+
+static RNormPlan rnorm_plan(long long rows, int cols, long long groups) {
   const long long t = rows / groups, blocks = cols > 2048 ? 256 : 512;       // (resident at once: 8 waves a CU)
-  const long long want = std::max<long long>((rows + blocks - 1) / blocks, std::max(4, rnorm_rows_per_block(cols)));
-  if (groups == rows) { per_chunk = want; per_group = 1; return (rows + want - 1) / want; }   // (a gate per element, or one row)
-  per_group = (t + want - 1) / want;
-  per_chunk = (t + per_group - 1) / per_group;
-  per_group = (t + per_chunk - 1) / per_chunk;
-  return per_group * groups;
+  const int rg = rnorm_rows_per_block(cols);
+  const long long want = std::max<long long>((rows + blocks - 1) / blocks, std::max(4, rg));
+  if (groups == rows) return {(rows + want - 1) / want, want, 1, 0};          // (a gate per element, or one row)
+  const long long per_group = (t + want - 1) / want, per_chunk = (t + per_group - 1) / per_group, of_group = (t + per_chunk - 1) / per_chunk;
+  if (of_group * groups <= 2 * blocks || t * rg > 4 * want) return {of_group * groups, per_chunk, of_group, 0};
+  const long long run = ((want + t - 1) / t + rg - 1) / rg * rg;              // groups of a chunk
+  return {(groups + run - 1) / run, run * t, 1, 1};
 }
+
+static long long rnorm_workspace(const RNormPlan& q, int cols) { return q.chunks * (5 + (q.walk ? rnorm_rows_per_block(cols) : 0)) * cols; }
 
 static bool rnorm_struct_ok(const VeexResidualNorm* d) {
   if (d != nullptr && (d->struct_size == 0 || d->struct_size == (int)sizeof(VeexResidualNorm))) return true;
@@ -530,7 +580,7 @@ static void rnorm_fill(RNormParams& p, const VeexResidualNorm* d) {
   p.rows = d->rows; p.cols = d->cols; p.layer = d->kind == VEEX_NORM_LAYER; p.eps = d->eps;
   p.groups = p.gate != nullptr ? d->groups : 1;
   p.rows_per_group = std::max<long long>(d->rows / p.groups, 1);
-  p.rows_per_chunk = p.chunks_per_group = 1;
+  p.rows_per_chunk = p.chunks_per_group = 1; p.walk = 0;
 }
 
 extern "C" {
@@ -555,8 +605,7 @@ int veex_residual_norm_fwd(const VeexResidualNorm* d, hipStream_t st) {
 long long veex_residual_norm_bwd_workspace_floats(long long rows, int cols, long long groups) {
   if (rows < 0 || cols < 1 || groups < 1 || (rows > 0 && rows % groups != 0)) return -1;
   if (rows == 0) return 0;
-  long long a, b;
-  return rnorm_chunks(rows, cols, groups, a, b) * 5 * cols;
+  return rnorm_workspace(rnorm_plan(rows, cols, groups), cols);
 }
 
 int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
@@ -569,9 +618,11 @@ int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
   RNormParams p;
   rnorm_fill(p, d);
   p.x_out = p.u = nullptr;
-  const long long chunks = rnorm_chunks(p.rows, p.cols, p.groups, p.rows_per_chunk, p.chunks_per_group);
-  if (d->workspace_floats < chunks * 5 * p.cols) { veex_set_error("residual_norm backward: workspace of %lld floats is needed", chunks * 5 * p.cols); return VEEX_ENOMEM; }
-  if (!trunk_grid_ok(chunks, 1024)) { veex_set_error("residual_norm backward: more gate groups than a launch takes"); return VEEX_EINVAL; }
+  const RNormPlan plan = rnorm_plan(p.rows, p.cols, p.groups);
+  const long long chunks = plan.chunks, need = rnorm_workspace(plan, p.cols);
+  p.rows_per_chunk = plan.rows_per_chunk; p.chunks_per_group = plan.chunks_per_group; p.walk = plan.walk;
+  if (d->workspace_floats < need) { veex_set_error("residual_norm backward: workspace of %lld floats is needed", need); return VEEX_ENOMEM; }
+  if (p.groups != p.rows && p.groups >= (1 << 22)) { veex_set_error("residual_norm backward: 2^22 gate groups or more"); return VEEX_EINVAL; }
   const bool vec = rnorm_vec(p, d->dtype);
   if (d->dtype == VEEX_T_F32) return rnorm_bwd_launch<float>(p, vec, chunks, st);
   if (d->dtype == VEEX_T_BF16) return rnorm_bwd_launch<bf16_t>(p, vec, chunks, st);
