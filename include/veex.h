@@ -305,14 +305,15 @@ int veex_dense_bwd(const VeexDense* d, veexStream_t s);
 #define VEEX_NORM_LAYER 0
 #define VEEX_NORM_RMS 1
 #define VEEX_NORM_MAX_COLS 16384
+#define VEEX_NORM_MAX_GROUPS (1 << 22)     /* a call that trains: groups < this, or = rows */
 
 /* x_out = x + scale gate Norm(h; post_w, post_b), u = Norm(x_out; pre_w, pre_b); with h NULL: u = Norm(x; pre_w, pre_b).
  * Norm: (v - mean) / sqrt(var + eps) * w + b over the row (LAYER), v / sqrt(mean(v^2) + eps) * w + b (RMS); NULL weights
  * and biases are 1 and 0.  gate [groups][cols], row g for rows/groups consecutive rows of x; scale [cols]; both may be NULL (1).
  * stats [rows][4] fp32, 16-byte aligned: written by the forward when not NULL, read by the backward.
  * Backward: gradients of whatever output pointer is not NULL, from dx_out and du (NULL: zero); workspace of
- * veex_residual_norm_bwd_workspace_floats(rows, cols, groups) floats (groups = 1 without gate or h); rows >= 1; up to 2^22
- * groups, or one a row. */
+ * veex_residual_norm_bwd_workspace_floats(rows, cols, groups) floats (groups = 1 without gate or h); rows >= 1.  A call that trains (a
+ * forward with stats, a backward) takes fewer than VEEX_NORM_MAX_GROUPS groups, or one a row. */
 typedef struct VeexResidualNorm {
   const void* x; const void* h; const void* gate; const void* scale;
   const void* post_w; const void* post_b; const void* pre_w; const void* pre_b;

@@ -1,4 +1,6 @@
-"""residual_norm with a gate of many small groups: its values and gradients and the workspace of its backward pass."""
+"""residual_norm with a gate of many small groups: its values and gradients, the workspace of its backward pass, and where it ends."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -27,6 +29,21 @@ def test_workspace_does_not_grow_with_the_groups(rows, cols):
         floats = _lib.lib.veex_residual_norm_bwd_workspace_floats(rows, cols, groups)
         assert 0 < floats <= 5 * (_lanes(cols) + 1) * blocks * cols, groups
     assert _lib.lib.veex_residual_norm_bwd_workspace_floats(131072, 1024, 65536) * 4 < 16 << 20        # 1.3 GB with a partial row a group
+
+
+def test_a_training_forward_refuses_what_the_backward_would(ops):
+    from vae_eeg_xai_amd import _lib
+    q = _lib.ResidualNormDesc()
+    q.struct_size = C.sizeof(q)
+    q.rows, q.cols, q.groups, q.eps = 1 << 23, 8, 1 << 22, 1e-3
+    q.x = q.h = q.gate = q.x_out = q.u = q.stats = 1 << 20        # never dereferenced
+    assert _lib.lib.veex_residual_norm_fwd(C.byref(q), None) == -1 and "groups" in _lib.lib.veex_last_error().decode()
+    x, gate = torch.zeros(1 << 23, 1), torch.zeros(1 << 22, 1)
+    for k in range(3):
+        t = [x, x, gate]
+        t[k] = t[k].clone().requires_grad_()
+        with pytest.raises(ValueError, match="groups"):
+            ops.residual_norm(*t)
 
 
 # widths that take 8 lanes to 16 waves a row, whole and odd; a last run that is not full; row lanes without a group

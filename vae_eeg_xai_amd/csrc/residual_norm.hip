@@ -559,11 +559,12 @@ static bool rnorm_struct_ok(const VeexResidualNorm* d) {
   return false;
 }
 
-static int rnorm_check(const char* who, long long rows, int cols, long long groups, int dtype, int kind, double eps) {
+static int rnorm_check(const char* who, long long rows, int cols, long long groups, int dtype, int kind, double eps, bool train) {
   if (!trunk_dtype_ok(dtype) || (kind != VEEX_NORM_LAYER && kind != VEEX_NORM_RMS)) { veex_set_error("%s: unknown dtype or kind", who); return VEEX_EINVAL; }
   if (rows < 0 || cols < 1 || cols > VEEX_NORM_MAX_COLS) { veex_set_error("%s: rows >= 0 and 1 <= cols <= %d are needed", who, VEEX_NORM_MAX_COLS); return VEEX_EINVAL; }
   if (rows > (1ll << 31)) { veex_set_error("%s: at most 2^31 rows", who); return VEEX_EINVAL; }
   if (groups < 1 || (rows > 0 && rows % groups != 0)) { veex_set_error("%s: the gate's groups have to divide the rows", who); return VEEX_EINVAL; }
+  if (train && groups != rows && groups >= VEEX_NORM_MAX_GROUPS) { veex_set_error("%s: in training a gate has fewer than 2^22 groups, or one a row", who); return VEEX_EINVAL; }
   if (!(eps >= 0.0)) { veex_set_error("%s: eps has to be >= 0", who); return VEEX_EINVAL; }
   return 0;
 }
@@ -591,7 +592,7 @@ int veex_residual_norm_fwd(const VeexResidualNorm* d, hipStream_t st) {
     veex_set_error("residual_norm: x and u (with h also x_out) are needed"); return VEEX_EINVAL;
   }
   if (!trunk_aligned16(d->stats)) { veex_set_error("residual_norm: stats has to be 16-byte aligned"); return VEEX_EINVAL; }
-  if (int rc = rnorm_check("residual_norm", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps)) return rc;
+  if (int rc = rnorm_check("residual_norm", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps, d->stats != nullptr)) return rc;
   if (d->rows == 0) return 0;
   RNormParams p;
   rnorm_fill(p, d);
@@ -613,7 +614,7 @@ int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
   if (d->x == nullptr || d->stats == nullptr || !trunk_aligned16(d->stats) || d->workspace == nullptr) {
     veex_set_error("residual_norm backward: x, 16-byte aligned stats and workspace are needed"); return VEEX_EINVAL;
   }
-  if (int rc = rnorm_check("residual_norm backward", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps)) return rc;
+  if (int rc = rnorm_check("residual_norm backward", d->rows, d->cols, d->gate != nullptr ? d->groups : 1, d->dtype, d->kind, d->eps, true)) return rc;
   if (d->rows == 0) { veex_set_error("residual_norm backward: no rows"); return VEEX_EINVAL; }
   RNormParams p;
   rnorm_fill(p, d);
@@ -622,7 +623,6 @@ int veex_residual_norm_bwd(const VeexResidualNorm* d, hipStream_t st) {
   const long long chunks = plan.chunks, need = rnorm_workspace(plan, p.cols);
   p.rows_per_chunk = plan.rows_per_chunk; p.chunks_per_group = plan.chunks_per_group; p.walk = plan.walk;
   if (d->workspace_floats < need) { veex_set_error("residual_norm backward: workspace of %lld floats is needed", need); return VEEX_ENOMEM; }
-  if (p.groups != p.rows && p.groups >= (1 << 22)) { veex_set_error("residual_norm backward: 2^22 gate groups or more"); return VEEX_EINVAL; }
   const bool vec = rnorm_vec(p, d->dtype);
   if (d->dtype == VEEX_T_F32) return rnorm_bwd_launch<float>(p, vec, chunks, st);
   if (d->dtype == VEEX_T_BF16) return rnorm_bwd_launch<bf16_t>(p, vec, chunks, st);

@@ -436,6 +436,8 @@ std::tuple<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& h_in,
   bool grad = false;
   for (const Tensor& v : t) grad = grad || learns(v);
   if (grad && at::GradMode::is_enabled()) {
+    TORCH_CHECK_VALUE(groups < VEEX_NORM_MAX_GROUPS || groups == rows_of(x), "residual_norm: gate ", gate.sizes(), " for x ", x.sizes(),
+                      " in training; it takes fewer than 2^22 groups, or one a row");
     const auto r = ResidualNorm::apply(x, h_in, gate_in, scale, post_w, post_b, pre_w, pre_b, groups, code, eps);
     return {h.defined() ? r[0] : x, r.back()};
   }
