@@ -122,38 +122,104 @@ __device__ __forceinline__ void dt_wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// the 32 rows from `row` on that a tensor of `rows` has, as bits
+__device__ __forceinline__ unsigned dt_rows_in(long long row, long long rows) {
+  return rows - row >= 32 ? ~0u : rows <= row ? 0u : (1u << (rows - row)) - 1u;
+}
+
+// Which of the 32 rows of a packed operand from `row` on hold a NaN among the k's of [k_begin, k_end): a bit each, the same in every lane.
+// (The first plane says it: a value that is not finite is its first term alone.  Rows and k's lie in pieces of 8, padded with zeros.)
+template <bool KC>
+__device__ __forceinline__ unsigned dt_nan_rows(const DtTensor& t, long long row, long long rows, long long k_begin, long long k_end, int lane) {
+  const long long own = KC ? row + (lane & 31) : row + 8 * (lane & 3);
+  const int step = 16, k0 = KC ? 8 * (lane >> 5) : lane >> 2;       // 16 k's a turn
+  const char* p = static_cast<const char*>(t.p) + (KC ? own * t.ld_bytes : own * 2);
+  const unsigned all = dt_rows_in(row, rows);
+  unsigned found = 0u;
+  for (long long k = k_begin; k < k_end && (found & all) != all; k += 4 * step) {
+    unsigned mine = 0u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const long long at = k + q * step + k0;
+      if (own < rows && at < k_end) {
+        const Piece<bf16_t, 8> x = piece_load<bf16_t, 8>(reinterpret_cast<const bf16_t*>(p + (KC ? at * 2 : at * t.ld_bytes)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine |= (float)x.v[e] != (float)x.v[e] ? 1u << (KC ? 0 : e) : 0u;
+      }
+    }
+    if (KC) {
+      const unsigned long long b = __ballot(mine != 0u);
+      found |= (unsigned)b | (unsigned)(b >> 32);
+    } else {
+#pragma unroll
+      for (int o = 4; o < 64; o <<= 1) mine |= __shfl_xor(mine, o);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) found |= __shfl(mine, q) << (8 * q);
+    }
+  }
+  return found;
+}
+
 // Split operands and infinities: an infinite operand times the other's lower terms gives NaN where fp32 gives an infinity.  A 32 x 32
-// block that holds a NaN is computed again with the fp32 MFMA from the terms' sums (which are the operands to 2^-27, and exactly them
-// where they are not finite), and its NaN elements take those values.  Finite data never come here.
+// block that holds such a NaN is computed again with the fp32 MFMA from the terms' sums (which are the operands to 2^-27, and exactly them
+// where they are not finite), and its NaN elements take those values.  A NaN that its row of A or its column of B explains stays: a run that
+// has diverged to NaN looks for them and computes nothing again (4096x1024x1024 forward: x all NaN 59 us for 62 without, w all NaN 94; an infinity
+// in each row of x, where all of it is computed again, 418).  Finite data come here only where partial products overflow to opposite
+// infinities.
 template <bool AKC, bool BKC, int MT, int NT>
 __device__ __forceinline__ void dt_mend(const DtGemm& g, f32x16 (&acc)[MT][NT], long long i0, int j0, long long k_begin, long long k_end, int lane) {
   const int l31 = lane & 31, lh = lane >> 5;
-  auto value = [](const DtTensor& t, bool kc, long long row, long long k) -> float {
-    const char* p = static_cast<const char*>(t.p) + (kc ? row * t.ld_bytes + k * 2 : k * t.ld_bytes + row * 2);
-    return (float)*reinterpret_cast<const bf16_t*>(p) + (float)*reinterpret_cast<const bf16_t*>(p + t.plane_bytes) +
-           (float)*reinterpret_cast<const bf16_t*>(p + 2 * t.plane_bytes);
+  // the terms' sums of the 8 k's from k on, of one row (elements outside read the tensor's first one, so that all loads are on their way at once)
+  auto values = [&](const DtTensor& t, bool kc, long long row, bool in, long long k, float (&v)[8]) {
+    const bf16_t* const safe = static_cast<const bf16_t*>(t.p);
+    const long long ld = t.ld_bytes / 2, plane = t.plane_bytes / 2;
+    bf16_t x[3][8];
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl) {
+      if (kc) {
+        const Piece<bf16_t, 8> y = piece_load<bf16_t, 8>(in && k < k_end ? safe + row * ld + k + pl * plane : safe);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[pl][e] = y.v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[pl][e] = *(in && k + e < k_end ? safe + (k + e) * ld + row + pl * plane : safe);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = in && (kc ? k : k + e) < k_end ? (float)x[0][e] + (float)x[1][e] + (float)x[2][e] : 0.f;
   };
 #pragma unroll
   for (int mi = 0; mi < MT; ++mi)
 #pragma unroll
     for (int nj = 0; nj < NT; ++nj) {
-      bool nan = false;
+      // this lane's elements of the block are row i0 + 32 mi + l31, columns j0 + 32 nj + 8 (r / 4) + 4 lh + r % 4
+      unsigned nan = 0u;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) nan |= acc[mi][nj][r] != acc[mi][nj][r];
-      if (!__any(nan)) continue;
-      const long long i = i0 + mi * 32 + l31;
-      const int j = j0 + nj * 32 + l31;
+      for (int r = 0; r < 16; ++r) nan |= acc[mi][nj][r] != acc[mi][nj][r] ? 1u << r : 0u;
+      if (!__any(nan != 0u)) continue;
+      const long long row = i0 + mi * 32, i = row + l31;
+      const int col = j0 + nj * 32, j = col + l31;
+      const unsigned rows = ~dt_rows_in(row, g.I) | dt_nan_rows<AKC>(g.a, row, g.I, k_begin, k_end, lane);
+      if ((rows >> l31 & 1u) != 0u) nan = 0u;
+      if (!__any(nan != 0u)) continue;
+      const unsigned cols = ~dt_rows_in(col, g.J) | dt_nan_rows<BKC>(g.b, col, g.J, k_begin, k_end, lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if ((cols >> (8 * (r / 4) + 4 * lh + r % 4) & 1u) != 0u) nan &= ~(1u << r);
+      if (!__any(nan != 0u)) continue;
       f32x16 s;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll 1
-      for (long long k = k_begin; k < k_end; k += 2) {
-        const bool in = k + lh < k_end;
-        const float av = in && i < g.I ? value(g.a, AKC, i, k + lh) : 0.f, bv = in && j < g.J ? value(g.b, BKC, j, k + lh) : 0.f;
-        s = __builtin_amdgcn_mfma_f32_32x32x2f32(bv, av, s, 0, 0, 0);
+      for (long long k = k_begin; k < k_end; k += 16) {      // lane half lh holds the k's k + 8 lh .. + 7
+        float av[8], bv[8];
+        values(g.a, AKC, i, i < g.I, k + 8 * lh, av);
+        values(g.b, BKC, j, j < g.J, k + 8 * lh, bv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(bv[e], av[e], s, 0, 0, 0);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[mi][nj][r] = acc[mi][nj][r] != acc[mi][nj][r] ? s[r] : acc[mi][nj][r];
+      for (int r = 0; r < 16; ++r) acc[mi][nj][r] = (nan >> r & 1u) != 0u ? s[r] : acc[mi][nj][r];
     }
 }
 
