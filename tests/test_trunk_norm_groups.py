@@ -104,3 +104,18 @@ def test_a_batch_entrys_gate_for_two_tokens(ops):
         # (the first four: the same arithmetic in another kernel; dgate: two terms; dscale: 6 000 terms in another order)
         terms = 6000 if k == 5 else 8
         assert float((a - b).abs().max()) <= 4 * terms ** 0.5 * ref.U * 8 * float(b.abs().max()), k
+
+
+@pytest.mark.gpu
+def test_low_level_ops_refuse_a_gate_that_does_not_fit(ops):
+    """A gate without rows beside an x with some is an error, not a missing gate; so are no groups."""
+    x, none = torch.zeros(4, 8, device="cuda"), torch.zeros(0, 8, device="cuda")
+    stats = torch.zeros(4, 4, device="cuda")
+    rest = [None] * 5
+    for gate, groups in ((none, 1), (none, 4), (None, 0), (x, 0), (x[:3], 3), (x[:2], 4)):
+        with pytest.raises(ValueError):
+            ops.residual_norm_fwd(x, x, gate, *rest, groups, 0, 1e-3, False)
+        with pytest.raises(ValueError):
+            ops.residual_norm_bwd(x, x, gate, *rest, groups, 0, 1e-3, stats, x, x, [True] * 8)
+    out, u, _ = ops.residual_norm_fwd(none, none, none, *rest, 1, 0, 1e-3, True)        # no rows at all: nothing to do
+    assert out.shape == (0, 8) and u.shape == (0, 8)

@@ -301,7 +301,8 @@ void check_norm_args(const Tensor (&t)[8], int64_t groups, double eps) {
   TORCH_CHECK_VALUE(!t[1].defined() || t[1].sizes() == x.sizes(), "residual_norm: h (", t[1].sizes(), ") is not of x's shape ", x.sizes());
   for (int i = 3; i < 8; ++i)
     TORCH_CHECK_VALUE(!t[i].defined() || (t[i].dim() == 1 && t[i].size(0) == x.size(-1)), "residual_norm: ", names[i], " ", t[i].sizes(), " is not (", x.size(-1), ",)");
-  TORCH_CHECK_VALUE(groups >= 1 && (!t[2].defined() || t[2].numel() == 0 || (t[2].numel() == groups * x.size(-1) && rows_of(x) % groups == 0)),
+  TORCH_CHECK_VALUE(groups >= 1, "residual_norm: a gate of ", groups, " groups");
+  TORCH_CHECK_VALUE(!t[2].defined() || rows_of(x) == 0 || (t[2].numel() == groups * x.size(-1) && rows_of(x) % groups == 0),
                     "residual_norm: gate ", t[2].sizes(), " does not go with x ", x.sizes());
 }
 
