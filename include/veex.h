@@ -301,6 +301,15 @@ long long veex_dense_fwd_workspace_bytes(const VeexDense* d);
 int veex_dense_fwd(const VeexDense* d, veexStream_t s);
 long long veex_dense_bwd_workspace_bytes(const VeexDense* d);
 int veex_dense_bwd(const VeexDense* d, veexStream_t s);
+/* Host only: which kernels the call that d describes takes for a product (0: y, 1: dx, 2: dw): one of VEEX_DENSE_*, plus 256 times the number of blocks
+ * that its reduction is split over; -1: bad.  Goes by sizes, type, ldx and the pointers' alignment; for tests and tuning. */
+#define VEEX_DENSE_GENERAL 0         /* 64x64 tiles, fp32 matrix cores, any strides */
+#define VEEX_DENSE_FEW 1             /* few rows */
+#define VEEX_DENSE_FEW_SHORT 2       /* few rows, short columns: one launch */
+#define VEEX_DENSE_TILE_256X256 3    /* 16-bit matrix cores */
+#define VEEX_DENSE_TILE_256X128 4
+#define VEEX_DENSE_TILE_128X128 5
+int veex_dense_plan(const VeexDense* d, int product);
 
 #define VEEX_NORM_LAYER 0
 #define VEEX_NORM_RMS 1

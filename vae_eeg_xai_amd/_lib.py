@@ -134,6 +134,7 @@ SIGNATURES = {
     "veex_column_medians": (_I, [_P, _I, _I, _P, _P, _P]),
     "veex_band_outside_counts": (_I, [_P, _I, _I, _I, _P, _P, _P, _P]),
     "veex_dropout": (_I, [_P, _P, _P, _L, _I, _I, _D, _U, _U, _P, _P]),
+    "veex_dense_plan": (_I, [C.POINTER(DenseDesc), _I]),
     "veex_dense_fwd_workspace_bytes": (_L, [C.POINTER(DenseDesc)]),
     "veex_dense_fwd": (_I, [C.POINTER(DenseDesc), _P]),
     "veex_dense_bwd_workspace_bytes": (_L, [C.POINTER(DenseDesc)]),

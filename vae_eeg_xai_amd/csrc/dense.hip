@@ -796,6 +796,27 @@ static BwdLayout bwd_layout(const VeexDense* d, const DropArgs& drop) {
 
 extern "C" {
 
+int veex_dense_plan(const VeexDense* d, int product) {
+  DropArgs drop;
+  if (dense_check(d, "dense", drop) != 0) return -1;
+  if (product < kKindFwd || product > kKindDw || d->rows == 0) { veex_set_error("dense: product 0 (y), 1 (dx) or 2 (dw), and rows, are needed"); return -1; }
+  const DenseGemm g = dense_product(product, d, nullptr);
+  if (product == kKindFwd && few_rows(d)) {
+    const int elem = trunk_elem_bytes(d->dtype);
+    if (few_short(g, elem)) return VEEX_DENSE_FEW_SHORT | 1 << 8;
+    int s; long long per;
+    few_split(g, operand_vec(g.b, g.J, elem), elem, s, per);
+    return VEEX_DENSE_FEW | s << 8;
+  }
+  if (!uses_tiles(d)) {
+    int s; long long per;
+    general_split(g.I, g.J, g.K, s, per);
+    return VEEX_DENSE_GENERAL | s << 8;
+  }
+  const TilePlan t = tile_plan(d, g.I, g.J, g.K);
+  return (t.tile == 0 ? VEEX_DENSE_TILE_256X256 : t.tile == 1 ? VEEX_DENSE_TILE_256X128 : VEEX_DENSE_TILE_128X128) | (int)t.splits << 8;
+}
+
 long long veex_dense_fwd_workspace_bytes(const VeexDense* d) {
   DropArgs drop;
   if (dense_check(d, "dense", drop) != 0) return -1;
