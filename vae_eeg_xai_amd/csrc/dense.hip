@@ -563,9 +563,10 @@ static int general_grads_launch(const DenseGemm (&g)[2], hipStream_t st) {
   if (!trunk_grid_ok(n0 + n1, 256)) return too_many_tiles();
   const bool vec = (n0 == 0 || general_vec(kKindDx, g[0], sizeof(T))) && (n1 == 0 || general_vec(kKindDw, g[1], sizeof(T)));
   const dim3 grid((unsigned)(n0 + n1));
-  // dx's blocks come first, unless those of dw take over four times as long: started last they would run on alone (2048x6400x100 fp32
-  // backward 105 us, 84 with dw first; 512x6400x100, twice as long, 34 and 37)
-  const bool dw_first = n0 == 0 || (n1 > 0 && g[1].k_per_split > 4 * g[0].k_per_split);
+  // dx's blocks come first, unless those of dw take over twice as long: started last they would run on alone (fp32 backward us, dx first and
+  // dw first: dw's blocks three times as long, 3000x1500x150 60 and 54, 1024x4096x150 53 and 46; eight times, 2048x6400x100 104 and 82; twice,
+  // 512x6400x100 30 and 33, 2048x2048x100 36 and 34; a tenth, 128x4096x4096 93 and 98, 64x4096x14336 179 and 206)
+  const bool dw_first = n0 == 0 || (n1 > 0 && g[1].k_per_split > 2 * g[0].k_per_split);
   const unsigned dx_from = dw_first ? (unsigned)n1 : 0u, dw_from = dw_first ? 0u : (unsigned)n0;
   if (vec) hipLaunchKernelGGL((dense_general_grads_kernel<T, true>), grid, dim3(256), 0, st, g[0], g[1], (unsigned)t0, (unsigned)t1, dx_from, dw_from);
   else hipLaunchKernelGGL((dense_general_grads_kernel<T, false>), grid, dim3(256), 0, st, g[0], g[1], (unsigned)t0, (unsigned)t1, dx_from, dw_from);
