@@ -283,8 +283,13 @@ int veex_dropout(const void* x, const void* residual, void* y, long long rows, i
  * Backward: dz = D'(dy) act'(z), dx = dz w^T, dw = x^T dz, db = column sums of dz; each of dx, dw, db may be NULL.  pre is what
  * the forward wrote there; for VEEX_ACT_RELU without residual it may be the forward's y instead (y > 0 exactly where an element
  * was kept and z > 0), for VEEX_ACT_NONE it is not read.  d(residual) is dy.
- * rows <= 2^31, k and n <= 2^30, and a launch takes 2^24 tiles of 64 x 64 (VEEX_EINVAL beyond).  Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned,
- * of at least the bytes that the _workspace function of the direction returns for the same struct (host only; -1: bad). */
+ * rows <= 2^31, k and n <= 2^30, and a launch takes fewer than 2^24 tiles of 64 x 64 times the blocks that share a reduction (dx and dw
+ * together), or, where the matrix-core tiles serve (veex_dense_plan), fewer than 2^22 of those a product; VEEX_EINVAL beyond.
+ * 16-bit types: besides y, dx, dw and db, z (pre) and dz are rounded to the type (fp16's dz times a constant that keeps a finite dy finite); sums
+ * are fp32, db one over the unrounded dz.  Activations are
+ * evaluated with the hardware's exp2 and reciprocal (1 ulp of fp32).  fp32: large products are six bf16 ones (an error of 2^-25 of each term beside the
+ * sum's own; operands below about 2^-110 keep fewer bits).
+ * Zero-initialise the struct; set struct_size = sizeof(VeexDense).  workspace: caller-owned device memory, 16-byte aligned, of at least the bytes that the _workspace function of the direction returns for the same struct (host only; -1: bad). */
 typedef struct VeexDense {
   const void* x; const void* w; const void* bias; const void* residual;
   void* y; void* pre;

@@ -11,7 +11,7 @@
 // there, so one kernel serves every type).  Operand tiles are staged through registers into [k][row] LDS; a tensor whose rows
 // are whole aligned pieces loads 8 elements at a time, others element by element.  The MFMA takes B's rows as its first operand, so
 // that a lane ends up with 4 consecutive columns of one row.
-// Bound: the fp32 MFMA in long reductions (1024x4096x4096 fp32 108 TFLOP/s, 128x4096x4096 84; a large library product 153), and in
+// Bound: the fp32 MFMA in long reductions (128x4096x4096 fp32 83 TFLOP/s, 64x4096x14336 76; a large library product 153), and in
 // small layers the way in and out of a tile: 512x28x4096 fp32 6.6 us, 512x6400x100 16 us and 5 for the join of its 32 splits.
 // ---------------------------------------------------------------------------------------------------------------
 #define DG_LD 68     // floats per LDS row: 64 + one 16-byte piece

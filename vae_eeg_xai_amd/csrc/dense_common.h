@@ -22,7 +22,8 @@ struct DenseEpi {
 // A 16-bit result keeps 11 bits at most, so there the hardware's exp2 and reciprocal (1 ulp) serve; fp32 takes the accurate expf
 // and division.  gelu needs Phi(z) = erfc(-z / sqrt 2) / 2: with x = |z| / sqrt 2 and t = 1 / (1 + p x), erfc(x) = P(t) t exp(-x^2), P
 // fitted here to exp(x^2) erfc(x) / t on 0 <= x <= 9.5 for the least largest relative error (7.3e-7 with 7 coefficients, 1.7e-8
-// with 9; fp32 rounding brings the latter to 3.5e-7).  The derivative's exp(-z^2 / 2) is the same exponential.
+// with 9).  In fp32 all of Phi(z) is off by up to 6e-7 for z > -4, and further down by what the rounding of z^2 does to exp(-z^2 / 2): 1.3e-6 to
+// -8, 4e-6 at -12 (against Phi 1e-15 and 1e-33).  The derivative's exp(-z^2 / 2) is the same exponential.
 template <typename T> __device__ __forceinline__ float act_exp(float x) {
   if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(x * 1.44269504f);
   else return expf(x);

@@ -10,9 +10,11 @@
 //
 // Bound: HBM.  A row lives in the registers of 8 lanes to 16 waves (8 or 16 elements a lane), so the forward pass reads x, h and
 // gate once and writes x_out and u once; the backward pass recomputes x_out from x and h in fp32 instead of reading the
-// rounded one (the same bytes, and the gradient is that of the unrounded chain).  8192x4096 bf16: forward 50 us (5.4 TB/s),
-// backward 91 us with its column sums (4.4 TB/s); fp32 99 and 131 us (5.4 and 6.2 TB/s; a copy of 1 GB runs at 4.9).  All statistics and sums are fp32; the
-// variance is the mean of squared deviations (two passes over registers), not a difference of moments.
+// rounded one (the same bytes, and the gradient is that of the unrounded chain).  8192x4096 bf16 with a gate of 8 groups: forward 58 us
+// (4.6 TB/s), backward 104 us and 10 for its column sums (3.5 TB/s); fp32, the same call again and again, 98 and 174 us (5.5 and 4.6 TB/s); a copy
+// of 1 GB runs at 4.9.  (Where a comment below gives two times of a backward pass, x and h stood for dx_out and du too: a third fewer
+// bytes.)  All statistics and sums are fp32; the variance is the mean of squared deviations (two passes over registers), not a
+// difference of moments.
 // Column sums: each block adds up its own run of rows in registers, writes one partial row per sum, and a second kernel adds
 // the partial rows in a fixed order: no atomics, the same bits every time.
 #include "trunk_common.h"
@@ -480,7 +482,7 @@ __global__ __launch_bounds__(1024) void rnorm_sums_kernel(RNormParams p, long lo
 
 // lanes a row: the fewest that hold it at 8 elements each, from 8 to 16 waves (65536 rows of 64 columns, fp32: 64 lanes a row 34 us
 // forward and 63 backward, 8 lanes 12 and 37; of 128: 35 and 63, 16 lanes 21 and 38); wider rows take 16 elements a lane, and some
-// spilled registers (16384 columns, 2048 rows, bf16: 110 and 344 us, 2.4 and 1.2 TB/s).  GO(lanes, elements)
+// spilled registers (16384 columns, 2048 rows, bf16: 117 and 437 us, 2.3 and 0.9 TB/s).  GO(lanes, elements)
 #define RNORM_BY_WIDTH(GO)                                                                              \
   do {                                                                                                  \
     if (p.cols <= 64) { GO(8, 8); } else if (p.cols <= 128) { GO(16, 8); } else if (p.cols <= 256) { GO(32, 8); }     \

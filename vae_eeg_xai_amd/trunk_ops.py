@@ -12,7 +12,13 @@
         16384 columns.  gate: one row of N for all of x ((N,)), one for each of x's leading indices ((B, N) or (B, 1, N) for
         x (B, T, N)), or x's shape; for a two-dimensional x also (G, N) with G dividing the rows, row r taking gate[r // (rows / G)].
 
-float32, bfloat16 and float16, one type for all tensors of a call; sums and statistics are fp32 inside.  All are differentiable
+float32, bfloat16 and float16, one type for all tensors of a call; sums and statistics are fp32 inside.  In 16-bit types dense
+rounds two more things than its results: z = x w + bias is kept for the backward pass in the type, as separate layers would keep
+it, and dz = D'(dy) act'(z) goes into the products dx = dz w^T and dw = x^T dz in it (their error is that of two roundings, 1.4 times
+that of one; db sums the unrounded dz).  Large float32 products are made of bf16 terms, to float32's rounding; operands below about
+1e-33 keep fewer bits there.  A gate that learns has fewer than 2^22 rows, or one for each row of x.
+
+All are differentiable
 once (dropout any number of times) in every tensor but ``counter``, in reverse mode: a tensor with a forward-mode tangent
 (torch.func.jvp, forward_ad.make_dual) is refused with NotImplementedError.
 
