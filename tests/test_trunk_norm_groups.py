@@ -103,6 +103,7 @@ def test_a_batch_entrys_gate_for_two_tokens(ops):
     for k, (a, b) in enumerate(zip(few, full)):
         # (the first four: the same arithmetic in another kernel; dgate: two terms; dscale: 6 000 terms in another order)
         terms = 6000 if k == 5 else 8
+        a, b = a.detach(), b.detach()
         assert float((a - b).abs().max()) <= 4 * terms ** 0.5 * ref.U * 8 * float(b.abs().max()), k
 
 
@@ -119,3 +120,35 @@ def test_low_level_ops_refuse_a_gate_that_does_not_fit(ops):
             ops.residual_norm_bwd(x, x, gate, *rest, groups, 0, 1e-3, stats, x, x, [True] * 8)
     out, u, _ = ops.residual_norm_fwd(none, none, none, *rest, 1, 0, 1e-3, True)        # no rows at all: nothing to do
     assert out.shape == (0, 8) and u.shape == (0, 8)
+
+
+@pytest.mark.gpu
+def test_many_groups_captured_and_on_another_stream(ops):
+    """A backward pass of many groups keeps nothing between calls: captured, it is replayed on new inputs between eager calls, and gives their bits."""
+    m, n, groups = 16386, 101, 8193
+    g = torch.Generator(device="cuda").manual_seed(6)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    t = [r(m, n), r(m, n), r(groups, n), *(r(n) for _ in range(5))]
+    dO, dU = r(m, n), r(m, n)
+
+    def step():
+        stats = ops.residual_norm_fwd(*t, groups, 0, 1e-3, True)[2]
+        return ops.residual_norm_bwd(*t, groups, 0, 1e-3, stats, dO, dU, [True] * 8)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(warm, step()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for _ in range(3):
+        t[0].copy_(r(m, n))
+        t[2].copy_(r(groups, n))
+        eager = [v.clone() for v in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager))
